@@ -1,0 +1,107 @@
+// Dropout whose mask is drawn from a counter and never stored.
+//
+//   y[i] = kept(i) ? x[i] * f : 0,   f = 65536 / (65536 - t),   t = round(p * 65536)
+//
+// kept(i) depends on (seed, offset, i) alone, so the gradient is the same call on the incoming gradient: nothing but
+// the 16-byte state is saved for the backward pass.  What is dropped is written as zero without being looked at (a NaN
+// or an infinity there leaves no trace).  One read and one write of the tensor, the floor of the operation.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "philox.cuh"
+
+namespace atb {
+
+template <class T> __device__ __forceinline__ float drop_load(T v);
+template <> __device__ __forceinline__ float drop_load<float>(float v) { return v; }
+template <> __device__ __forceinline__ float drop_load<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float drop_load<__half>(__half v) { return __half2float(v); }
+template <class T> __device__ __forceinline__ T drop_store(float v);
+template <> __device__ __forceinline__ float drop_store<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 drop_store<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half drop_store<__half>(float v) { return __float2half_rn(v); }
+
+template <class T> struct alignas(16) Eight { T v[8]; };
+
+template <class T>
+__device__ __forceinline__ Eight<T> eight_load(const T* p)
+{
+    Eight<T> e;
+    const uint4* src = reinterpret_cast<const uint4*>(p);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(e) / 16); ++i) reinterpret_cast<uint4*>(&e)[i] = __ldcs(src + i);
+    return e;
+}
+
+// One thread takes whole groups of 8 elements (one draw each).  VEC: 16-byte aligned tensors.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) dropout_kernel(const T* x, T* y, long long numel, DropState d, float factor)
+{
+    const PhiloxKey key(d.rng);
+    const long long groups = (numel + 7) >> 3, stride = static_cast<long long>(gridDim.x) * blockDim.x;
+    for (long long g = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; g < groups; g += stride) {
+        const long long i0 = g << 3;
+        if (VEC && i0 + 8 <= numel) {
+            Eight<T> e = eight_load(x + i0);
+            const unsigned m = philox_keep8(key, g, d.threshold);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e.v[j] = drop_store<T>((m >> j) & 1u ? drop_load(e.v[j]) * factor : 0.0f);
+            uint4* dst = reinterpret_cast<uint4*>(y + i0);
+#pragma unroll
+            for (int j = 0; j < static_cast<int>(sizeof(e) / 16); ++j) dst[j] = reinterpret_cast<const uint4*>(&e)[j];
+        } else {
+            const unsigned m = philox_keep8(key, g, d.threshold);
+            for (int j = 0; j < 8 && i0 + j < numel; ++j)
+                y[i0 + j] = drop_store<T>((m >> j) & 1u ? drop_load(x[i0 + j]) * factor : 0.0f);
+        }
+    }
+}
+
+// state = {seed, offset}: `taken` gets the state that this call draws from, the offset moves on by one.  On the device,
+// so that every replay of a captured graph draws anew.
+__global__ void drop_advance_kernel(unsigned long long* __restrict__ state, unsigned long long* __restrict__ taken)
+{
+    const unsigned long long seed = state[0], off = state[1];
+    taken[0] = seed;
+    taken[1] = off;
+    state[1] = off + 1;
+}
+
+template <class T>
+static void launch_dropout(const void* x, void* y, long long numel, const DropState& d, float factor, cudaStream_t s)
+{
+    const bool vec = aligned_to(x, 16) && aligned_to(y, 16);
+    const int grid = grid_for((numel + 7) / 8, 256, 16 * sm_count());
+    if (vec) dropout_kernel<T, true><<<grid, 256, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
+    else dropout_kernel<T, false><<<grid, 256, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
+}
+
+}  // namespace atb
+
+using namespace atb;
+
+extern "C" int atb_dropout(const void* x, void* y, int dtype, long long numel, int threshold, const void* rng, void* stream)
+{
+    ATB_REQUIRE(numel >= 0, "negative numel");
+    ATB_REQUIRE(threshold >= 0 && threshold <= 65536, "threshold must lie in [0, 65536]");
+    if (numel == 0) return ATB_OK;
+    ATB_REQUIRE(x && y && rng, "null pointer");
+    ATB_REQUIRE(aligned_to(rng, 8), "rng must be 8-byte aligned");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const DropState d{static_cast<const unsigned long long*>(rng), static_cast<unsigned>(threshold)};
+    const float factor = threshold == 65536 ? 0.0f : static_cast<float>(65536.0 / (65536 - threshold));
+    if (dtype == ATB_F32) launch_dropout<float>(x, y, numel, d, factor, s);
+    else if (dtype == ATB_BF16) launch_dropout<__nv_bfloat16>(x, y, numel, d, factor, s);
+    else if (dtype == ATB_F16) launch_dropout<__half>(x, y, numel, d, factor, s);
+    else return fail_invalid("dtype must be fp32, bf16 or fp16");
+    return check_launch("dropout_kernel");
+}
+
+extern "C" int atb_dropout_advance(void* state, void* taken, void* stream)
+{
+    ATB_REQUIRE(state && taken && aligned_to(state, 8) && aligned_to(taken, 8), "state and taken must be 8-byte aligned device pointers");
+    drop_advance_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<unsigned long long*>(state),
+                                                                       static_cast<unsigned long long*>(taken));
+    return check_launch("drop_advance_kernel");
+}

@@ -1,0 +1,62 @@
+"""Dropout whose mask is drawn from a counter-based generator and never stored.
+
+The reference has no dropout of its own; its models use torch's, which keeps a mask (or a generator's state) for the
+backward pass.  Here element i is kept or not by (seed, offset, i) alone, so the backward pass draws the same mask again,
+and ``gemm_fp8.linear_fp8`` applies it inside its quantiser and its gradient product without a pass of its own.
+"""
+
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+from torch.autograd import Function
+
+from ..backend import ops as _ops
+
+
+class _counter_dropout(Function):
+
+    @staticmethod
+    def forward(ctx, x, p, rng):
+        ctx.p = p
+        ctx.save_for_backward(rng)
+        return _ops.dropout(x, p, rng)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        rng, = ctx.saved_tensors
+        return _ops.dropout(grad_output, ctx.p, rng), None, None
+
+
+def counter_dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tensor:
+    """x / (1 - p) where kept, 0 elsewhere, with gradient.  ``rng``: int64 {seed, offset} on x's device; it is read again in
+    the backward pass, so pass a state that stays as it is (``backend.ops.dropout_advance`` hands one out)."""
+    return _counter_dropout.apply(x, p, rng)
+
+
+def new_state(seed: int | None) -> torch.Tensor:
+    """{seed, 0}; without a seed, one from torch's default generator."""
+    if seed is None:
+        seed = int(torch.randint(2 ** 62, ()))
+    return torch.tensor([seed, 0], dtype=torch.int64)
+
+
+class CounterDropout(nn.Module):
+    """Dropout layer on ``counter_dropout``.  Its state {seed, offset} is a buffer: it moves on by one on the device with
+    every training forward (also in replays of a captured graph), is saved in checkpoints, and decides the masks, so a
+    resumed run draws what the interrupted one would have drawn.  Give every rank its own seed."""
+
+    def __init__(self, p: float = 0.5, seed: int | None = None):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"dropout probability must be between 0 and 1, got {p}")
+        self.p = p
+        self.register_buffer('rng', new_state(seed))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if not self.training or self.p == 0.0:
+            return x
+        return counter_dropout(x, self.p, _ops.dropout_advance(self.rng))
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}"

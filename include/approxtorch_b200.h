@@ -34,6 +34,11 @@ extern "C" {
 #define ATB_F32 0
 #define ATB_I8 1
 #define ATB_U8 2
+/* further element types of the 8-bit floating point operators and of dropout */
+#define ATB_BF16 3
+#define ATB_F16 4
+#define ATB_E4M3 5
+#define ATB_E5M2 6
 
 const char* atb_last_error(void);
 int atb_version(void);
@@ -286,6 +291,41 @@ int atb_lut_dwconv_bwd(const float* go, const void* x, int dtype, const uint8_t*
                        const float* dx, const float* dw_tab, const float* go_scale, float* grad_x, float* grad_w,
                        int N, int C, int H, int W, int kh, int kw, int sh, int sw, int ph, int pw,
                        int dh, int dw, int pad_index, void* stream);
+
+/* ---- 8-bit floating point with a scale for each block of 128 (no counterpart in the reference) -----------
+ * A block is 128 consecutive elements of a row (block_rows 1) or 128 x 128 (block_rows 128).  Its scale is the power of
+ * two 2^(byte - 127), stored as that byte; its elements are e4m3 or e5m2 numbers (f8: ATB_E4M3 / ATB_E5M2).
+ *
+ * Quantise x [R, C] (fp32 / bf16 / fp16, row pitch ldx elements): byte = the smallest in 1..254 with
+ * max|x| <= F 2^(byte - 127), F = 448 or 57344; q = x / scale rounded to nearest even.  A block with a NaN or an infinity
+ * gets byte 255 (NaN) and NaN everywhere.
+ *   q  [R, C], row pitch ldq (a multiple of 16, base 16-byte aligned; the pitch's padding may be written)
+ *   s  [R or ceil(R/128), ceil(C/128)], row pitch lds
+ *   qt [C, R], st [C or ceil(C/128), ceil(R/128)]: x transposed, quantised in blocks along R; both or neither
+ * drop_threshold > 0: x is dropped out first, as atb_dropout does on the contiguous [R, C] tensor, but without its factor
+ * (block_rows 1 only). */
+int atb_fp8_quantize(const void* x, int x_dtype, long long R, long long C, long long ldx, int f8, int block_rows,
+                     void* q, long long ldq, uint8_t* s, long long lds, void* qt, long long ldqt, uint8_t* st,
+                     long long ldst, int drop_threshold, const void* rng, void* stream);
+/* y[m, n] = alpha * sum_k A[m, k] B[n, k] (scales applied) + bias[n], summed in fp32, rounded once to y_dtype
+ * (fp32 / bf16 / fp16); A [M, K], B [N, K].  Row pitches lda, ldb: multiples of 16, bases 16-byte aligned; ldsa, ldsb:
+ * multiples of 4, bases 4-byte aligned, and every scale row readable up to a multiple of 4 bytes.  bias fp32 or NULL.
+ * drop_threshold > 0: elements of y that atb_dropout would drop from the contiguous [M, N] tensor become 0 (no factor). */
+int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_t* sa, long long ldsa, int a_block_rows,
+                 const void* b, int b_f8, long long ldb, const uint8_t* sb, long long ldsb, int b_block_rows,
+                 const float* bias, float alpha, void* y, int y_dtype, long long ldy, int M, int N, int K,
+                 int drop_threshold, const void* rng, void* stream);
+/* Device-side error word of the product (host pointer out; synchronises): 1 = a block gave up waiting for its operands
+ * and left tiles unwritten. */
+int atb_fp8_status(int* status /*host*/);
+
+/* ---- counter-based dropout (no counterpart in the reference) ----------------------------------------------
+ * y[i] = kept(i) ? x[i] * 65536 / (65536 - threshold) : 0.  kept(i): the 16 bits of element i drawn by Philox4x32-10
+ * (key = seed, counter = (i / 8, offset), low halves first) are >= threshold.  rng: device {seed, offset}, 2 x 64 bits.
+ * The gradient is the same call on the incoming gradient.  x == y is allowed. */
+int atb_dropout(const void* x, void* y, int dtype, long long numel, int threshold, const void* rng, void* stream);
+/* taken = state; state.offset += 1 (on the device, so that replays of a captured graph draw anew). */
+int atb_dropout_advance(void* state, void* taken, void* stream);
 
 /* ---- measurement aid (no counterpart in the reference) ---------------------------------------------
  * Launches `blocks` blocks of 1024 threads that each issue iters x 8 conflict-free 8-byte shared-memory loads

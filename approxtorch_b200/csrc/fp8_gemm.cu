@@ -8,14 +8,21 @@
 // consecutive instructions read the same byte.  So the product runs at the rate of an unscaled 8-bit product; promoting
 // every 128-step partial sum through registers instead would cost a read of the accumulator per 128 steps.
 //
-// One block of threads per SM walks over the output tiles:
+// fp8_gemm_kernel, for products of many tiles: one block of threads per SM (CG = 1), or two blocks on two SMs that work on
+// one tile of 256 rows (CG = 2), walk over the output tiles:
 //   warp 0      one thread requests the operand tiles by TMA (128-byte swizzle, one 128-step slice = one 128-byte row);
-//   warp 1      one thread moves the scales to tensor memory (tcgen05.cp) and issues the MMAs;
+//   warp 1      one thread moves the scales to tensor memory (tcgen05.cp) and issues the MMAs (of the pair: the first
+//               block's thread, for both);
 //   warp 2      gathers the scale bytes of four slices at a time (one 32-bit word per row) into the order in which
 //               tcgen05.cp wants them: 32 rows of 16 bytes, word j of row i = operand row i + 32 j;
 //   warp 3      owns the tensor-memory allocation;
-//   warps 4-7   read finished accumulators, scale, add the bias and store.
-// Two accumulators let the epilogue of a tile run under the MMAs of the next.
+//   warps 4-7   read finished accumulators, scale, add the bias and store, 32 x 32 elements at a time through shared
+//               memory so that a row's bytes leave together.
+// Two accumulators let the epilogue of a tile run under the MMAs of the next.  Why pairs: each block of a pair holds its
+// own 128 rows of A and half the rows of B and the tensor core reads both halves, so a slice of a 256 x 224 tile costs
+// each SM 30 KB instead of the 44 KB of a 128 x 224 tile, and what bounds the product is the path from L2 to the SMs.
+//
+// fp8_split_kernel, for products of few tiles (serving, small heads): see there.
 //
 // Operand rows beyond M or N and steps beyond K are zeros that TMA fills in; scale bytes beyond the last block are
 // never selected, and rows beyond the last get 1.
@@ -31,10 +38,11 @@ namespace atb {
 __device__ int g_fp8_status = 0;                      // 1: a block gave up waiting
 
 constexpr int kF8Threads = 256, kF8EpiWarp = 4;
-constexpr int kF8TileM = 128, kF8MaxTileN = 240;
+constexpr int kF8TileM = 128, kF8MaxTileN = 224;          // of one block; a pair's tile has twice the rows
 constexpr int kF8SfSlots = 4, kF8SfSlotBytes = 3 * 512;   // 128 rows of A, up to 256 rows of B
 constexpr int kF8SfCol = 488, kF8SfCols = 12;             // tensor-memory columns of the two scale buffers
-constexpr int kF8Smem = 220 * 1024;
+constexpr int kF8Smem = 224 * 1024, kF8MaxStages = 8;
+constexpr int kF8Group = 8;                               // row tiles that are walked together (their operands meet in L2)
 
 struct Fp8Params {
     const uint8_t* sa;
@@ -48,7 +56,7 @@ struct Fp8Params {
     int M, N, kblocks;
     int tile_n, mt, nt, stages;
     uint32_t idesc;
-    bool vec;
+    bool vec;                            // rows of y start on 16-byte boundaries
     DropState drop;
 };
 
@@ -70,7 +78,7 @@ __device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, volatile 
 {
     for (int i = 0; i < (1 << 21); ++i) {
         uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
         if ((i & 63) == 63 && *abort_flag) return false;
@@ -78,10 +86,31 @@ __device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, volatile 
     *abort_flag = 1;
     return false;
 }
+// the same shared address in the first block of the pair
+__device__ __forceinline__ uint32_t f8_leader(uint32_t addr)
+{
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ void f8_arrive_cluster(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void f8_cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// CG = 2: the bytes land here, the barrier may be the other block's
+template <int CG>
 __device__ __forceinline__ void f8_tma(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
 {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+    if (CG == 1)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 // K-major operand with 128-byte swizzle: 8-row atoms 1024 bytes apart
 __device__ __forceinline__ uint64_t f8_desc(uint32_t saddr)
@@ -95,20 +124,34 @@ __device__ __forceinline__ uint64_t f8_sf_desc(uint32_t saddr)
     return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(1) << 16) |
            (static_cast<uint64_t>(128 >> 4) << 32) | (static_cast<uint64_t>(1) << 46);
 }
+template <int CG>
 __device__ __forceinline__ void f8_copy_scales(uint32_t tmem, uint64_t desc)
 {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    if (CG == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
+template <int CG>
 __device__ __forceinline__ void f8_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate)
 {
     const uint32_t acc = accumulate ? 1u : 0u;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                 ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
+    if (CG == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
 }
+// arrives at the barrier when the MMAs issued so far are done; CG = 2: at the same barrier of both blocks
+template <int CG>
 __device__ __forceinline__ void f8_commit(uint32_t bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if (CG == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
 }
 __device__ __forceinline__ void f8_tmem_ld32(uint32_t (&v)[32], uint32_t addr)
 {
@@ -126,67 +169,89 @@ template <> __device__ __forceinline__ float f8_out<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 f8_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half f8_out<__half>(float v) { return __float2half_rn(v); }
 
-template <class T>
+// row and column tile of the t-th output tile: kF8Group row tiles at a time, column by column
+__device__ __forceinline__ void f8_tile(int t, int mt, int nt, int& tm, int& tn)
+{
+    const int per = kF8Group * nt, g = t / per, rows = min(kF8Group, mt - g * kF8Group), in = t - g * per;
+    tn = in / rows;
+    tm = g * kF8Group + (in - tn * rows);
+}
+
+template <class T, int CG>
 __global__ void __launch_bounds__(kF8Threads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp8Params p)
 {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    __shared__ __align__(8) uint64_t s_full[8], s_empty[8], s_sf_full[kF8SfSlots], s_sf_empty[kF8SfSlots], s_acc_full[2], s_acc_empty[2];
+    __shared__ __align__(8) uint64_t s_full[kF8MaxStages], s_empty[kF8MaxStages], s_sf_full[kF8SfSlots], s_sf_empty[kF8SfSlots], s_acc_full[2], s_acc_empty[2];
+    constexpr int kPitch = 32 * sizeof(T) + 16;              // of a staged row: 16-byte accesses without bank conflicts
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = CG == 2 ? static_cast<int>(blockIdx.x & 1u) : 0;
+    const int first = blockIdx.x / CG, step = gridDim.x / CG;
     const uint32_t smem0 = (f8_smem(smem_raw) + 1023u) & ~1023u;
-    const uint32_t stage_bytes = kF8TileM * 128 + p.tile_n * 128;
-    const uint32_t sf0 = smem0 + p.stages * stage_bytes;
+    const int b_rows = p.tile_n / CG;                        // rows of B that this block holds
+    const uint32_t stage_bytes = kF8TileM * 128 + b_rows * 128;
+    const uint32_t sf0 = smem0 + p.stages * stage_bytes, stage0 = sf0 + kF8SfSlots * kF8SfSlotBytes;
     const uint32_t full0 = f8_smem(s_full), empty0 = f8_smem(s_empty), sff0 = f8_smem(s_sf_full), sfe0 = f8_smem(s_sf_empty);
     const uint32_t accf0 = f8_smem(s_acc_full), acce0 = f8_smem(s_acc_empty);
     volatile int* abort_flag = &s_abort;
     if (tid == 0) {
         s_abort = 0;
-        for (int s = 0; s < 8; ++s) { f8_bar_init(full0 + 8 * s, 1); f8_bar_init(empty0 + 8 * s, 1); }
-        for (int s = 0; s < kF8SfSlots; ++s) { f8_bar_init(sff0 + 8 * s, 1); f8_bar_init(sfe0 + 8 * s, 1); }
-        for (int s = 0; s < 2; ++s) { f8_bar_init(accf0 + 8 * s, 1); f8_bar_init(acce0 + 8 * s, 4); }
+        for (int s = 0; s < kF8MaxStages; ++s) { f8_bar_init(full0 + 8 * s, 1); f8_bar_init(empty0 + 8 * s, 1); }
+        for (int s = 0; s < kF8SfSlots; ++s) { f8_bar_init(sff0 + 8 * s, CG); f8_bar_init(sfe0 + 8 * s, 1); }
+        for (int s = 0; s < 2; ++s) { f8_bar_init(accf0 + 8 * s, 1); f8_bar_init(acce0 + 8 * s, 4 * CG); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (CG == 2) f8_cluster_sync();
     if (warp == 3) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(f8_smem(&s_tmem)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(f8_smem(&s_tmem)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(f8_smem(&s_tmem)) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    if (CG == 2) f8_cluster_sync(); else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
     const int ntiles = p.mt * p.nt, kb_n = p.kblocks, quads = (kb_n + 3) >> 2;
 
     if (warp == 0) {
         if (lane == 0) {
-            uint32_t it = 0;
+            uint32_t s = 0, parity = 1, issued = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
-                const int m0 = (t % p.mt) * kF8TileM, n0 = (t / p.mt) * p.tile_n;
-                for (int kb = 0; kb < kb_n; ++kb, ++it) {
-                    const uint32_t s = it % p.stages;
-                    if (!(ok = f8_wait(empty0 + 8 * s, ((it / p.stages) & 1u) ^ 1u, abort_flag))) break;
-                    f8_expect(full0 + 8 * s, stage_bytes);
-                    f8_tma(smem0 + s * stage_bytes, &map_a, kb * 128, m0, full0 + 8 * s);
-                    f8_tma(smem0 + s * stage_bytes + kF8TileM * 128, &map_b, kb * 128, n0, full0 + 8 * s);
+            for (int t = first; t < ntiles && ok; t += step) {
+                int tm, tn;
+                f8_tile(t, p.mt, p.nt, tm, tn);
+                const int m0 = (tm * CG + rank) * kF8TileM, n0 = tn * p.tile_n + rank * b_rows;
+                for (int kb = 0; kb < kb_n; ++kb, ++issued) {
+                    if (!(ok = f8_wait(empty0 + 8 * s, parity, abort_flag))) break;
+                    if (rank == 0) f8_expect(full0 + 8 * s, CG * stage_bytes);
+                    const uint32_t bar = CG == 2 ? f8_leader(full0 + 8 * s) : full0 + 8 * s;
+                    f8_tma<CG>(smem0 + s * stage_bytes, &map_a, kb * 128, m0, bar);
+                    f8_tma<CG>(smem0 + s * stage_bytes + kF8TileM * 128, &map_b, kb * 128, n0, bar);
+                    if (++s == static_cast<uint32_t>(p.stages)) { s = 0; parity ^= 1u; }
                 }
             }
             // nothing may be in flight when the block ends (all of it has landed unless a role gave up)
-            for (uint32_t j = it > static_cast<uint32_t>(p.stages) ? it - p.stages : 0; j < it; ++j) {
-                int never = 0;
-                f8_wait(full0 + 8 * (j % p.stages), (j / p.stages) & 1u, &never);
-            }
+            if (rank == 0)
+                for (uint32_t j = issued > static_cast<uint32_t>(p.stages) ? issued - p.stages : 0; j < issued; ++j) {
+                    int never = 0;
+                    f8_wait(full0 + 8 * (j % p.stages), (j / p.stages) & 1u, &never);
+                }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            uint32_t it = 0, quad = 0, tile = 0;
+        if (lane == 0 && rank == 0) {
+            uint32_t s = 0, parity = 0, quad = 0, tile = 0;
             bool ok = true;
-            for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++tile) {
+            for (int t = first; t < ntiles && ok; t += step, ++tile) {
                 const uint32_t buf = tile & 1u, d = tmem + buf * p.tile_n;
                 if (!(ok = f8_wait(acce0 + 8 * buf, ((tile >> 1) & 1u) ^ 1u, abort_flag))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int kb = 0; kb < kb_n; ++kb, ++it) {
+                for (int kb = 0; kb < kb_n; ++kb) {
                     const uint32_t sfa = tmem + kF8SfCol + (quad & 1u) * kF8SfCols, sfb = sfa + 4;
                     if ((kb & 3) == 0) {
                         const uint32_t slot = quad % kF8SfSlots;
@@ -195,28 +260,30 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                         if (!(ok = f8_wait(sff0 + 8 * slot, (quad / kF8SfSlots) & 1u, abort_flag))) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint32_t src = sf0 + slot * kF8SfSlotBytes;
-                        f8_copy_scales(sfa, f8_sf_desc(src));
-                        f8_copy_scales(sfb, f8_sf_desc(src + 512));
-                        if (p.tile_n > 128) f8_copy_scales(sfb + 4, f8_sf_desc(src + 1024));
+                        f8_copy_scales<CG>(sfa, f8_sf_desc(src));
+                        f8_copy_scales<CG>(sfb, f8_sf_desc(src + 512));
+                        if (p.tile_n > 128) f8_copy_scales<CG>(sfb + 4, f8_sf_desc(src + 1024));
                     }
-                    const uint32_t s = it % p.stages;
-                    if (!(ok = f8_wait(full0 + 8 * s, (it / p.stages) & 1u, abort_flag))) break;
+                    if (!(ok = f8_wait(full0 + 8 * s, parity, abort_flag))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t da = f8_desc(smem0 + s * stage_bytes), db = f8_desc(smem0 + s * stage_bytes + kF8TileM * 128);
                     const uint32_t idesc = p.idesc | (static_cast<uint32_t>(kb & 3) << 29) | (static_cast<uint32_t>(kb & 3) << 4);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) f8_mma(d, da + 2 * j, db + 2 * j, idesc, sfa, sfb, kb > 0 || j > 0);
-                    f8_commit(empty0 + 8 * s);
-                    if ((kb & 3) == 3 || kb == kb_n - 1) { f8_commit(sfe0 + 8 * (quad % kF8SfSlots)); ++quad; }
+                    for (int j = 0; j < 4; ++j) f8_mma<CG>(d, da + 2 * j, db + 2 * j, idesc, sfa, sfb, kb > 0 || j > 0);
+                    f8_commit<CG>(empty0 + 8 * s);
+                    if ((kb & 3) == 3 || kb == kb_n - 1) { f8_commit<CG>(sfe0 + 8 * (quad % kF8SfSlots)); ++quad; }
+                    if (++s == static_cast<uint32_t>(p.stages)) { s = 0; parity ^= 1u; }
                 }
-                if (ok) f8_commit(accf0 + 8 * buf);
+                if (ok) f8_commit<CG>(accf0 + 8 * buf);
             }
         }
     } else if (warp == 2) {
         uint32_t quad = 0;
         bool ok = true;
-        for (int t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
-            const int m0 = (t % p.mt) * kF8TileM, n0 = (t / p.mt) * p.tile_n;
+        for (int t = first; t < ntiles && ok; t += step) {
+            int tm, tn;
+            f8_tile(t, p.mt, p.nt, tm, tn);
+            const int m0 = (tm * CG + rank) * kF8TileM, n0 = tn * p.tile_n;
             for (int q = 0; q < quads; ++q, ++quad) {
                 const uint32_t slot = quad % kF8SfSlots, dst = sf0 + slot * kF8SfSlotBytes + lane * 16;
                 uint32_t w[12];
@@ -236,26 +303,31 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                                  "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) f8_arrive(sff0 + 8 * slot);
+                if (lane == 0) {
+                    if (CG == 2) f8_arrive_cluster(f8_leader(sff0 + 8 * slot)); else f8_arrive(sff0 + 8 * slot);
+                }
             }
         }
     } else if (warp >= kF8EpiWarp) {
-        const int row_in_tile = (warp & 3) * 32 + lane;
+        const int row0 = (warp & 3) * 32;
+        uint8_t* const stage = smem_raw + (stage0 - f8_smem(smem_raw)) + (warp & 3) * 32 * kPitch;
         uint32_t tile = 0;
         T* const y = static_cast<T*>(p.y);
-        for (int t = blockIdx.x; t < ntiles; t += gridDim.x, ++tile) {
-            const int m = (t % p.mt) * kF8TileM + row_in_tile, n0 = (t / p.mt) * p.tile_n;
+        for (int t = first; t < ntiles; t += step, ++tile) {
+            int tm, tn;
+            f8_tile(t, p.mt, p.nt, tm, tn);
+            const int m0 = (tm * CG + rank) * kF8TileM + row0, n0 = tn * p.tile_n;
             const uint32_t buf = tile & 1u;
             if (!f8_wait(accf0 + 8 * buf, (tile >> 1) & 1u, abort_flag)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t src = tmem + buf * p.tile_n + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+            const uint32_t src = tmem + buf * p.tile_n + (static_cast<uint32_t>(row0) << 16);
+            const int rows = min(32, p.M - m0);
             for (int c = 0; c < p.tile_n; c += 32) {
                 const int n = n0 + c;
-                if (n >= p.N) break;                         // the same for the whole warp
+                if (n >= p.N || rows <= 0) break;            // the same for the whole warp
                 uint32_t v[32];
                 f8_tmem_ld32(v, src + c);
-                if (m >= p.M) continue;
-                const int cols = min(min(32, p.N - n), p.tile_n - c);
+                const int cols = min(32, p.N - n);
                 T out[32];
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
@@ -267,37 +339,51 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     const PhiloxKey key(p.drop.rng);
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        const unsigned keep = philox_keep8_at(key, static_cast<unsigned long long>(m) * p.N + n + 8 * g, p.drop.threshold);
+                        const unsigned keep = philox_keep8_at(key, static_cast<unsigned long long>(m0 + lane) * p.N + n + 8 * g, p.drop.threshold);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) if (!((keep >> j) & 1u)) out[8 * g + j] = f8_out<T>(0.0f);
                     }
                 }
-                T* dst = y + static_cast<long long>(m) * p.ldy + n;
-                constexpr int kPer = 16 / sizeof(T);
+                constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer;       // of a 32-element row
+                __syncwarp();                                                   // the last chunk's readers are through
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) {
+                    uint4 pack;
+                    T* e = reinterpret_cast<T*>(&pack);
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) e[i] = out[j * kPer + i];
+                    *reinterpret_cast<uint4*>(stage + lane * kPitch + 16 * j) = pack;
+                }
+                __syncwarp();
                 if (p.vec && cols == 32) {
+                    const int piece = lane % kPieces;
 #pragma unroll
-                    for (int j = 0; j < 32 / kPer; ++j) {
-                        uint4 pack;
-                        T* e = reinterpret_cast<T*>(&pack);
-#pragma unroll
-                        for (int i = 0; i < kPer; ++i) e[i] = out[j * kPer + i];
-                        reinterpret_cast<uint4*>(dst)[j] = pack;
+                    for (int i = 0; i < kPieces; ++i) {
+                        const int r = lane / kPieces + i * (32 / kPieces);
+                        if (r < rows)
+                            *reinterpret_cast<uint4*>(y + static_cast<long long>(m0 + r) * p.ldy + n + piece * kPer) =
+                                *reinterpret_cast<const uint4*>(stage + r * kPitch + 16 * piece);
                     }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) if (j < cols) dst[j] = out[j];
+                } else if (lane < cols) {
+                    for (int r = 0; r < rows; ++r)
+                        y[static_cast<long long>(m0 + r) * p.ldy + n + lane] = *reinterpret_cast<const T*>(stage + r * kPitch + lane * sizeof(T));
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) f8_arrive(acce0 + 8 * buf);
+            if (lane == 0) {
+                if (CG == 2) f8_arrive_cluster(f8_leader(acce0 + 8 * buf)); else f8_arrive(acce0 + 8 * buf);
+            }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    if (CG == 2) f8_cluster_sync(); else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (tid == 0 && s_abort) g_fp8_status = 1;
-    if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 3) {
+        if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
 }
 
 // y = bias (a product over nothing)
@@ -344,14 +430,31 @@ static int operand_map(CUtensorMap* map, const void* base, long long R, long lon
     return ATB_OK;
 }
 
-template <class T>
+template <class T, int CG>
 static int launch_fp8(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Params& p, cudaStream_t s)
 {
-    cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
-    if (e != cudaSuccess) { set_error("cudaFuncSetAttribute: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
-    const int tiles = p.mt * p.nt, grid = tiles < sm_count() ? tiles : sm_count();
-    fp8_gemm_kernel<T><<<grid, kF8Threads, kF8Smem, s>>>(ma, mb, p);
+    cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<T, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
+    const int tiles = p.mt * p.nt, fit = sm_count() / CG;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(CG * (tiles < fit ? tiles : fit));
+    cfg.blockDim = dim3(kF8Threads);
+    cfg.dynamicSmemBytes = kF8Smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = CG;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = CG == 2 ? 1 : 0;
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<T, CG>, ma, mb, p);
+    if (e != cudaSuccess) { set_error("fp8_gemm_kernel: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
     return check_launch("fp8_gemm_kernel");
+}
+
+template <class T>
+static int launch_fp8_cg(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Params& p, int cg, cudaStream_t s)
+{
+    return cg == 2 ? launch_fp8<T, 2>(ma, mb, p, s) : launch_fp8<T, 1>(ma, mb, p, s);
 }
 
 template <class T>
@@ -398,25 +501,26 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     p.sa = sa; p.sb = sb; p.ldsa = ldsa; p.ldsb = ldsb;
     p.a_shift = a_block_rows == 128 ? 7 : 0; p.b_shift = b_block_rows == 128 ? 7 : 0;
     p.bias = bias; p.alpha = alpha; p.y = y; p.ldy = ldy; p.M = M; p.N = N; p.kblocks = kblocks;
-    p.tile_n = N >= 192 ? 192 : ((N + 31) / 32) * 32;
-    p.mt = (M + kF8TileM - 1) / kF8TileM;
+    const int cg = M > kF8TileM ? 2 : 1;
+    p.tile_n = N >= kF8MaxTileN ? kF8MaxTileN : ((N + 31) / 32) * 32;
+    p.mt = (M + cg * kF8TileM - 1) / (cg * kF8TileM);
     p.nt = (N + p.tile_n - 1) / p.tile_n;
     ATB_REQUIRE(static_cast<long long>(p.mt) * p.nt < (1LL << 30), "too many tiles");
-    const int stage = kF8TileM * 128 + p.tile_n * 128;
-    p.stages = (kF8Smem - 1024 - kF8SfSlots * kF8SfSlotBytes) / stage;
-    if (p.stages > 8) p.stages = 8;
+    const int stage = kF8TileM * 128 + p.tile_n / cg * 128;
+    p.stages = (kF8Smem - 1024 - kF8SfSlots * kF8SfSlotBytes - 4 * 32 * (32 * size + 16)) / stage;
+    if (p.stages > kF8MaxStages) p.stages = kF8MaxStages;
     p.idesc = (a_f8 == ATB_E5M2 ? 1u << 7 : 0u) | (b_f8 == ATB_E5M2 ? 1u << 10 : 0u) |
-              (static_cast<uint32_t>(p.tile_n >> 3) << 17) | (1u << 23) | (1u << 27);
+              (static_cast<uint32_t>(p.tile_n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(cg) << 27);
     p.vec = aligned_to(y, 16) && (ldy * size) % 16 == 0;
     p.drop = DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)};
 
     CUtensorMap ma, mb;
     int rc = operand_map(&ma, a, M, K, lda, kF8TileM);
-    if (rc == ATB_OK) rc = operand_map(&mb, b, N, K, ldb, p.tile_n);
+    if (rc == ATB_OK) rc = operand_map(&mb, b, N, K, ldb, p.tile_n / cg);
     if (rc != ATB_OK) return rc;
-    if (y_dtype == ATB_F32) return launch_fp8<float>(ma, mb, p, s);
-    if (y_dtype == ATB_BF16) return launch_fp8<__nv_bfloat16>(ma, mb, p, s);
-    return launch_fp8<__half>(ma, mb, p, s);
+    if (y_dtype == ATB_F32) return launch_fp8_cg<float>(ma, mb, p, cg, s);
+    if (y_dtype == ATB_BF16) return launch_fp8_cg<__nv_bfloat16>(ma, mb, p, cg, s);
+    return launch_fp8_cg<__half>(ma, mb, p, cg, s);
 }
 
 extern "C" int atb_fp8_status(int* status)

@@ -512,11 +512,11 @@ def _fp8_quantize(x: Tensor, dtype: torch.dtype, block_rows: int, transposed: bo
     nb, nbt = -(-C // 128), -(-R // 128)
     e8 = torch.float8_e8m0fnu
     q = _padded(R, C, 16, dtype, dev)
-    s = _padded(R if block_rows == 1 else nbt, nb, 4, e8, dev)
+    s = _padded(R if block_rows == 1 else nbt, nb, 16, e8, dev)
     qt = st = None
     if transposed:
         qt = _padded(C, R, 16, dtype, dev)
-        st = _padded(C if block_rows == 1 else nb, nbt, 4, e8, dev)
+        st = _padded(C if block_rows == 1 else nb, nbt, 16, e8, dev)
     if R and C:
         _enqueue("atb_fp8_quantize", dev, x.data_ptr(), _FLOAT_CODE[x.dtype], R, C, x.stride(0) if R > 1 else C,
                  _F8_CODE[dtype], block_rows, q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0),
@@ -579,11 +579,13 @@ def _fp8_operand(t: Tensor, scale: Tensor, name: str):
         t = _repacked(t, 16)
         ld = -(-K // 16) * 16
     rows = scale.shape[0]
-    width = -(-nb // 4) * 4
-    lds = scale.stride(0) if rows > 1 else width
+    lds = scale.stride(0) if rows > 1 else -(-nb // 4) * 4
+    # the kernel reads words, or 16 bytes at a time where base and pitch allow it
+    unit = 16 if lds % 16 == 0 and scale.data_ptr() % 16 == 0 else 4
+    width = -(-nb // unit) * unit
     if (nb > 1 and scale.stride(1) != 1) or lds % 4 or lds < nb or scale.data_ptr() % 4 or not _room(scale, lds, width):
-        scale = _repacked(scale, 4)
-        lds = width
+        scale = _repacked(scale, 16)
+        lds = -(-nb // 16) * 16
     return t, ld, scale, lds, 1 if rows == R else 128
 
 

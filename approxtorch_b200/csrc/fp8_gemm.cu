@@ -13,9 +13,9 @@
 //   warp 0      one thread requests the operand tiles by TMA (128-byte swizzle, one 128-step slice = one 128-byte row);
 //   warp 1      one thread moves the scales to tensor memory (tcgen05.cp) and issues the MMAs (of the pair: the first
 //               block's thread, for both);
-//   warp 2      gathers the scale bytes of four slices at a time (one 32-bit word per row) into the order in which
-//               tcgen05.cp wants them: 32 rows of 16 bytes, word j of row i = operand row i + 32 j;
-//   warp 3      owns the tensor-memory allocation;
+//   warps 2-3   gather the scale bytes, 16 slices at a time (one load per row), and hand them over four slices (a quad) at a
+//               time in the order in which tcgen05.cp wants them: 32 rows of 16 bytes, word j of row i = operand row
+//               i + 32 j (warp 3 also owns the tensor-memory allocation);
 //   warps 4-7   read finished accumulators, scale, add the bias and store, 32 x 32 elements at a time through shared
 //               memory so that a row's bytes leave together.
 // Two accumulators let the epilogue of a tile run under the MMAs of the next.  Why pairs: each block of a pair holds its
@@ -38,10 +38,10 @@ namespace atb {
 __device__ int g_fp8_status = 0;                      // 1: a block gave up waiting
 
 constexpr int kF8Threads = 256, kF8EpiWarp = 4;
-constexpr int kF8TileM = 128, kF8MaxTileN = 224;          // of one block; a pair's tile has twice the rows
-constexpr int kF8SfSlots = 4, kF8SfSlotBytes = 3 * 512;   // 128 rows of A, up to 256 rows of B
+constexpr int kF8TileM = 128, kF8MaxTileN = 256;          // of one block; a pair's tile has twice the rows
+constexpr int kF8SfSlots = 8, kF8SfSlotBytes = 3 * 512;   // a run of quads for each gathering warp; 128 rows of A, up to 256 of B
 constexpr int kF8SfCol = 488, kF8SfCols = 12;             // tensor-memory columns of the two scale buffers
-constexpr int kF8Smem = 224 * 1024, kF8MaxStages = 8;
+constexpr int kF8Smem = 226 * 1024, kF8MaxStages = 8;
 constexpr int kF8Group = 8;                               // row tiles that are walked together (their operands meet in L2)
 
 struct Fp8Params {
@@ -49,6 +49,7 @@ struct Fp8Params {
     const uint8_t* sb;
     long long ldsa, ldsb;
     int a_shift, b_shift;                // 0: a scale per row, 7: per 128 rows
+    bool sf_vec;                         // scale rows of both operands start on 16-byte boundaries
     const float* bias;
     float alpha;
     void* y;
@@ -73,18 +74,41 @@ __device__ __forceinline__ void f8_expect(uint32_t bar, uint32_t bytes)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// bounded wait that also gives up when another role of the block has
+// Bounded wait that also gives up when another role of the block has.  CLUSTER: the arrivals it waits for order another
+// block's writes (an acquire over the cluster costs far more than one over the block; only the hand-overs that need it
+// pay for it).
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag)
 {
-    for (int i = 0; i < (1 << 21); ++i) {
+    for (int i = 0; i < (1 << 18); ++i) {        // about a second
         uint32_t ok;
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (CLUSTER)
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        else
+            asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                         : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
         if ((i & 63) == 63 && *abort_flag) return false;
     }
     *abort_flag = 1;
     return false;
+}
+// one look at a barrier
+__device__ __forceinline__ bool f8_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
+// one lane of a converged warp.  (The roles below run as whole warps and issue under this predicate: a branch on the lane
+// number instead makes the compiler rebuild every descriptor operand lane by lane, and the MMA issue became the bound.)
+__device__ __forceinline__ bool f8_elect()
+{
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
 }
 // the same shared address in the first block of the pair
 __device__ __forceinline__ uint32_t f8_leader(uint32_t addr)
@@ -130,18 +154,19 @@ __device__ __forceinline__ void f8_copy_scales(uint32_t tmem, uint64_t desc)
     if (CG == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
     else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(desc) : "memory");
 }
+// one 32-step MMA; a_lo, b_lo: the low words of the operands' descriptors (f8_desc)
 template <int CG>
-__device__ __forceinline__ void f8_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate)
+__device__ __forceinline__ void f8_mma(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t sfa, uint32_t sfb, bool accumulate)
 {
-    const uint32_t acc = accumulate ? 1u : 0u;
+    const uint32_t acc = accumulate ? 1u : 0u, hi = static_cast<uint32_t>(f8_desc(0) >> 32);
     if (CG == 1)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                     ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %6, 0;\n\tmov.b64 da, {%1, %7};\n\tmov.b64 db, {%2, %7};\n\t"
+                     "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc), "r"(hi) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-                     "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-                     ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %6, 0;\n\tmov.b64 da, {%1, %7};\n\tmov.b64 db, {%2, %7};\n\t"
+                     "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], da, db, %3, [%4], [%5], p;\n\t}"
+                     ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc), "r"(hi) : "memory");
 }
 // arrives at the barrier when the MMAs issued so far are done; CG = 2: at the same barrier of both blocks
 template <int CG>
@@ -168,6 +193,65 @@ template <class T> __device__ __forceinline__ T f8_out(float v);
 template <> __device__ __forceinline__ float f8_out<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 f8_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half f8_out<__half>(float v) { return __float2half_rn(v); }
+template <class T> __device__ __forceinline__ uint32_t f8_pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t f8_pack2<__nv_bfloat16>(float a, float b)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t f8_pack2<__half>(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16 bytes of results to shared memory and back
+template <class T>
+__device__ __forceinline__ void f8_put16(uint32_t addr, const float* f)
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(f[i]);
+        else w[i] = f8_pack2<T>(f[2 * i], f[2 * i + 1]);
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+}
+__device__ __forceinline__ uint4 f8_get16(uint32_t addr)
+{
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+template <class T>
+__device__ __forceinline__ T f8_get(uint32_t addr)
+{
+    T r;
+    if constexpr (sizeof(T) == 4) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r) : "r"(addr) : "memory");
+    else {
+        uint16_t h;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr) : "memory");
+        r = *reinterpret_cast<T*>(&h);
+    }
+    return r;
+}
+// zeros where 32 consecutive elements are dropped.  Out of line: rare, and long enough to push the loop out of the
+// instruction cache.
+__device__ __noinline__ unsigned f8_keep8(const unsigned long long* rng, unsigned threshold, unsigned long long element)
+{
+    return philox_keep8_at(PhiloxKey(rng), element, threshold);
+}
+__device__ __forceinline__ void f8_mask32(const DropState& d, unsigned long long element, float (&f)[32])
+{
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const unsigned keep = f8_keep8(d.rng, d.threshold, element + 8 * g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[8 * g + j] = (keep >> j) & 1u ? f[8 * g + j] : 0.0f;
+    }
+}
+
+__device__ __forceinline__ uint32_t f8_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // row and column tile of the t-th output tile: kF8Group row tiles at a time, column by column
 __device__ __forceinline__ void f8_tile(int t, int mt, int nt, int& tm, int& tn)
@@ -184,9 +268,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    __shared__ __align__(8) uint64_t s_full[kF8MaxStages], s_empty[kF8MaxStages], s_sf_full[kF8SfSlots], s_sf_empty[kF8SfSlots], s_acc_full[2], s_acc_empty[2];
+    __shared__ __align__(8) uint64_t s_full[kF8MaxStages], s_empty[kF8MaxStages], s_sf_full[kF8SfSlots], s_sf_empty[kF8SfSlots], s_acc_full[2], s_acc_empty[2], s_acc_part;
     constexpr int kPitch = 32 * sizeof(T) + 16;              // of a staged row: 16-byte accesses without bank conflicts
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);  // the same for a warp, and the compiler knows it
     const int rank = CG == 2 ? static_cast<int>(blockIdx.x & 1u) : 0;
     const int first = blockIdx.x / CG, step = gridDim.x / CG;
     const uint32_t smem0 = (f8_smem(smem_raw) + 1023u) & ~1023u;
@@ -194,17 +279,55 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const uint32_t stage_bytes = kF8TileM * 128 + b_rows * 128;
     const uint32_t sf0 = smem0 + p.stages * stage_bytes, stage0 = sf0 + kF8SfSlots * kF8SfSlotBytes;
     const uint32_t full0 = f8_smem(s_full), empty0 = f8_smem(s_empty), sff0 = f8_smem(s_sf_full), sfe0 = f8_smem(s_sf_empty);
-    const uint32_t accf0 = f8_smem(s_acc_full), acce0 = f8_smem(s_acc_empty);
+    const uint32_t accf0 = f8_smem(s_acc_full), acce0 = f8_smem(s_acc_empty), accp = f8_smem(&s_acc_part);
+    const int ntiles = p.mt * p.nt, kb_n = p.kblocks, quads = (kb_n + 3) >> 2, runs = (kb_n + 15) >> 4;
     volatile int* abort_flag = &s_abort;
-    if (tid == 0) {
-        s_abort = 0;
-        for (int s = 0; s < kF8MaxStages; ++s) { f8_bar_init(full0 + 8 * s, 1); f8_bar_init(empty0 + 8 * s, 1); }
-        for (int s = 0; s < kF8SfSlots; ++s) { f8_bar_init(sff0 + 8 * s, CG); f8_bar_init(sfe0 + 8 * s, 1); }
-        for (int s = 0; s < 2; ++s) { f8_bar_init(accf0 + 8 * s, 1); f8_bar_init(acce0 + 8 * s, 4 * CG); }
+
+    // 16 bytes (a run of up to four quads) of the scale rows of a tile: lane i gets operand rows i, i + 32, ...  Rows beyond
+    // the last repeat it: their products are never stored.
+    uint4 w[12];
+    auto fetch = [&](int turn, int run) {
+        int tm, tn;
+        f8_tile(first + turn * step, p.mt, p.nt, tm, tn);
+        const int m0 = (tm * CG + rank) * kF8TileM + lane, n0 = tn * p.tile_n + lane;
+        const uint8_t* a = p.sa + 16 * run;
+        const uint8_t* b = p.sb + 16 * run;
+        if (p.sf_vec) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(a + static_cast<long long>(min(m0 + 32 * j, p.M - 1) >> p.a_shift) * p.ldsa));
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (32 * j < p.tile_n) w[4 + j] = __ldg(reinterpret_cast<const uint4*>(b + static_cast<long long>(min(n0 + 32 * j, p.N - 1) >> p.b_shift) * p.ldsb));
+        } else {
+            const int words = quads - 4 * run;               // that this run has left
+            for (int i = 0; i < 4 && i < words; ++i) {
+#pragma unroll
+                for (int j = 0; j < 12; ++j) {
+                    const uint8_t* src = j < 4 ? a + static_cast<long long>(min(m0 + 32 * j, p.M - 1) >> p.a_shift) * p.ldsa
+                                               : b + static_cast<long long>(min(n0 + 32 * (j - 4), p.N - 1) >> p.b_shift) * p.ldsb;
+                    const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+                    if (i == 0) w[j].x = v; else if (i == 1) w[j].y = v; else if (i == 2) w[j].z = v; else w[j].w = v;
+                }
+            }
+        }
+    };
+    const int my_turns = first < ntiles ? (ntiles - 1 - first) / step + 1 : 0;
+    int sf_turn = 0, sf_run = warp - 2;                      // of the scale warps' next run: tile of this block, run of the tile
+    auto sf_settle = [&] { while (sf_run >= runs) { sf_run -= runs; ++sf_turn; } };
+
+    if (warp == 0) {
+        if (lane == 0) s_abort = 0;
+        for (int i = lane; i < kF8MaxStages; i += 32) { f8_bar_init(full0 + 8 * i, 1); f8_bar_init(empty0 + 8 * i, 1); }
+        if (lane < kF8SfSlots) { f8_bar_init(sff0 + 8 * lane, CG); f8_bar_init(sfe0 + 8 * lane, 1); }
+        if (lane < 2) { f8_bar_init(accf0 + 8 * lane, 1); f8_bar_init(acce0 + 8 * lane, 4 * CG); }
+        if (lane == 0) f8_bar_init(accp, 4 * CG);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (CG == 2) f8_cluster_sync();
-    if (warp == 3) {
+    } else if (warp == 1) {
+        if (f8_elect()) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+        }
+    } else if (warp == 3) {
         if (CG == 1) {
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(f8_smem(&s_tmem)) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -213,104 +336,140 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
+    if (warp == 2 || warp == 3) {
+        sf_settle();
+        if (sf_turn < my_turns) fetch(sf_turn, sf_run);
+    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     if (CG == 2) f8_cluster_sync(); else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
-    const int ntiles = p.mt * p.nt, kb_n = p.kblocks, quads = (kb_n + 3) >> 2;
+    // Two accumulators side by side, or, where they and the scales do not fit, sharing columns: the epilogue then reads the
+    // shared ones first and says so, and the next tile's MMAs start.
+    const uint32_t d_step = min(p.tile_n, kF8SfCol - p.tile_n);
+    const bool overlap = d_step < static_cast<uint32_t>(p.tile_n);
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t s = 0, parity = 1, issued = 0;
-            bool ok = true;
-            for (int t = first; t < ntiles && ok; t += step) {
-                int tm, tn;
-                f8_tile(t, p.mt, p.nt, tm, tn);
-                const int m0 = (tm * CG + rank) * kF8TileM, n0 = tn * p.tile_n + rank * b_rows;
-                for (int kb = 0; kb < kb_n; ++kb, ++issued) {
-                    if (!(ok = f8_wait(empty0 + 8 * s, parity, abort_flag))) break;
-                    if (rank == 0) f8_expect(full0 + 8 * s, CG * stage_bytes);
-                    const uint32_t bar = CG == 2 ? f8_leader(full0 + 8 * s) : full0 + 8 * s;
-                    f8_tma<CG>(smem0 + s * stage_bytes, &map_a, kb * 128, m0, bar);
-                    f8_tma<CG>(smem0 + s * stage_bytes + kF8TileM * 128, &map_b, kb * 128, n0, bar);
-                    if (++s == static_cast<uint32_t>(p.stages)) { s = 0; parity ^= 1u; }
-                }
-            }
-            // nothing may be in flight when the block ends (all of it has landed unless a role gave up)
-            if (rank == 0)
-                for (uint32_t j = issued > static_cast<uint32_t>(p.stages) ? issued - p.stages : 0; j < issued; ++j) {
-                    int never = 0;
-                    f8_wait(full0 + 8 * (j % p.stages), (j / p.stages) & 1u, &never);
-                }
-        }
-    } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            uint32_t s = 0, parity = 0, quad = 0, tile = 0;
-            bool ok = true;
-            for (int t = first; t < ntiles && ok; t += step, ++tile) {
-                const uint32_t buf = tile & 1u, d = tmem + buf * p.tile_n;
-                if (!(ok = f8_wait(acce0 + 8 * buf, ((tile >> 1) & 1u) ^ 1u, abort_flag))) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int kb = 0; kb < kb_n; ++kb) {
-                    const uint32_t sfa = tmem + kF8SfCol + (quad & 1u) * kF8SfCols, sfb = sfa + 4;
-                    if ((kb & 3) == 0) {
-                        const uint32_t slot = quad % kF8SfSlots;
-                        // the buffer's last readers, the MMAs of two quads ago, have to be done
-                        if (quad >= 2 && !(ok = f8_wait(sfe0 + 8 * ((quad - 2) % kF8SfSlots), ((quad - 2) / kF8SfSlots) & 1u, abort_flag))) break;
-                        if (!(ok = f8_wait(sff0 + 8 * slot, (quad / kF8SfSlots) & 1u, abort_flag))) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t src = sf0 + slot * kF8SfSlotBytes;
-                        f8_copy_scales<CG>(sfa, f8_sf_desc(src));
-                        f8_copy_scales<CG>(sfb, f8_sf_desc(src + 512));
-                        if (p.tile_n > 128) f8_copy_scales<CG>(sfb + 4, f8_sf_desc(src + 1024));
-                    }
-                    if (!(ok = f8_wait(full0 + 8 * s, parity, abort_flag))) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t da = f8_desc(smem0 + s * stage_bytes), db = f8_desc(smem0 + s * stage_bytes + kF8TileM * 128);
-                    const uint32_t idesc = p.idesc | (static_cast<uint32_t>(kb & 3) << 29) | (static_cast<uint32_t>(kb & 3) << 4);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) f8_mma<CG>(d, da + 2 * j, db + 2 * j, idesc, sfa, sfb, kb > 0 || j > 0);
-                    f8_commit<CG>(empty0 + 8 * s);
-                    if ((kb & 3) == 3 || kb == kb_n - 1) { f8_commit<CG>(sfe0 + 8 * (quad % kF8SfSlots)); ++quad; }
-                    if (++s == static_cast<uint32_t>(p.stages)) { s = 0; parity ^= 1u; }
-                }
-                if (ok) f8_commit<CG>(accf0 + 8 * buf);
-            }
-        }
-    } else if (warp == 2) {
-        uint32_t quad = 0;
+        uint32_t s = 0, parity = 1, issued = 0;
         bool ok = true;
         for (int t = first; t < ntiles && ok; t += step) {
             int tm, tn;
             f8_tile(t, p.mt, p.nt, tm, tn);
-            const int m0 = (tm * CG + rank) * kF8TileM, n0 = tn * p.tile_n;
-            for (int q = 0; q < quads; ++q, ++quad) {
-                const uint32_t slot = quad % kF8SfSlots, dst = sf0 + slot * kF8SfSlotBytes + lane * 16;
-                uint32_t w[12];
-#pragma unroll
-                for (int j = 0; j < 12; ++j) {
-                    const bool is_a = j < 4;
-                    const int r = is_a ? m0 + lane + 32 * j : n0 + lane + 32 * (j - 4);
-                    const bool in = is_a ? r < p.M : (r < p.N && 32 * (j - 4) < p.tile_n);
-                    const uint8_t* src = is_a ? p.sa + static_cast<long long>(r >> p.a_shift) * p.ldsa
-                                              : p.sb + static_cast<long long>(r >> p.b_shift) * p.ldsb;
-                    w[j] = in ? __ldg(reinterpret_cast<const uint32_t*>(src) + q) : 0x7F7F7F7Fu;
+            const int m0 = (tm * CG + rank) * kF8TileM, n0 = tn * p.tile_n + rank * b_rows;
+            for (int kb = 0; kb < kb_n; ++kb, ++issued) {
+                if (!(ok = f8_wait(empty0 + 8 * s, parity, abort_flag))) break;
+                if (f8_elect()) {
+                    if (rank == 0) f8_expect(full0 + 8 * s, CG * stage_bytes);
+                    const uint32_t bar = CG == 2 ? f8_leader(full0 + 8 * s) : full0 + 8 * s;
+                    f8_tma<CG>(smem0 + s * stage_bytes, &map_a, kb * 128, m0, bar);
+                    f8_tma<CG>(smem0 + s * stage_bytes + kF8TileM * 128, &map_b, kb * 128, n0, bar);
                 }
-                if (!(ok = f8_wait(sfe0 + 8 * slot, ((quad / kF8SfSlots) & 1u) ^ 1u, abort_flag))) break;
+                __syncwarp();
+                if (++s == static_cast<uint32_t>(p.stages)) { s = 0; parity ^= 1u; }
+            }
+        }
+        // nothing may be in flight when the block ends (all of it has landed unless a role gave up)
+        if (rank == 0)
+            for (uint32_t j = issued > static_cast<uint32_t>(p.stages) ? issued - p.stages : 0; j < issued; ++j) {
+                int never = 0;
+                f8_wait(full0 + 8 * (j % p.stages), (j / p.stages) & 1u, &never);
+            }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            uint32_t parity = 0, quad = 0, tile = 0;
+            // Scales of a quad to tensor memory, one quad ahead of the MMAs.  The gathering warps fill four slots each, in turn
+            // by runs; a scale buffer is free when the MMAs of two quads before are done.
+            uint32_t staged = 0, run = 0, run_left = 0, tile_left = 0, taken[2] = {0, 0};
+            uint32_t older_bar = 0, older_parity = 0, last_bar = 0, last_parity = 0;
+            const uint32_t total = static_cast<uint32_t>(my_turns) * quads;
+            auto stage_scales = [&]() -> bool {
+                if (staged >= total) return true;
+                if (tile_left == 0) tile_left = quads;
+                if (run_left == 0) { run_left = min(tile_left, 4u); ++run; }
+                const uint32_t from = (run - 1) & 1u, n = from ? taken[1] : taken[0], slot = 4 * from + (n & 3u), turn_parity = (n >> 2) & 1u;
+                if (staged >= 2 && !f8_wait(older_bar, older_parity, abort_flag)) return false;
+                if (!f8_wait<CG == 2>(sff0 + 8 * slot, turn_parity, abort_flag)) return false;
+                older_bar = last_bar; older_parity = last_parity;
+                last_bar = sfe0 + 8 * slot; last_parity = turn_parity;
+                if (from) ++taken[1]; else ++taken[0];
+                --run_left; --tile_left;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t src = sf0 + slot * kF8SfSlotBytes, dst = tmem + kF8SfCol + (staged & 1u) * kF8SfCols;
+                if (f8_elect()) {
+                    f8_copy_scales<CG>(dst, f8_sf_desc(src));
+                    f8_copy_scales<CG>(dst + 4, f8_sf_desc(src + 512));
+                    if (p.tile_n > 128) f8_copy_scales<CG>(dst + 8, f8_sf_desc(src + 1024));
+                }
+                __syncwarp();
+                ++staged;
+                return true;
+            };
+            // a stage's barrier and the low word of its A descriptor, walked side by side
+            const uint32_t a_first = static_cast<uint32_t>(f8_desc(smem0)), a_step = stage_bytes >> 4, a_end = a_first + p.stages * a_step;
+            uint32_t a_lo = a_first, full = full0;
+            bool ok = stage_scales(), ready = false;
+            for (int t = first; t < ntiles && ok; t += step, ++tile) {
+                const uint32_t buf = tile & 1u, d = tmem + buf * d_step;
+                if (!(ok = f8_wait<CG == 2>(acce0 + 8 * buf, ((tile >> 1) & 1u) ^ 1u, abort_flag))) break;
+                if (overlap && tile > 0 && !(ok = f8_wait<CG == 2>(accp, (tile - 1) & 1u, abort_flag))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int q = 0; q < quads && ok; ++q, ++quad) {
+                    const uint32_t sfa = tmem + kF8SfCol + (quad & 1u) * kF8SfCols, slot = last_bar;
+                    const int slices = min(4, kb_n - 4 * q);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (i >= slices) break;
+                        if (!ready && !(ok = f8_wait(full, parity, abort_flag))) break;
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t at = a_lo, empty = full + (empty0 - full0);
+                        a_lo += a_step;
+                        full += 8;
+                        if (a_lo == a_end) { a_lo = a_first; full = full0; parity ^= 1u; }
+                        ready = f8_test(full, parity);           // answered while the MMAs below are issued
+                        const uint32_t idesc = p.idesc | (static_cast<uint32_t>(i) << 29) | (static_cast<uint32_t>(i) << 4);
+                        if (f8_elect()) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) f8_mma<CG>(d, at + 2 * j, at + (kF8TileM * 128 >> 4) + 2 * j, idesc, sfa, sfa + 4, q > 0 || i > 0 || j > 0);
+                            f8_commit<CG>(empty);
+                            if (i == slices - 1) f8_commit<CG>(slot);
+                        }
+                        __syncwarp();
+                        if (i == min(1, slices - 1) && !(ok = stage_scales())) break;
+                    }
+                }
+                if (ok && f8_elect()) f8_commit<CG>(accf0 + 8 * buf);
+                __syncwarp();
+            }
+        }
+    } else if (warp < kF8EpiWarp) {
+        // Warps 2 and 3 take every other run.  A warp asks for its next run after the last hand-over of the one before (the
+        // fence of a hand-over would wait for loads in flight).
+        uint32_t handed = 0;                                 // quads of this warp so far; it fills four slots of its own in turn
+        bool ok = true;
+        while (ok && sf_turn < my_turns) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if (4 * sf_run + q >= quads) break;
+                const uint32_t slot = 4 * (warp - 2) + (handed & 3u), dst = sf0 + slot * kF8SfSlotBytes + lane * 16;
+                if (!(ok = f8_wait(sfe0 + 8 * slot, ((handed >> 2) & 1u) ^ 1u, abort_flag))) break;
+                ++handed;
 #pragma unroll
                 for (int j = 0; j < 3; ++j)
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + 512 * j), "r"(w[4 * j]), "r"(w[4 * j + 1]),
-                                 "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + 512 * j), "r"(f8_word(w[4 * j], q)), "r"(f8_word(w[4 * j + 1], q)),
+                                 "r"(f8_word(w[4 * j + 2], q)), "r"(f8_word(w[4 * j + 3], q)) : "memory");
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
                     if (CG == 2) f8_arrive_cluster(f8_leader(sff0 + 8 * slot)); else f8_arrive(sff0 + 8 * slot);
                 }
             }
+            sf_run += 2;
+            sf_settle();
+            if (ok && sf_turn < my_turns) fetch(sf_turn, sf_run);
         }
     } else if (warp >= kF8EpiWarp) {
-        const int row0 = (warp & 3) * 32;
-        uint8_t* const stage = smem_raw + (stage0 - f8_smem(smem_raw)) + (warp & 3) * 32 * kPitch;
+        const int row0 = (warp & 3) * 32, chunks = p.tile_n / 32;
+        const uint32_t stage = stage0 + (warp & 3) * 32 * kPitch;
         uint32_t tile = 0;
         T* const y = static_cast<T*>(p.y);
         for (int t = first; t < ntiles; t += step, ++tile) {
@@ -320,53 +479,53 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             const uint32_t buf = tile & 1u;
             if (!f8_wait(accf0 + 8 * buf, (tile >> 1) & 1u, abort_flag)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t src = tmem + buf * p.tile_n + (static_cast<uint32_t>(row0) << 16);
+            const uint32_t src = tmem + buf * d_step + (static_cast<uint32_t>(row0) << 16);
             const int rows = min(32, p.M - m0);
-            for (int c = 0; c < p.tile_n; c += 32) {
-                const int n = n0 + c;
-                if (n >= p.N || rows <= 0) break;            // the same for the whole warp
+            for (int i = 0; i < chunks; ++i) {
+                const int c = 32 * (overlap && buf == 0 ? (i == 0 ? chunks - 1 : i - 1) : i), n = n0 + c;
+                const bool live = n < p.N && rows > 0;       // the same for the whole warp
                 uint32_t v[32];
-                f8_tmem_ld32(v, src + c);
+                if (live) f8_tmem_ld32(v, src + c);
+                if (overlap && i == 0) {
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) { if (CG == 2) f8_arrive_cluster(f8_leader(accp)); else f8_arrive(accp); }
+                }
+                if (!live) continue;
                 const int cols = min(32, p.N - n);
-                T out[32];
+                float f[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    float f = p.alpha * __uint_as_float(v[j]);
-                    if (p.bias != nullptr && j < cols) f += __ldg(p.bias + n + j);
-                    out[j] = f8_out<T>(f);
+                for (int j = 0; j < 32; ++j) f[j] = p.alpha * __uint_as_float(v[j]);
+                if (p.bias != nullptr) {
+                    const int top = p.N - 1 - n;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) f[j] += __ldg(p.bias + n + min(j, top));
                 }
-                if (p.drop.rng != nullptr) {
-                    const PhiloxKey key(p.drop.rng);
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const unsigned keep = philox_keep8_at(key, static_cast<unsigned long long>(m0 + lane) * p.N + n + 8 * g, p.drop.threshold);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) if (!((keep >> j) & 1u)) out[8 * g + j] = f8_out<T>(0.0f);
-                    }
-                }
+                if (p.drop.rng != nullptr) f8_mask32(p.drop, static_cast<unsigned long long>(m0 + lane) * p.N + n, f);
                 constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer;       // of a 32-element row
                 __syncwarp();                                                   // the last chunk's readers are through
 #pragma unroll
-                for (int j = 0; j < kPieces; ++j) {
-                    uint4 pack;
-                    T* e = reinterpret_cast<T*>(&pack);
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) e[i] = out[j * kPer + i];
-                    *reinterpret_cast<uint4*>(stage + lane * kPitch + 16 * j) = pack;
-                }
+                for (int j = 0; j < kPieces; ++j) f8_put16<T>(stage + lane * kPitch + 16 * j, f + j * kPer);
                 __syncwarp();
                 if (p.vec && cols == 32) {
-                    const int piece = lane % kPieces;
+                    const int piece = lane % kPieces, r0 = lane / kPieces;
+                    T* dst = y + static_cast<long long>(m0 + r0) * p.ldy + n + piece * kPer;
+                    uint4 e[kPieces];
 #pragma unroll
-                    for (int i = 0; i < kPieces; ++i) {
-                        const int r = lane / kPieces + i * (32 / kPieces);
-                        if (r < rows)
-                            *reinterpret_cast<uint4*>(y + static_cast<long long>(m0 + r) * p.ldy + n + piece * kPer) =
-                                *reinterpret_cast<const uint4*>(stage + r * kPitch + 16 * piece);
+                    for (int j = 0; j < kPieces; ++j) e[j] = f8_get16(stage + (r0 + j * (32 / kPieces)) * kPitch + 16 * piece);
+                    if (rows >= 32) {
+#pragma unroll
+                        for (int j = 0; j < kPieces; ++j) *reinterpret_cast<uint4*>(dst + j * (32 / kPieces) * p.ldy) = e[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kPieces; ++j)
+                            if (r0 + j * (32 / kPieces) < rows) *reinterpret_cast<uint4*>(dst + j * (32 / kPieces) * p.ldy) = e[j];
                     }
                 } else if (lane < cols) {
-                    for (int r = 0; r < rows; ++r)
-                        y[static_cast<long long>(m0 + r) * p.ldy + n + lane] = *reinterpret_cast<const T*>(stage + r * kPitch + lane * sizeof(T));
+                    T* dst = y + static_cast<long long>(m0) * p.ldy + n + lane;
+                    const int live_rows = min(rows, 32);
+#pragma unroll 8
+                    for (int r = 0; r < live_rows; ++r) dst[r * p.ldy] = f8_get<T>(stage + r * kPitch + lane * sizeof(T));
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -500,6 +659,7 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     Fp8Params p{};
     p.sa = sa; p.sb = sb; p.ldsa = ldsa; p.ldsb = ldsb;
     p.a_shift = a_block_rows == 128 ? 7 : 0; p.b_shift = b_block_rows == 128 ? 7 : 0;
+    p.sf_vec = aligned_to(sa, 16) && ldsa % 16 == 0 && aligned_to(sb, 16) && ldsb % 16 == 0;
     p.bias = bias; p.alpha = alpha; p.y = y; p.ldy = ldy; p.M = M; p.N = N; p.kblocks = kblocks;
     const int cg = M > kF8TileM ? 2 : 1;
     p.tile_n = N >= kF8MaxTileN ? kF8MaxTileN : ((N + 31) / 32) * 32;

@@ -309,7 +309,8 @@ int atb_fp8_quantize(const void* x, int x_dtype, long long R, long long C, long 
                      long long ldst, int drop_threshold, const void* rng, void* stream);
 /* y[m, n] = alpha * sum_k A[m, k] B[n, k] (scales applied) + bias[n], summed in fp32, rounded once to y_dtype
  * (fp32 / bf16 / fp16); A [M, K], B [N, K].  Row pitches lda, ldb: multiples of 16, bases 16-byte aligned; ldsa, ldsb:
- * multiples of 4, bases 4-byte aligned, and every scale row readable up to a multiple of 4 bytes.  bias fp32 or NULL.
+ * multiples of 4, bases 4-byte aligned, and every scale row readable up to a multiple of 4 bytes (of 16, where base and
+ * pitch are multiples of 16).  bias fp32 or NULL.
  * drop_threshold > 0: elements of y that atb_dropout would drop from the contiguous [M, N] tensor become 0 (no factor). */
 int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_t* sa, long long ldsa, int a_block_rows,
                  const void* b, int b_f8, long long ldb, const uint8_t* sb, long long ldsb, int b_block_rows,

@@ -29,6 +29,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <math.h>
 
 #include "common.cuh"
 #include "philox.cuh"
@@ -42,6 +43,7 @@ constexpr int kF8TileM = 128, kF8MaxTileN = 256;          // of one block; a pai
 constexpr int kF8SfSlots = 8, kF8SfSlotBytes = 3 * 512;   // a run of quads for each gathering warp; 128 rows of A, up to 256 of B
 constexpr int kF8SfCol = 488, kF8SfCols = 12;             // tensor-memory columns of the two scale buffers
 constexpr int kF8Smem = 226 * 1024, kF8MaxStages = 8;
+constexpr int kF8MaxQuads = 40;                           // of one block of fp8_split_kernel
 constexpr int kF8Group = 8;                               // row tiles that are walked together (their operands meet in L2)
 
 struct Fp8Params {
@@ -117,8 +119,13 @@ __device__ __forceinline__ uint32_t f8_leader(uint32_t addr)
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
-__device__ __forceinline__ void f8_arrive_cluster(uint32_t bar)
+// An arrival at a barrier of the pair's first block.  MEMORY: it hands over what this block wrote to its shared memory;
+// without, it only says that tensor memory has been read, which the tcgen05 fences on both sides order.
+template <bool MEMORY>
+__device__ __forceinline__ void f8_arrive_leader(uint32_t local_bar)
 {
+    const uint32_t bar = f8_leader(local_bar);
+    if (!MEMORY) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); return; }
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void f8_cluster_sync()
@@ -185,6 +192,15 @@ __device__ __forceinline__ void f8_tmem_ld32(uint32_t (&v)[32], uint32_t addr)
                    "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
                    "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
                    "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+                 : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void f8_tmem_ld16(uint32_t (&v)[16], uint32_t addr)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+                   "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
                  : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -410,8 +426,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             bool ok = stage_scales(), ready = false;
             for (int t = first; t < ntiles && ok; t += step, ++tile) {
                 const uint32_t buf = tile & 1u, d = tmem + buf * d_step;
-                if (!(ok = f8_wait<CG == 2>(acce0 + 8 * buf, ((tile >> 1) & 1u) ^ 1u, abort_flag))) break;
-                if (overlap && tile > 0 && !(ok = f8_wait<CG == 2>(accp, (tile - 1) & 1u, abort_flag))) break;
+                if (!(ok = f8_wait(acce0 + 8 * buf, ((tile >> 1) & 1u) ^ 1u, abort_flag))) break;
+                if (overlap && tile > 0 && !(ok = f8_wait(accp, (tile - 1) & 1u, abort_flag))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (int q = 0; q < quads && ok; ++q, ++quad) {
                     const uint32_t sfa = tmem + kF8SfCol + (quad & 1u) * kF8SfCols, slot = last_bar;
@@ -460,7 +476,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    if (CG == 2) f8_arrive_cluster(f8_leader(sff0 + 8 * slot)); else f8_arrive(sff0 + 8 * slot);
+                    if (CG == 2) f8_arrive_leader<true>(sff0 + 8 * slot); else f8_arrive(sff0 + 8 * slot);
                 }
             }
             sf_run += 2;
@@ -489,7 +505,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (overlap && i == 0) {
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) { if (CG == 2) f8_arrive_cluster(f8_leader(accp)); else f8_arrive(accp); }
+                    if (lane == 0) { if (CG == 2) f8_arrive_leader<false>(accp); else f8_arrive(accp); }
                 }
                 if (!live) continue;
                 const int cols = min(32, p.N - n);
@@ -531,7 +547,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                if (CG == 2) f8_arrive_cluster(f8_leader(acce0 + 8 * buf)); else f8_arrive(acce0 + 8 * buf);
+                if (CG == 2) f8_arrive_leader<false>(acce0 + 8 * buf); else f8_arrive(acce0 + 8 * buf);
             }
         }
     }
@@ -543,6 +559,206 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
+}
+
+// ---- products of few tiles --------------------------------------------------------------------------------------------
+// y = alpha A B^T + bias for few rows of A (serving) or small matrices: one tile of 128 rows of B by tile_c rows of A, and
+// the reduction cut over the S blocks of a cluster, so that 4096 x 4096 weights and one row of A keep 128 SMs reading
+// instead of 32.  B supplies the MMA's 128 rows whatever M is, so no tensor-core row is wasted on a missing token; each
+// block requests its whole share of B at once (up to kF8MaxStages slices).  The S partial tiles meet in shared memory: every
+// block adds up its share of the columns over the cluster in the order of the blocks (bit for bit repeatable) and stores
+// it.  No workspace, no counters, one launch.
+struct Fp8SplitParams {
+    const uint8_t* sa;
+    const uint8_t* sb;
+    long long ldsa, ldsb;
+    int a_shift, b_shift;
+    const float* bias;
+    float alpha;
+    void* y;
+    long long ldy;
+    int M, N, kblocks;
+    int tile_c, ct, splits, stages;          // ct: column tiles
+    uint32_t tmem_cols;
+    uint32_t idesc;
+    DropState drop;
+};
+
+__device__ __forceinline__ float f8_remote(uint32_t addr, uint32_t block)
+{
+    float v;
+    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}"
+                 : "=f"(v) : "r"(addr), "r"(block) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t f8_cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kF8Threads)
+fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a, const Fp8SplitParams p)
+{
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    __shared__ __align__(8) uint64_t s_full[kF8MaxStages], s_empty[kF8MaxStages], s_sf[kF8MaxQuads], s_acc;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
+    const uint32_t rank = f8_cluster_rank();
+    const int tile = blockIdx.x / p.splits, n0 = (tile / p.ct) * kF8TileM, m0 = (tile % p.ct) * p.tile_c;
+    const int kb0 = static_cast<int>(static_cast<long long>(p.kblocks) * rank / p.splits);
+    const int kb1 = static_cast<int>(static_cast<long long>(p.kblocks) * (rank + 1) / p.splits);
+    const uint32_t smem0 = (f8_smem(smem_raw) + 1023u) & ~1023u;
+    const uint32_t stage_bytes = (kF8TileM + p.tile_c) * 128, sf0 = smem0 + p.stages * stage_bytes;
+    const uint32_t full0 = f8_smem(s_full), empty0 = f8_smem(s_empty), sff0 = f8_smem(s_sf), acc0 = f8_smem(&s_acc);
+    volatile int* abort_flag = &s_abort;
+    if (warp == 0) {
+        if (lane == 0) { s_abort = 0; f8_bar_init(acc0, 1); }
+        if (lane < kF8MaxStages) { f8_bar_init(full0 + 8 * lane, 1); f8_bar_init(empty0 + 8 * lane, 1); }
+        for (int i = lane; i < kF8MaxQuads; i += 32) f8_bar_init(sff0 + 8 * i, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    } else if (warp == 1) {
+        if (f8_elect()) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
+        }
+    } else if (warp == 3) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(f8_smem(&s_tmem)), "r"(p.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = s_tmem;
+    const int q0 = kb0 >> 2, quads = ((kb1 + 3) >> 2) - q0;      // of this block, by place in a scale row
+
+    if (warp == 0) {
+        uint32_t s = 0, parity = 1;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (!(ok = f8_wait(empty0 + 8 * s, parity, abort_flag))) break;
+            if (f8_elect()) {
+                f8_expect(full0 + 8 * s, stage_bytes);
+                f8_tma<1>(smem0 + s * stage_bytes, &map_b, kb * 128, n0, full0 + 8 * s);
+                f8_tma<1>(smem0 + s * stage_bytes + kF8TileM * 128, &map_a, kb * 128, m0, full0 + 8 * s);
+            }
+            __syncwarp();
+            if (++s == static_cast<uint32_t>(p.stages)) { s = 0; parity ^= 1u; }
+        }
+        if (!ok)                                             // nothing may be in flight when the block ends
+            for (int j = 0; j < p.stages; ++j) { int never = 0; f8_wait(full0 + 8 * j, parity ^ (j < static_cast<int>(s) ? 1u : 0u), &never); }
+    } else if (warp == 1) {
+        const uint32_t a_first = static_cast<uint32_t>(f8_desc(smem0)), a_step = stage_bytes >> 4, a_end = a_first + p.stages * a_step;
+        uint32_t a_lo = a_first, full = full0, parity = 0, sfa = tmem + p.tile_c - 8;
+        bool ok = true, ready = false;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (kb == kb0 || (kb & 3) == 0) {
+                const int q = (kb >> 2) - q0;
+                sfa += 8;
+                if (!(ok = f8_wait(sff0 + 8 * q, 0, abort_flag))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (f8_elect()) {
+                    f8_copy_scales<1>(sfa, f8_sf_desc(sf0 + q * 1024));
+                    f8_copy_scales<1>(sfa + 4, f8_sf_desc(sf0 + q * 1024 + 512));
+                }
+                __syncwarp();
+            }
+            if (!ready && !(ok = f8_wait(full, parity, abort_flag))) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at = a_lo, empty = full + (empty0 - full0);
+            a_lo += a_step;
+            full += 8;
+            if (a_lo == a_end) { a_lo = a_first; full = full0; parity ^= 1u; }
+            ready = f8_test(full, parity);
+            const uint32_t idesc = p.idesc | (static_cast<uint32_t>(kb & 3) << 29) | (static_cast<uint32_t>(kb & 3) << 4);
+            if (f8_elect()) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f8_mma<1>(tmem, at + 2 * j, at + (kF8TileM * 128 >> 4) + 2 * j, idesc, sfa, sfa + 4, kb > kb0 || j > 0);
+                f8_commit<1>(empty);
+            }
+            __syncwarp();
+        }
+        if (ok && f8_elect()) f8_commit<1>(acc0);
+        __syncwarp();
+    } else if (warp < kF8EpiWarp) {
+        // scale words of a quad: lane i takes rows i, i + 32, ... of both operands
+        for (int q = warp - 2; q < quads; q += 2) {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint8_t* src = j < 4 ? p.sb + static_cast<long long>(min(n0 + lane + 32 * j, p.N - 1) >> p.b_shift) * p.ldsb
+                                           : p.sa + static_cast<long long>(min(m0 + lane + 32 * (j - 4), p.M - 1) >> p.a_shift) * p.ldsa;
+                w[j] = j < 4 || 32 * (j - 4) < p.tile_c ? __ldg(reinterpret_cast<const uint32_t*>(src) + q0 + q) : 0x7F7F7F7Fu;
+            }
+            const uint32_t dst = sf0 + q * 1024 + lane * 16;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + 512 * j), "r"(w[4 * j]), "r"(w[4 * j + 1]),
+                             "r"(w[4 * j + 2]), "r"(w[4 * j + 3]) : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) f8_arrive(sff0 + 8 * q);
+        }
+    }
+    const int cols = min(p.tile_c, p.M - m0);
+    T* const y = static_cast<T*>(p.y) + static_cast<long long>(m0) * p.ldy;
+    auto store = [&](int n, int c, float v, float bias) {
+        float f = p.alpha * v + bias;
+        if (p.drop.rng != nullptr) {
+            const unsigned long long e = static_cast<unsigned long long>(m0 + c) * p.N + n;
+            if (!((f8_keep8(p.drop.rng, p.drop.threshold, e & ~7ull) >> (e & 7u)) & 1u)) f = 0.0f;
+        }
+        y[c * p.ldy + n] = f8_out<T>(f);
+    };
+    if (warp >= kF8EpiWarp) {
+        if (f8_wait(acc0, 0, abort_flag)) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int row = (warp & 3) * 32 + lane, n = n0 + row;
+            const float bias = p.splits == 1 && p.bias != nullptr && n < p.N ? __ldg(p.bias + n) : 0.0f;
+            for (int c = 0; c < cols; c += 16) {
+                uint32_t v[16];
+                f8_tmem_ld16(v, tmem + c + (static_cast<uint32_t>((warp & 3) * 32) << 16));
+                if (p.splits == 1) {                         // nothing to meet: straight to y, a warp's lanes side by side
+                    if (n < p.N) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) if (c + j < cols) store(n, c + j, __uint_as_float(v[j]), bias);
+                    }
+                } else {                                     // over the stages: all MMAs are done
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        asm volatile("st.shared.b32 [%0], %1;" ::"r"(smem0 + ((c + j) * kF8TileM + row) * 4), "r"(v[j]) : "memory");
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        }
+    }
+    __syncwarp();
+    if (p.splits == 1) __syncthreads(); else f8_cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+    if (tid == 0 && s_abort) g_fp8_status = 1;
+    if (p.splits == 1) return;
+    // ---- every block finishes its share of the columns, four at a time so that the reads overlap
+    const int row = tid & (kF8TileM - 1), n = n0 + row;
+    if (n < p.N) {
+        const float bias = p.bias != nullptr ? __ldg(p.bias + n) : 0.0f;
+        const int step = 2 * p.splits;
+        for (int c = static_cast<int>(rank) + p.splits * (tid >> 7); c < cols; c += 4 * step) {
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int j = 0; j < p.splits; ++j) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (c + i * step < cols) sum[i] += f8_remote(smem0 + ((c + i * step) * kF8TileM + row) * 4, j);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (c + i * step < cols) store(n, c + i * step, sum[i], bias);
+        }
+    }
+    f8_cluster_sync();                                       // no block leaves while another reads its part
 }
 
 // y = bias (a product over nothing)
@@ -589,10 +805,64 @@ static int operand_map(CUtensorMap* map, const void* base, long long R, long lon
     return ATB_OK;
 }
 
+// How a product is cut: the kernel, tile and number of blocks to a tile with the least estimated time.  Microseconds as
+// measured on B200 (8-bit operands of random numbers): a slice (128 steps) of a tile costs 0.06 + 0.0013 per column to a
+// pair of blocks (the MMAs; 0.22 at least, the issue), 0.165 + 0.00106 per column to a single block; a tile besides, 0.4 +
+// 0.003 per column; a launch with a first load, 3.9 (pairs: 5.0).  The split kernel: 0.14 + 0.0016 per row of A for a slice,
+// 0.8 + 0.025 per row of A and 0.06 per block of the cluster for a tile, 3.2 for the launch.
+struct Fp8Plan {
+    int cg, tile;            // fp8_gemm_kernel: blocks to a tile, columns
+    int splits;              // fp8_split_kernel where not 0: blocks to a tile; tile = rows of A
+};
+
+static Fp8Plan fp8_plan(int M, int N, int kblocks)
+{
+    Fp8Plan best{1, 32, 0};
+    double least = 1e300;
+    const int sms = sm_count();
+    for (int cg = 1; cg <= 2; ++cg) {
+        const double mt = (M + cg * kF8TileM - 1) / (cg * kF8TileM);
+        for (int tile = 32; tile <= kF8MaxTileN; tile += 32) {
+            if (tile > 32 && tile - 32 >= N) break;
+            const double nt = (N + tile - 1) / tile, waves = ceil(mt * nt / (sms / cg));
+            const double slice = cg == 2 ? fmax(0.22, 0.06 + 0.0013 * tile) : 0.165 + 0.00106 * tile;
+            const double t = waves * (kblocks * slice + 0.4 + 0.003 * tile) + (cg == 2 ? 5.0 : 3.9);
+            if (t < least) { least = t; best = Fp8Plan{cg, tile, 0}; }
+        }
+    }
+    const double nt = (N + kF8TileM - 1) / kF8TileM;
+    for (int tile = 16; tile <= kF8TileM; tile += 16) {
+        if (tile > 16 && tile - 16 >= M) break;
+        const double mt = (M + tile - 1) / tile;
+        if (mt * nt > 16.0 * sms) continue;                  // many tiles: never the better kernel
+        for (int splits = 1; splits <= 8 && splits <= kblocks; ++splits) {
+            const int kbs = (kblocks + splits - 1) / splits;
+            if (kbs / 4 + 2 > kF8MaxQuads) continue;
+            const double waves = ceil(mt * nt * splits / sms);
+            const double t = waves * (kbs * (0.14 + 0.0016 * tile) + 0.8 + 0.025 * tile + 0.06 * splits) + 3.2;
+            if (t < least) { least = t; best = Fp8Plan{1, tile, splits}; }
+        }
+    }
+    return best;
+}
+
+// the kernels' shared memory is above the default limit: allowed once per device
+template <class K>
+static cudaError_t allow_smem(K kernel, bool (&done)[64])
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev])) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    return e;
+}
+
 template <class T, int CG>
 static int launch_fp8(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Params& p, cudaStream_t s)
 {
-    cudaError_t e = cudaFuncSetAttribute(fp8_gemm_kernel<T, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
+    static bool done[64];
+    cudaError_t e = allow_smem(fp8_gemm_kernel<T, CG>, done);
     const int tiles = p.mt * p.nt, fit = sm_count() / CG;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(CG * (tiles < fit ? tiles : fit));
@@ -614,6 +884,27 @@ template <class T>
 static int launch_fp8_cg(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Params& p, int cg, cudaStream_t s)
 {
     return cg == 2 ? launch_fp8<T, 2>(ma, mb, p, s) : launch_fp8<T, 1>(ma, mb, p, s);
+}
+
+template <class T>
+static int launch_split(const CUtensorMap& mb, const CUtensorMap& ma, const Fp8SplitParams& p, int tiles, size_t smem, cudaStream_t s)
+{
+    static bool done[64];
+    cudaError_t e = allow_smem(fp8_split_kernel<T>, done);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(tiles * p.splits);
+    cfg.blockDim = dim3(kF8Threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = p.splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, fp8_split_kernel<T>, mb, ma, p);
+    if (e != cudaSuccess) { set_error("fp8_split_kernel: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
+    return check_launch("fp8_split_kernel");
 }
 
 template <class T>
@@ -661,20 +952,52 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     p.a_shift = a_block_rows == 128 ? 7 : 0; p.b_shift = b_block_rows == 128 ? 7 : 0;
     p.sf_vec = aligned_to(sa, 16) && ldsa % 16 == 0 && aligned_to(sb, 16) && ldsb % 16 == 0;
     p.bias = bias; p.alpha = alpha; p.y = y; p.ldy = ldy; p.M = M; p.N = N; p.kblocks = kblocks;
-    const int cg = M > kF8TileM ? 2 : 1;
-    p.tile_n = N >= kF8MaxTileN ? kF8MaxTileN : ((N + 31) / 32) * 32;
+    const Fp8Plan plan = fp8_plan(M, N, kblocks);
+    const DropState drop{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)};
+    const uint32_t formats = (1u << 23);                     // scales are powers of two (ue8m0)
+    CUtensorMap ma, mb;
+    if (plan.splits) {
+        Fp8SplitParams q{sa, sb, ldsa, ldsb, p.a_shift, p.b_shift, bias, alpha, y, ldy, M, N, kblocks};
+        q.tile_c = plan.tile;
+        q.ct = (M + plan.tile - 1) / plan.tile;
+        q.splits = plan.splits;
+        const int kbs = (kblocks + plan.splits - 1) / plan.splits, quads = kbs / 4 + 2, stage = (kF8TileM + plan.tile) * 128;
+        const int sums = plan.tile * kF8TileM * 4;           // the partial tile takes the stages' place
+        q.stages = (kF8Smem - 1024 - quads * 1024) / stage;
+        q.stages = q.stages < kbs ? q.stages : kbs;
+        q.stages = q.stages < kF8MaxStages ? q.stages : kF8MaxStages;
+        q.stages = q.stages * stage >= sums ? q.stages : (sums + stage - 1) / stage;
+        q.tmem_cols = 32;
+        while (q.tmem_cols < static_cast<uint32_t>(plan.tile + 8 * quads)) q.tmem_cols *= 2;
+        q.idesc = formats | (b_f8 == ATB_E5M2 ? 1u << 7 : 0u) | (a_f8 == ATB_E5M2 ? 1u << 10 : 0u) | (static_cast<uint32_t>(plan.tile >> 3) << 17) | (1u << 27);
+        q.drop = drop;
+        // At least the tensor memory's share of an SM's 228 KB: blocks that fit an SM together then find their columns too.  (A
+        // block of one cluster that waited for columns held by another cluster's block, which waits for its own cluster on
+        // an SM where the first cluster holds the columns, would wait for ever.)
+        const size_t share = 456 * static_cast<size_t>(q.tmem_cols) - 1024;
+        size_t smem = 1024 + static_cast<size_t>(q.stages) * stage + static_cast<size_t>(quads) * 1024;
+        smem = smem < share ? share : smem;
+        smem = smem < kF8Smem ? smem : kF8Smem;              // (which leaves no room for a second block either)
+        const int tiles = ((N + kF8TileM - 1) / kF8TileM) * q.ct;
+        int rc = operand_map(&mb, b, N, K, ldb, kF8TileM);
+        if (rc == ATB_OK) rc = operand_map(&ma, a, M, K, lda, plan.tile);
+        if (rc != ATB_OK) return rc;
+        if (y_dtype == ATB_F32) return launch_split<float>(mb, ma, q, tiles, smem, s);
+        if (y_dtype == ATB_BF16) return launch_split<__nv_bfloat16>(mb, ma, q, tiles, smem, s);
+        return launch_split<__half>(mb, ma, q, tiles, smem, s);
+    }
+    const int cg = plan.cg;
+    p.tile_n = plan.tile;
     p.mt = (M + cg * kF8TileM - 1) / (cg * kF8TileM);
     p.nt = (N + p.tile_n - 1) / p.tile_n;
     ATB_REQUIRE(static_cast<long long>(p.mt) * p.nt < (1LL << 30), "too many tiles");
     const int stage = kF8TileM * 128 + p.tile_n / cg * 128;
     p.stages = (kF8Smem - 1024 - kF8SfSlots * kF8SfSlotBytes - 4 * 32 * (32 * size + 16)) / stage;
     if (p.stages > kF8MaxStages) p.stages = kF8MaxStages;
-    p.idesc = (a_f8 == ATB_E5M2 ? 1u << 7 : 0u) | (b_f8 == ATB_E5M2 ? 1u << 10 : 0u) |
-              (static_cast<uint32_t>(p.tile_n >> 3) << 17) | (1u << 23) | (static_cast<uint32_t>(cg) << 27);
+    p.idesc = formats | (a_f8 == ATB_E5M2 ? 1u << 7 : 0u) | (b_f8 == ATB_E5M2 ? 1u << 10 : 0u) |
+              (static_cast<uint32_t>(p.tile_n >> 3) << 17) | (static_cast<uint32_t>(cg) << 27);
     p.vec = aligned_to(y, 16) && (ldy * size) % 16 == 0;
-    p.drop = DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)};
-
-    CUtensorMap ma, mb;
+    p.drop = drop;
     int rc = operand_map(&ma, a, M, K, lda, kF8TileM);
     if (rc == ATB_OK) rc = operand_map(&mb, b, N, K, ldb, p.tile_n / cg);
     if (rc != ATB_OK) return rc;

@@ -38,11 +38,13 @@ namespace atb {
 
 __device__ int g_fp8_status = 0;                      // 1: a block gave up waiting
 
-constexpr int kF8Threads = 256, kF8EpiWarp = 4;
+constexpr int kF8Threads = 256, kF8EpiWarp = 4, kF8EpiWarps = 4;
+constexpr int kF8SumThreads = 384, kF8SumEpiWarps = 8, kF8SumTileN = 192, kF8SumQuads = 2;   // with fp32 sums of partial products
 constexpr int kF8TileM = 128, kF8MaxTileN = 256;          // of one block; a pair's tile has twice the rows
 constexpr int kF8SfSlots = 8, kF8SfSlotBytes = 3 * 512;   // a run of quads for each gathering warp; 128 rows of A, up to 256 of B
 constexpr int kF8SfCol = 488, kF8SfCols = 12;             // tensor-memory columns of the two scale buffers
 constexpr int kF8Smem = 226 * 1024, kF8MaxStages = 8;
+constexpr int kF8SumsFrom = 16;                          // slices beyond which an fp32 result is added up from partial sums
 constexpr int kF8MaxQuads = 40;                           // of one block of fp8_split_kernel
 constexpr int kF8Group = 8;                               // row tiles that are walked together (their operands meet in L2)
 
@@ -277,8 +279,12 @@ __device__ __forceinline__ void f8_tile(int t, int mt, int nt, int& tm, int& tn)
     tm = g * kF8Group + (in - tn * rows);
 }
 
-template <class T, int CG>
-__global__ void __launch_bounds__(kF8Threads, 1)
+// SUMS: the tensor core's accumulator cuts what does not fit its 24 bits instead of rounding it, which leaves a bias towards
+// zero that grows with the number of additions (2e-6 of a result over 8192 steps).  A bf16 or fp16 result hides it; for a
+// long reduction to fp32 the accumulators are read every 1024 steps (kF8SumQuads quads) and added up, rounded, in the
+// registers of eight epilogue warps, the two accumulators taking turns.
+template <class T, int CG, bool SUMS>
+__global__ void __launch_bounds__(SUMS ? kF8SumThreads : kF8Threads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp8Params p)
 {
     extern __shared__ uint8_t smem_raw[];
@@ -335,8 +341,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (lane == 0) s_abort = 0;
         for (int i = lane; i < kF8MaxStages; i += 32) { f8_bar_init(full0 + 8 * i, 1); f8_bar_init(empty0 + 8 * i, 1); }
         if (lane < kF8SfSlots) { f8_bar_init(sff0 + 8 * lane, CG); f8_bar_init(sfe0 + 8 * lane, 1); }
-        if (lane < 2) { f8_bar_init(accf0 + 8 * lane, 1); f8_bar_init(acce0 + 8 * lane, 4 * CG); }
-        if (lane == 0) f8_bar_init(accp, 4 * CG);
+        if (lane < 2) { f8_bar_init(accf0 + 8 * lane, 1); f8_bar_init(acce0 + 8 * lane, (SUMS ? kF8SumEpiWarps : kF8EpiWarps) * CG); }
+        if (lane == 0) f8_bar_init(accp, kF8EpiWarps * CG);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     } else if (warp == 1) {
         if (f8_elect()) {
@@ -392,7 +398,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             }
     } else if (warp == 1) {
         if (rank == 0) {
-            uint32_t parity = 0, quad = 0, tile = 0;
+            uint32_t parity = 0, quad = 0, tile = 0;         // tile: accumulators used so far
             // Scales of a quad to tensor memory, one quad ahead of the MMAs.  The gathering warps fill four slots each, in turn
             // by runs; a scale buffer is free when the MMAs of two quads before are done.
             uint32_t staged = 0, run = 0, run_left = 0, tile_left = 0, taken[2] = {0, 0};
@@ -424,14 +430,17 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             const uint32_t a_first = static_cast<uint32_t>(f8_desc(smem0)), a_step = stage_bytes >> 4, a_end = a_first + p.stages * a_step;
             uint32_t a_lo = a_first, full = full0;
             bool ok = stage_scales(), ready = false;
-            for (int t = first; t < ntiles && ok; t += step, ++tile) {
+            const int item_quads = SUMS ? kF8SumQuads : quads, items = (quads + item_quads - 1) / item_quads * my_turns;
+            for (int it = 0, left = quads; it < items && ok; ++it, ++tile) {
                 const uint32_t buf = tile & 1u, d = tmem + buf * d_step;
+                const int now = min(left, item_quads), kb_left = min(4 * now, kb_n - 4 * (quads - left));   // of this accumulator
+                left = left == now ? quads : left - now;
                 if (!(ok = f8_wait(acce0 + 8 * buf, ((tile >> 1) & 1u) ^ 1u, abort_flag))) break;
                 if (overlap && tile > 0 && !(ok = f8_wait(accp, (tile - 1) & 1u, abort_flag))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                for (int q = 0; q < quads && ok; ++q, ++quad) {
+                for (int q = 0; q < now && ok; ++q, ++quad) {
                     const uint32_t sfa = tmem + kF8SfCol + (quad & 1u) * kF8SfCols, slot = last_bar;
-                    const int slices = min(4, kb_n - 4 * q);
+                    const int slices = min(4, kb_left - 4 * q);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (i >= slices) break;
@@ -484,70 +493,107 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (ok && sf_turn < my_turns) fetch(sf_turn, sf_run);
         }
     } else if (warp >= kF8EpiWarp) {
-        const int row0 = (warp & 3) * 32, chunks = p.tile_n / 32;
-        const uint32_t stage = stage0 + (warp & 3) * 32 * kPitch;
-        uint32_t tile = 0;
+        const int row0 = (warp & 3) * 32;
+        const uint32_t stage = stage0 + (warp - kF8EpiWarp) * 32 * kPitch;
+        const uint32_t lanes = static_cast<uint32_t>(row0) << 16;
         T* const y = static_cast<T*>(p.y);
-        for (int t = first; t < ntiles; t += step, ++tile) {
-            int tm, tn;
-            f8_tile(t, p.mt, p.nt, tm, tn);
-            const int m0 = (tm * CG + rank) * kF8TileM + row0, n0 = tn * p.tile_n;
-            const uint32_t buf = tile & 1u;
-            if (!f8_wait(accf0 + 8 * buf, (tile >> 1) & 1u, abort_flag)) break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t src = tmem + buf * d_step + (static_cast<uint32_t>(row0) << 16);
-            const int rows = min(32, p.M - m0);
-            for (int i = 0; i < chunks; ++i) {
-                const int c = 32 * (overlap && buf == 0 ? (i == 0 ? chunks - 1 : i - 1) : i), n = n0 + c;
-                const bool live = n < p.N && rows > 0;       // the same for the whole warp
-                uint32_t v[32];
-                if (live) f8_tmem_ld32(v, src + c);
-                if (overlap && i == 0) {
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) { if (CG == 2) f8_arrive_leader<false>(accp); else f8_arrive(accp); }
-                }
-                if (!live) continue;
-                const int cols = min(32, p.N - n);
-                float f[32];
+        // 32 x 32 results: f holds this lane's row, columns n ...
+        auto emit = [&](float (&f)[32], int m0, int n, int rows) {
+            const int cols = min(32, p.N - n);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) f[j] = p.alpha * __uint_as_float(v[j]);
-                if (p.bias != nullptr) {
-                    const int top = p.N - 1 - n;
+            for (int j = 0; j < 32; ++j) f[j] *= p.alpha;
+            if (p.bias != nullptr) {
+                const int top = p.N - 1 - n;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) f[j] += __ldg(p.bias + n + min(j, top));
-                }
-                if (p.drop.rng != nullptr) f8_mask32(p.drop, static_cast<unsigned long long>(m0 + lane) * p.N + n, f);
-                constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer;       // of a 32-element row
-                __syncwarp();                                                   // the last chunk's readers are through
-#pragma unroll
-                for (int j = 0; j < kPieces; ++j) f8_put16<T>(stage + lane * kPitch + 16 * j, f + j * kPer);
-                __syncwarp();
-                if (p.vec && cols == 32) {
-                    const int piece = lane % kPieces, r0 = lane / kPieces;
-                    T* dst = y + static_cast<long long>(m0 + r0) * p.ldy + n + piece * kPer;
-                    uint4 e[kPieces];
-#pragma unroll
-                    for (int j = 0; j < kPieces; ++j) e[j] = f8_get16(stage + (r0 + j * (32 / kPieces)) * kPitch + 16 * piece);
-                    if (rows >= 32) {
-#pragma unroll
-                        for (int j = 0; j < kPieces; ++j) *reinterpret_cast<uint4*>(dst + j * (32 / kPieces) * p.ldy) = e[j];
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < kPieces; ++j)
-                            if (r0 + j * (32 / kPieces) < rows) *reinterpret_cast<uint4*>(dst + j * (32 / kPieces) * p.ldy) = e[j];
-                    }
-                } else if (lane < cols) {
-                    T* dst = y + static_cast<long long>(m0) * p.ldy + n + lane;
-                    const int live_rows = min(rows, 32);
-#pragma unroll 8
-                    for (int r = 0; r < live_rows; ++r) dst[r * p.ldy] = f8_get<T>(stage + r * kPitch + lane * sizeof(T));
-                }
+                for (int j = 0; j < 32; ++j) f[j] += __ldg(p.bias + n + min(j, top));
             }
+            if (p.drop.rng != nullptr) f8_mask32(p.drop, static_cast<unsigned long long>(m0 + lane) * p.N + n, f);
+            constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer;           // of a 32-element row
+            __syncwarp();                                                       // the last chunk's readers are through
+#pragma unroll
+            for (int j = 0; j < kPieces; ++j) f8_put16<T>(stage + lane * kPitch + 16 * j, f + j * kPer);
+            __syncwarp();
+            if (p.vec && cols == 32) {
+                const int piece = lane % kPieces, r0 = lane / kPieces;
+                T* dst = y + static_cast<long long>(m0 + r0) * p.ldy + n + piece * kPer;
+                uint4 e[kPieces];
+#pragma unroll
+                for (int j = 0; j < kPieces; ++j) e[j] = f8_get16(stage + (r0 + j * (32 / kPieces)) * kPitch + 16 * piece);
+                if (rows >= 32) {
+#pragma unroll
+                    for (int j = 0; j < kPieces; ++j) *reinterpret_cast<uint4*>(dst + j * (32 / kPieces) * p.ldy) = e[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kPieces; ++j)
+                        if (r0 + j * (32 / kPieces) < rows) *reinterpret_cast<uint4*>(dst + j * (32 / kPieces) * p.ldy) = e[j];
+                }
+            } else if (lane < cols) {
+                T* dst = y + static_cast<long long>(m0) * p.ldy + n + lane;
+                const int live_rows = min(rows, 32);
+#pragma unroll 8
+                for (int r = 0; r < live_rows; ++r) dst[r * p.ldy] = f8_get<T>(stage + r * kPitch + lane * sizeof(T));
+            }
+        };
+        auto release = [&](uint32_t buf) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) {
-                if (CG == 2) f8_arrive_leader<false>(acce0 + 8 * buf); else f8_arrive(acce0 + 8 * buf);
+            if (lane == 0) { if (CG == 2) f8_arrive_leader<false>(acce0 + 8 * buf); else f8_arrive(acce0 + 8 * buf); }
+        };
+        uint32_t item = 0;                                   // accumulators read so far
+        bool ok = true;
+        for (int t = first; t < ntiles && ok; t += step) {
+            int tm, tn;
+            f8_tile(t, p.mt, p.nt, tm, tn);
+            const int m0 = (tm * CG + rank) * kF8TileM + row0, n0 = tn * p.tile_n, rows = p.M - m0;
+            if constexpr (SUMS) {
+                // the eight warps share the columns in halves of up to 96
+                const int half = p.tile_n / 2, c0 = half * ((warp - kF8EpiWarp) >> 2);
+                float sums[kF8SumTileN / 64][32];
+                for (int q = 0; q < quads; q += kF8SumQuads, ++item) {
+                    const uint32_t buf = item & 1u;
+                    if (!(ok = f8_wait(accf0 + 8 * buf, (item >> 1) & 1u, abort_flag))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                    for (int i = 0; i < kF8SumTileN / 64; ++i) {
+                        if (32 * i >= half) break;
+                        uint32_t v[32];
+                        f8_tmem_ld32(v, tmem + buf * d_step + lanes + c0 + 32 * i);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sums[i][j] = q == 0 ? __uint_as_float(v[j]) : sums[i][j] + __uint_as_float(v[j]);
+                    }
+                    release(buf);
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < kF8SumTileN / 64; ++i) {
+                    if (32 * i >= half) break;
+                    const int n = n0 + c0 + 32 * i;
+                    if (n < p.N && rows > 0) emit(sums[i], m0, n, rows);
+                }
+            } else {
+                const int chunks = p.tile_n / 32;
+                const uint32_t buf = item & 1u;
+                if (!(ok = f8_wait(accf0 + 8 * buf, (item >> 1) & 1u, abort_flag))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t src = tmem + buf * d_step + lanes;
+                for (int i = 0; i < chunks; ++i) {
+                    const int c = 32 * (overlap && buf == 0 ? (i == 0 ? chunks - 1 : i - 1) : i), n = n0 + c;
+                    const bool live = n < p.N && rows > 0;   // the same for the whole warp
+                    uint32_t v[32];
+                    if (live) f8_tmem_ld32(v, src + c);
+                    if (overlap && i == 0) {
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) { if (CG == 2) f8_arrive_leader<false>(accp); else f8_arrive(accp); }
+                    }
+                    if (!live) continue;
+                    float f[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+                    emit(f, m0, n, rows);
+                }
+                release(buf);
+                ++item;
             }
         }
     }
@@ -815,15 +861,19 @@ struct Fp8Plan {
     int splits;              // fp8_split_kernel where not 0: blocks to a tile; tile = rows of A
 };
 
-static Fp8Plan fp8_plan(int M, int N, int kblocks)
+// fp32: the result is fp32, so a reduction over more than 2048 steps is added up from partial sums (SUMS): tiles of 64, 128 or
+// 192 columns, and no block of the split kernel gets more than that.
+static Fp8Plan fp8_plan(int M, int N, int kblocks, bool fp32)
 {
-    Fp8Plan best{1, 32, 0};
+    const bool sums = fp32 && kblocks > kF8SumsFrom;
+    Fp8Plan best{1, sums ? 64 : 32, 0};
     double least = 1e300;
     const int sms = sm_count();
     for (int cg = 1; cg <= 2; ++cg) {
         const double mt = (M + cg * kF8TileM - 1) / (cg * kF8TileM);
-        for (int tile = 32; tile <= kF8MaxTileN; tile += 32) {
-            if (tile > 32 && tile - 32 >= N) break;
+        const int unit = sums ? 64 : 32;
+        for (int tile = unit; tile <= (sums ? kF8SumTileN : kF8MaxTileN); tile += unit) {
+            if (tile > unit && tile - unit >= N) break;
             const double nt = (N + tile - 1) / tile, waves = ceil(mt * nt / (sms / cg));
             const double slice = cg == 2 ? fmax(0.22, 0.06 + 0.0013 * tile) : 0.165 + 0.00106 * tile;
             const double t = waves * (kblocks * slice + 0.4 + 0.003 * tile) + (cg == 2 ? 5.0 : 3.9);
@@ -837,7 +887,7 @@ static Fp8Plan fp8_plan(int M, int N, int kblocks)
         if (mt * nt > 16.0 * sms) continue;                  // many tiles: never the better kernel
         for (int splits = 1; splits <= 8 && splits <= kblocks; ++splits) {
             const int kbs = (kblocks + splits - 1) / splits;
-            if (kbs / 4 + 2 > kF8MaxQuads) continue;
+            if (kbs / 4 + 2 > kF8MaxQuads || (fp32 && kbs > kF8SumsFrom)) continue;
             const double waves = ceil(mt * nt * splits / sms);
             const double t = waves * (kbs * (0.14 + 0.0016 * tile) + 0.8 + 0.025 * tile + 0.06 * splits) + 3.2;
             if (t < least) { least = t; best = Fp8Plan{1, tile, splits}; }
@@ -858,15 +908,15 @@ static cudaError_t allow_smem(K kernel, bool (&done)[64])
     return e;
 }
 
-template <class T, int CG>
+template <class T, int CG, bool SUMS>
 static int launch_fp8(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Params& p, cudaStream_t s)
 {
     static bool done[64];
-    cudaError_t e = allow_smem(fp8_gemm_kernel<T, CG>, done);
+    cudaError_t e = allow_smem(fp8_gemm_kernel<T, CG, SUMS>, done);
     const int tiles = p.mt * p.nt, fit = sm_count() / CG;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(CG * (tiles < fit ? tiles : fit));
-    cfg.blockDim = dim3(kF8Threads);
+    cfg.blockDim = dim3(SUMS ? kF8SumThreads : kF8Threads);
     cfg.dynamicSmemBytes = kF8Smem;
     cfg.stream = s;
     cudaLaunchAttribute attr{};
@@ -875,15 +925,15 @@ static int launch_fp8(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Par
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = CG == 2 ? 1 : 0;
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<T, CG>, ma, mb, p);
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<T, CG, SUMS>, ma, mb, p);
     if (e != cudaSuccess) { set_error("fp8_gemm_kernel: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
     return check_launch("fp8_gemm_kernel");
 }
 
-template <class T>
+template <class T, bool SUMS>
 static int launch_fp8_cg(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Params& p, int cg, cudaStream_t s)
 {
-    return cg == 2 ? launch_fp8<T, 2>(ma, mb, p, s) : launch_fp8<T, 1>(ma, mb, p, s);
+    return cg == 2 ? launch_fp8<T, 2, SUMS>(ma, mb, p, s) : launch_fp8<T, 1, SUMS>(ma, mb, p, s);
 }
 
 template <class T>
@@ -952,7 +1002,8 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     p.a_shift = a_block_rows == 128 ? 7 : 0; p.b_shift = b_block_rows == 128 ? 7 : 0;
     p.sf_vec = aligned_to(sa, 16) && ldsa % 16 == 0 && aligned_to(sb, 16) && ldsb % 16 == 0;
     p.bias = bias; p.alpha = alpha; p.y = y; p.ldy = ldy; p.M = M; p.N = N; p.kblocks = kblocks;
-    const Fp8Plan plan = fp8_plan(M, N, kblocks);
+    const Fp8Plan plan = fp8_plan(M, N, kblocks, y_dtype == ATB_F32);
+    const bool sums = y_dtype == ATB_F32 && kblocks > kF8SumsFrom && !plan.splits;
     const DropState drop{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)};
     const uint32_t formats = (1u << 23);                     // scales are powers of two (ue8m0)
     CUtensorMap ma, mb;
@@ -992,7 +1043,7 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     p.nt = (N + p.tile_n - 1) / p.tile_n;
     ATB_REQUIRE(static_cast<long long>(p.mt) * p.nt < (1LL << 30), "too many tiles");
     const int stage = kF8TileM * 128 + p.tile_n / cg * 128;
-    p.stages = (kF8Smem - 1024 - kF8SfSlots * kF8SfSlotBytes - 4 * 32 * (32 * size + 16)) / stage;
+    p.stages = (kF8Smem - 1024 - kF8SfSlots * kF8SfSlotBytes - (sums ? kF8SumEpiWarps : kF8EpiWarps) * 32 * (32 * size + 16)) / stage;
     if (p.stages > kF8MaxStages) p.stages = kF8MaxStages;
     p.idesc = formats | (a_f8 == ATB_E5M2 ? 1u << 7 : 0u) | (b_f8 == ATB_E5M2 ? 1u << 10 : 0u) |
               (static_cast<uint32_t>(p.tile_n >> 3) << 17) | (static_cast<uint32_t>(cg) << 27);
@@ -1001,9 +1052,10 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     int rc = operand_map(&ma, a, M, K, lda, kF8TileM);
     if (rc == ATB_OK) rc = operand_map(&mb, b, N, K, ldb, p.tile_n / cg);
     if (rc != ATB_OK) return rc;
-    if (y_dtype == ATB_F32) return launch_fp8_cg<float>(ma, mb, p, cg, s);
-    if (y_dtype == ATB_BF16) return launch_fp8_cg<__nv_bfloat16>(ma, mb, p, cg, s);
-    return launch_fp8_cg<__half>(ma, mb, p, cg, s);
+    if (sums) return launch_fp8_cg<float, true>(ma, mb, p, cg, s);
+    if (y_dtype == ATB_F32) return launch_fp8_cg<float, false>(ma, mb, p, cg, s);
+    if (y_dtype == ATB_BF16) return launch_fp8_cg<__nv_bfloat16, false>(ma, mb, p, cg, s);
+    return launch_fp8_cg<__half, false>(ma, mb, p, cg, s);
 }
 
 extern "C" int atb_fp8_status(int* status)

@@ -34,27 +34,43 @@ __device__ __forceinline__ Eight<T> eight_load(const T* p)
     return e;
 }
 
-// One thread takes whole groups of 8 elements (one draw each).  VEC: 16-byte aligned tensors.
+// One thread takes whole groups of 8 elements (one draw each), kAhead of them at a time, requested together.  VEC: 16-byte
+// aligned tensors.
 template <class T, bool VEC>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* x, T* y, long long numel, DropState d, float factor)
 {
+    constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;
     const PhiloxKey key(d.rng);
-    const long long groups = (numel + 7) >> 3, stride = static_cast<long long>(gridDim.x) * blockDim.x;
-    for (long long g = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; g < groups; g += stride) {
-        const long long i0 = g << 3;
-        if (VEC && i0 + 8 <= numel) {
-            Eight<T> e = eight_load(x + i0);
-            const unsigned m = philox_keep8(key, g, d.threshold);
+    const long long whole = VEC ? numel >> 3 : 0, groups = (numel + 7) >> 3;
+    const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
+    long long g = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+    auto finish = [&](long long at, Eight<T>& e) {
+        const uint4 r = philox4x32_10(key, at);
+        const uint32_t v[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) e.v[j] = drop_store<T>((m >> j) & 1u ? drop_load(e.v[j]) * factor : 0.0f);
-            uint4* dst = reinterpret_cast<uint4*>(y + i0);
-#pragma unroll
-            for (int j = 0; j < static_cast<int>(sizeof(e) / 16); ++j) dst[j] = reinterpret_cast<const uint4*>(&e)[j];
-        } else {
-            const unsigned m = philox_keep8(key, g, d.threshold);
-            for (int j = 0; j < 8 && i0 + j < numel; ++j)
-                y[i0 + j] = drop_store<T>((m >> j) & 1u ? drop_load(x[i0 + j]) * factor : 0.0f);
+        for (int j = 0; j < 8; ++j) {
+            const unsigned h = j & 1 ? v[j >> 1] >> 16 : v[j >> 1] & 0xFFFFu;
+            e.v[j] = drop_store<T>(h >= d.threshold ? drop_load(e.v[j]) * factor : 0.0f);
         }
+        uint4* dst = reinterpret_cast<uint4*>(y + (at << 3));
+#pragma unroll
+        for (int j = 0; j < static_cast<int>(sizeof(e) / 16); ++j) __stcs(dst + j, reinterpret_cast<const uint4*>(&e)[j]);
+    };
+    for (; g + (kAhead - 1) * stride < whole; g += kAhead * stride) {
+        Eight<T> e[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) e[i] = eight_load(x + ((g + i * stride) << 3));
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) finish(g + i * stride, e[i]);
+    }
+    for (; g < whole; g += stride) {
+        Eight<T> e = eight_load(x + (g << 3));
+        finish(g, e);
+    }
+    for (; g < groups; g += stride) {                        // unaligned tensors, and what a last group is short of 8
+        const unsigned m = philox_keep8(key, g, d.threshold);
+        for (int j = 0; j < 8 && (g << 3) + j < numel; ++j)
+            y[(g << 3) + j] = drop_store<T>((m >> j) & 1u ? drop_load(x[(g << 3) + j]) * factor : 0.0f);
     }
 }
 

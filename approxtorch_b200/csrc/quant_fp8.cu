@@ -31,31 +31,67 @@ struct QuantArgs {
     uint8_t* st;      // [C or ceil(C/128), ldst]
     long long ldst;
     DropState drop;
+    bool vec;         // rows of x start on 16-byte boundaries
 };
 
-template <class T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_float<__half>(__half v) { return __half2float(v); }
+// What a lane holds of a row: 16 bytes in the input's own type (8 bf16 or fp16, 4 fp32).  Magnitudes are compared in that
+// type, two halves at a time where it has 16 bits; a NaN is kept as the larger.  Element order: word by word, low half first.
+template <class T> struct Piece;
+template <> struct Piece<float> {
+    static constexpr int kElems = 4;
+    static __device__ __forceinline__ unsigned mag(unsigned w) { return w & 0x7FFFFFFFu; }
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return max(a, b); }
+    static __device__ __forceinline__ unsigned fp32_bits(unsigned m) { return m; }               // of a whole word's maximum
+    template <int J> static __device__ __forceinline__ float get(const unsigned (&w)[4]) { return __uint_as_float(w[J]); }
+};
+template <> struct Piece<__nv_bfloat16> {
+    static constexpr int kElems = 8;
+    static __device__ __forceinline__ unsigned mag(unsigned w) { return w & 0x7FFF7FFFu; }
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b)
+    {
+        const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+        return *reinterpret_cast<const unsigned*>(&m);
+    }
+    static __device__ __forceinline__ unsigned fp32_bits(unsigned m) { return max(m << 16, m & 0xFFFF0000u); }   // of both halves
+    template <int J> static __device__ __forceinline__ float get(const unsigned (&w)[4])
+    {
+        return __uint_as_float(J & 1 ? w[J / 2] & 0xFFFF0000u : w[J / 2] << 16);
+    }
+};
+template <> struct Piece<__half> {
+    static constexpr int kElems = 8;
+    static __device__ __forceinline__ unsigned mag(unsigned w) { return w & 0x7FFF7FFFu; }
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b)
+    {
+        const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+        return *reinterpret_cast<const unsigned*>(&m);
+    }
+    static __device__ __forceinline__ unsigned fp32_bits(unsigned m)
+    {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
+        return max(__float_as_uint(f.x), __float_as_uint(f.y));
+    }
+    template <int J> static __device__ __forceinline__ float get(const unsigned (&w)[4])
+    {
+        const __half2 h = *reinterpret_cast<const __half2*>(&w[J / 2]);
+        return J & 1 ? __high2float(h) : __low2float(h);
+    }
+};
 
-// 8 consecutive elements of a row from column c on (beyond the row's end: zeros)
-template <class T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ row, long long c, long long C, float (&v)[8])
+// elements c ... of a row (beyond the row's end: zeros)
+template <class T>
+__device__ __forceinline__ void load_piece(const T* __restrict__ row, long long c, long long C, unsigned (&w)[4])
 {
-    if (VEC && c + 8 <= C) {
-        T raw[8];
-        const uint4* src = reinterpret_cast<const uint4*>(row + c);
+    constexpr int kElems = Piece<T>::kElems;
 #pragma unroll
-        for (int i = 0; i < static_cast<int>(sizeof(raw) / 16); ++i) reinterpret_cast<uint4*>(raw)[i] = __ldcs(src + i);
+    for (int i = 0; i < 4; ++i) w[i] = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_float(raw[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < C ? to_float(row[c + i]) : 0.0f;
+    for (int i = 0; i < kElems; ++i) {
+        if (c + i >= C) continue;
+        if constexpr (kElems == 4) w[i] = __float_as_uint(row[c + i]);
+        else w[i / 2] |= static_cast<unsigned>(reinterpret_cast<const unsigned short*>(row)[c + i]) << (16 * (i & 1));
     }
 }
-
-__device__ __forceinline__ unsigned magnitude(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // scale byte of a block from its largest magnitude's bits; 448 = 1.75 * 2^8, 57344 = 1.75 * 2^15
 template <bool E5>
@@ -80,192 +116,241 @@ __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d)
     return lo | (hi << 16);
 }
 
-__device__ __forceinline__ unsigned max16(unsigned v)      // over the 16 lanes that share a block of 128
+// clears what is dropped: bit j of keep stands for element j of the piece
+template <class T>
+__device__ __forceinline__ void drop_bits(unsigned (&w)[4], unsigned keep)
 {
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-    return v;
-}
-
-// ---- 1 x 128 blocks along the rows, one layout ---------------------------------------------------------------------
-// 16 lanes x 8 elements = one block; a block of threads takes 16 at a time.
-template <class T, bool E5, bool VEC, bool DROP>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a)
-{
-    const long long nb = (a.C + 127) >> 7, total = a.R * nb;
-    const int sub = threadIdx.x >> 4, l16 = threadIdx.x & 15;
-    for (long long base = static_cast<long long>(blockIdx.x) * 16; base < total; base += static_cast<long long>(gridDim.x) * 16) {
-        const long long id = base + sub;
-        const bool live = id < total;
-        const long long r = live ? id / nb : 0, b = live ? id - r * nb : 0, c = (b << 7) + l16 * 8;
-        float v[8];
-        load8<T, VEC>(static_cast<const T*>(a.x) + r * a.ldx, live ? c : a.C, a.C, v);
-        if (DROP) {
-            const PhiloxKey key(a.drop.rng);
-            const unsigned m = philox_keep8_at(key, static_cast<unsigned long long>(r * a.C + c), a.drop.threshold);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = (m >> i) & 1u ? v[i] : 0.0f;
-        }
-        unsigned amax = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax = max(amax, magnitude(v[i]));
-        amax = max16(amax);
-        const unsigned byte = scale_byte<E5>(amax);
-        const float inv = inverse_scale(byte);
-        if (live) {
-            if (c < a.ldq)
-                *reinterpret_cast<uint2*>(a.q + r * a.ldq + c) =
-                    make_uint2(pack4<E5>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-                               pack4<E5>(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
-            if (l16 == 0) a.s[r * a.lds + b] = static_cast<uint8_t>(byte);
-        }
+    for (int j = 0; j < Piece<T>::kElems; ++j) {
+        if ((keep >> j) & 1u) continue;
+        if (Piece<T>::kElems == 4) w[j] = 0;
+        else w[j / 2] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
     }
 }
-
-// ---- both layouts in one pass over x ---------------------------------------------------------------------------------
-// One block of threads = a 128 x 128 tile, each thread an 8 x 8 piece in registers: row maxima over 16 lanes, column
-// maxima over the thread's rows and then over the tile, both images from the same registers.  SQUARE: one scale for the
-// whole tile (weights) instead of one for each row and for each column.  The transposed image turns through shared
-// memory so that both leave in 128-byte rows.
-//
-// The turned tile is 128 rows of 128 bytes; the 16-byte piece p of row c sits at place p ^ ((c >> 3) & 7), so that the
-// 16 lanes that write one column piece each (rows 8 apart) spread over all banks.  (A padded pitch cannot: eight rows
-// of any 16-byte multiple are a multiple of the 128-byte bank cycle.)
-__device__ __forceinline__ int turn_at(int c, int byte) { return c * 128 + (byte ^ (((c >> 3) & 7) << 4)); }
-
-template <class T, bool E5, bool VEC, bool DROP, bool SQUARE>
-__global__ void __launch_bounds__(256, 2) quantize_tile_kernel(const QuantArgs a)
+// the same from the draws: word i of d holds the 16 bits of elements 2 i and 2 i + 1 of a group of 8
+__device__ __forceinline__ void drop_draws8(unsigned (&w)[4], const uint4& d, unsigned high)      // high = threshold << 16
 {
-    __shared__ unsigned s_col[8][128];
-    __shared__ __align__(16) uint8_t s_turn[128 * 128];
-    const int warp = threadIdx.x >> 5, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const long long r0 = static_cast<long long>(blockIdx.y) * 128, c0 = static_cast<long long>(blockIdx.x) * 128;
-    const long long c = c0 + tx * 8;
-    float v[8][8];
+    const unsigned v[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const long long r = r0 + ty * 8 + i;
-        load8<T, VEC>(static_cast<const T*>(a.x) + (r < a.R ? r : 0) * a.ldx, r < a.R ? c : a.C, a.C, v[i]);
+    for (int i = 0; i < 4; ++i) {
+        if (v[i] < high) w[i] &= 0x0000FFFFu;
+        if ((v[i] << 16) < high) w[i] &= 0xFFFF0000u;
+    }
+}
+__device__ __forceinline__ void drop_draws4(unsigned (&w)[4], unsigned d0, unsigned d1, unsigned high)
+{
+    if ((d0 << 16) < high) w[0] = 0;
+    if (d0 < high) w[1] = 0;
+    if ((d1 << 16) < high) w[2] = 0;
+    if (d1 < high) w[3] = 0;
+}
+
+// ---- the quantiser ------------------------------------------------------------------------------------------------------
+// A block of threads takes a tile of 128 rows x 128 columns; a lane holds 8 rows x 16 bytes of it in registers, in the
+// input's own type, so that enough threads are resident for their loads to cover the memory's latency.
+//   kRows     one layout, a scale for each row's 128 elements; warps do not meet
+//   kBoth     and the transposed layout, a scale for each column's 128 elements, from the same registers
+//   kSquare   one scale for the tile (weights), one or both layouts
+// A row's block is 16 (fp32: 32) lanes.  The maxima of a lane's 8 rows go through an exchange that halves the rows a lane
+// deals with in every step, so that a lane ends with one row, makes its scale once and hands 1 / scale around: instructions
+// are what bounds this kernel besides memory, and a scale made by every lane for every row was a third of them.
+// The transposed image turns through shared memory so that it leaves in 128-byte rows: column c is row c of s_turn, its
+// 8-byte pieces (8 rows of one lane) permuted by the column so that the lanes of a write spread over all banks.
+enum QuantMode { kRows = 0, kBoth = 1, kSquare = 2 };
+template <class T> constexpr int kQuantThreads = 16 * 128 / Piece<T>::kElems;      // 256, fp32: 512
+
+template <class T, bool E5, bool DROP, int MODE>
+__global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quantize_kernel(const QuantArgs a)
+{
+    using P = Piece<T>;
+    constexpr int kElems = P::kElems, kLanes = 128 / kElems;                       // of a row
+    constexpr int kWarps = kQuantThreads<T> / 32, kWords = 128 * static_cast<int>(sizeof(T)) / 4;   // words of a row
+    __shared__ __align__(16) unsigned s_max[MODE == kRows ? 1 : kWarps][MODE == kRows ? 4 : kWords];
+    __shared__ __align__(16) float s_inv[MODE == kBoth ? 128 : 4];
+    __shared__ __align__(16) uint8_t s_turn[MODE == kRows ? 16 : 128 * 128];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, in_row = lane % kLanes;
+    const int strip = threadIdx.x / kLanes;                                        // of 8 rows, 0 .. 15
+    const long long r0 = static_cast<long long>(blockIdx.y) * 128 + strip * 8, c0 = static_cast<long long>(blockIdx.x) * 128;
+    const long long c = c0 + in_row * kElems;
+    const int rows = static_cast<int>(max(0ll, min(8ll, a.R - r0)));
+    if (MODE == kRows && a.R <= r0 - (strip * 8) % (32 / kLanes * 8)) return;      // nothing for this warp
+    const T* const x = static_cast<const T*>(a.x) + r0 * a.ldx + c;
+
+    unsigned v[8][4];
+    if (a.vec && rows == 8 && c0 + 128 <= a.C) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint4 q = __ldcs(reinterpret_cast<const uint4*>(x + i * a.ldx));
+            v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
+        }
+    } else {
+        const T* const base = static_cast<const T*>(a.x) + (rows ? r0 : 0) * a.ldx;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) load_piece(base + (i < rows ? i : 0) * a.ldx, i < rows ? c : a.C, a.C, v[i]);
     }
     if (DROP) {
         const PhiloxKey key(a.drop.rng);
+        const unsigned high = a.drop.threshold << 16;
+        if (a.drop.threshold >= 65536u) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const unsigned m = philox_keep8_at(key, static_cast<unsigned long long>((r0 + ty * 8 + i) * a.C + c), a.drop.threshold);
+            for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = (m >> j) & 1u ? v[i][j] : 0.0f;
+                for (int j = 0; j < 4; ++j) v[i][j] = 0;
+        } else if ((a.C & 7) == 0) {
+            const unsigned long long g = static_cast<unsigned long long>(r0 * a.C + c) >> 3, row = static_cast<unsigned long long>(a.C) >> 3;
+            if (kElems == 8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) drop_draws8(v[i], philox4x32_10(key, g + i * row), high);
+            } else {
+                // a group of 8 elements is two lanes' share of a row: each draws for four rows and they exchange halves
+                const bool odd = lane & 1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint4 d = philox4x32_10(key, g + (odd ? i + 4 : i) * row);
+                    const unsigned e0 = __shfl_xor_sync(0xFFFFFFFFu, odd ? d.x : d.z, 1), e1 = __shfl_xor_sync(0xFFFFFFFFu, odd ? d.y : d.w, 1);
+                    drop_draws4(v[i], odd ? e0 : d.x, odd ? e1 : d.y, high);
+                    drop_draws4(v[i + 4], odd ? d.z : e0, odd ? d.w : e1, high);
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i) {
+                const unsigned keep = philox_keep8_at(key, static_cast<unsigned long long>((r0 + i) * a.C + c), a.drop.threshold);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) if (k == i) drop_bits<T>(v[k], keep);
+            }
         }
     }
-    // maxima
-    unsigned rowmax[8], colmax[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) colmax[j] = 0;
+
+    // maxima of the rows, and of the columns over this lane's rows
+    unsigned top[8], col[4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        rowmax[i] = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const unsigned m = magnitude(v[i][j]);
-            rowmax[i] = max(rowmax[i], m);
-            colmax[j] = max(colmax[j], m);
+        const unsigned m0 = P::mag(v[i][0]), m1 = P::mag(v[i][1]), m2 = P::mag(v[i][2]), m3 = P::mag(v[i][3]);
+        top[i] = P::larger(P::larger(m0, m1), P::larger(m2, m3));
+        if (MODE == kBoth) {
+            col[0] = i ? P::larger(col[0], m0) : m0; col[1] = i ? P::larger(col[1], m1) : m1;
+            col[2] = i ? P::larger(col[2], m2) : m2; col[3] = i ? P::larger(col[3], m3) : m3;
         }
     }
-    unsigned rbyte[8], cbyte[8];
-    if (SQUARE) {
-        unsigned m = 0;
+    float inv[8];                                            // 1 / scale of this lane's rows
+    if (MODE == kSquare) {
+        unsigned m = top[0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, rowmax[i]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        if ((threadIdx.x & 31) == 0) s_col[warp][0] = m;
+        for (int i = 1; i < 8; ++i) m = P::larger(m, top[i]);
+        m = __reduce_max_sync(0xFFFFFFFFu, P::fp32_bits(m));
+        if (lane == 0) s_max[warp][0] = m;
         __syncthreads();
-        m = 0;
+        m = __reduce_max_sync(0xFFFFFFFFu, lane < kWarps ? s_max[lane][0] : 0u);
+        const unsigned byte = scale_byte<E5>(m);
+        inv[0] = inverse_scale(byte);
 #pragma unroll
-        for (int w = 0; w < 8; ++w) m = max(m, s_col[w][0]);
-        const unsigned b = scale_byte<E5>(m);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) { rbyte[i] = b; cbyte[i] = b; }
+        for (int i = 1; i < 8; ++i) inv[i] = inv[0];
         if (threadIdx.x == 0) {
-            a.s[blockIdx.y * a.lds + blockIdx.x] = static_cast<uint8_t>(b);
-            if (a.st) a.st[blockIdx.x * a.ldst + blockIdx.y] = static_cast<uint8_t>(b);
+            a.s[blockIdx.y * a.lds + blockIdx.x] = static_cast<uint8_t>(byte);
+            if (a.st) a.st[blockIdx.x * a.ldst + blockIdx.y] = static_cast<uint8_t>(byte);
         }
     } else {
+        if (MODE == kBoth) {
+            if (kLanes == 16) {                              // the warp's two strips
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            rbyte[i] = scale_byte<E5>(max16(rowmax[i]));
-            const long long r = r0 + ty * 8 + i;
-            if (tx == 0 && r < a.R) a.s[r * a.lds + blockIdx.x] = static_cast<uint8_t>(rbyte[i]);
+                for (int j = 0; j < 4; ++j) col[j] = P::larger(col[j], __shfl_xor_sync(0xFFFFFFFFu, col[j], 16));
+            }
+            if (lane < kLanes) *reinterpret_cast<uint4*>(&s_max[warp][in_row * 4]) = make_uint4(col[0], col[1], col[2], col[3]);
+        }
+        // 8 rows x kLanes lanes: with every step a lane keeps half of its rows, the upper half if its bit is set
+#pragma unroll
+        for (int half = 4, bit = kLanes / 2; half >= 1; half >>= 1, bit >>= 1) {
+            const bool upper = lane & bit;
+#pragma unroll
+            for (int i = 0; i < half; ++i) {
+                const unsigned keep = upper ? top[i + half] : top[i], give = upper ? top[i] : top[i + half];
+                top[i] = P::larger(keep, __shfl_xor_sync(0xFFFFFFFFu, give, bit));
+            }
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) colmax[j] = max(colmax[j], __shfl_xor_sync(0xFFFFFFFFu, colmax[j], 16));
-        if ((threadIdx.x & 31) < 16) {
+        for (int bit = kLanes / 16; bit >= 1; bit >>= 1) top[0] = P::larger(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], bit));
+        const int row = in_row / (kLanes / 8);               // the one this lane is left with
+        const unsigned byte = scale_byte<E5>(P::fp32_bits(top[0]));
+        const float mine = inverse_scale(byte);
+        if (in_row % (kLanes / 8) == 0 && row < rows) a.s[(r0 + row) * a.lds + blockIdx.x] = static_cast<uint8_t>(byte);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s_col[warp][tx * 8 + j] = colmax[j];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            unsigned m = 0;
-#pragma unroll
-            for (int w = 0; w < 8; ++w) m = max(m, s_col[w][tx * 8 + j]);
-            cbyte[j] = scale_byte<E5>(m);
-            if (ty == 0 && c + j < a.C) a.st[(c + j) * a.ldst + blockIdx.y] = static_cast<uint8_t>(cbyte[j]);
-        }
+        for (int i = 0; i < 8; ++i) inv[i] = __shfl_sync(0xFFFFFFFFu, mine, i * (kLanes / 8), kLanes);
     }
     // the image as it lies
+    uint8_t* const q = a.q + r0 * a.ldq + c;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const long long r = r0 + ty * 8 + i;
-        const float inv = inverse_scale(rbyte[i]);
-        if (r < a.R && c < a.ldq)
-            *reinterpret_cast<uint2*>(a.q + r * a.ldq + c) =
-                make_uint2(pack4<E5>(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
-                           pack4<E5>(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv));
+        const unsigned lo = pack4<E5>(P::template get<0>(v[i]) * inv[i], P::template get<1>(v[i]) * inv[i],
+                                      P::template get<2>(v[i]) * inv[i], P::template get<3>(v[i]) * inv[i]);
+        if constexpr (kElems == 8) {
+            const unsigned hi = pack4<E5>(P::template get<4>(v[i]) * inv[i], P::template get<5>(v[i]) * inv[i],
+                                          P::template get<6>(v[i]) * inv[i], P::template get<7>(v[i]) * inv[i]);
+            if (i < rows && c < a.ldq) *reinterpret_cast<uint2*>(q + i * a.ldq) = make_uint2(lo, hi);
+        } else {
+            if (i < rows && c < a.ldq) *reinterpret_cast<unsigned*>(q + i * a.ldq) = lo;
+        }
     }
-    if (a.qt == nullptr) return;
-    // the transposed image: 8 rows of one column are 8 consecutive bytes of it
+    if (MODE == kRows || a.qt == nullptr) return;
+
+    if (MODE == kBoth) {
+        __syncthreads();
+        if (threadIdx.x < kWords) {                          // a word's columns (one, or two halves)
+            unsigned m = s_max[0][threadIdx.x];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float inv = inverse_scale(cbyte[j]);
-        *reinterpret_cast<uint2*>(s_turn + turn_at(tx * 8 + j, ty * 8)) =
-            make_uint2(pack4<E5>(v[0][j] * inv, v[1][j] * inv, v[2][j] * inv, v[3][j] * inv),
-                       pack4<E5>(v[4][j] * inv, v[5][j] * inv, v[6][j] * inv, v[7][j] * inv));
+            for (int w = 1; w < kWarps; ++w) m = P::larger(m, s_max[w][threadIdx.x]);
+            constexpr int kPer = 128 / kWords;
+#pragma unroll
+            for (int h = 0; h < kPer; ++h) {
+                const int cc = threadIdx.x * kPer + h;
+                const unsigned one = kPer == 1 ? m : h ? m >> 16 : m & 0xFFFFu;
+                const unsigned byte = scale_byte<E5>(P::fp32_bits(one));
+                s_inv[cc] = inverse_scale(byte);
+                if (c0 + cc < a.C) a.st[(c0 + cc) * a.ldst + blockIdx.y] = static_cast<uint8_t>(byte);
+            }
+        }
+        __syncthreads();
     }
+    auto turn = [&](int j, float f0, float f1, float f2, float f3, float f4, float f5, float f6, float f7) {
+        const float by = MODE == kBoth ? s_inv[in_row * kElems + j] : inv[0];
+        const int cc = in_row * kElems + j;
+        *reinterpret_cast<uint2*>(s_turn + cc * 128 + ((strip ^ in_row % 16) << 3)) =
+            make_uint2(pack4<E5>(f0 * by, f1 * by, f2 * by, f3 * by), pack4<E5>(f4 * by, f5 * by, f6 * by, f7 * by));
+    };
+#define ATB_TURN(J) turn(J, P::template get<J>(v[0]), P::template get<J>(v[1]), P::template get<J>(v[2]), P::template get<J>(v[3]), \
+                         P::template get<J>(v[4]), P::template get<J>(v[5]), P::template get<J>(v[6]), P::template get<J>(v[7]))
+    ATB_TURN(0); ATB_TURN(1); ATB_TURN(2); ATB_TURN(3);
+    if constexpr (kElems == 8) { ATB_TURN(4); ATB_TURN(5); ATB_TURN(6); ATB_TURN(7); }
+#undef ATB_TURN
     __syncthreads();
+    const long long rt = static_cast<long long>(blockIdx.y) * 128;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int cc = (threadIdx.x >> 3) + 32 * i, k = (threadIdx.x & 7) * 16;
-        if (c0 + cc < a.C && r0 + k < a.ldqt)
-            *reinterpret_cast<uint4*>(a.qt + (c0 + cc) * a.ldqt + r0 + k) = *reinterpret_cast<const uint4*>(s_turn + turn_at(cc, k));
+    for (int i = 0; i < 1024 / kQuantThreads<T>; ++i) {
+        const int cc = (threadIdx.x >> 3) + kQuantThreads<T> / 8 * i, piece = threadIdx.x & 7, by = cc / kElems % 16;
+        uint4 o = *reinterpret_cast<const uint4*>(s_turn + cc * 128 + ((piece ^ (by >> 1)) << 4));
+        if (by & 1) o = make_uint4(o.z, o.w, o.x, o.y);
+        if (c0 + cc < a.C && rt + piece * 16 < a.ldqt) *reinterpret_cast<uint4*>(a.qt + (c0 + cc) * a.ldqt + rt + piece * 16) = o;
     }
 }
 
-template <class T, bool E5, bool VEC, bool DROP>
-static int launch_quantize2(const QuantArgs& a, bool square, cudaStream_t s)
+template <class T, bool E5>
+static int launch_quantize(QuantArgs a, bool square, cudaStream_t s)
 {
-    if (a.qt == nullptr && !square) {
-        const long long total = a.R * ((a.C + 127) >> 7);
-        quantize_rows_kernel<T, E5, VEC, DROP><<<grid_for(total, 16, 16 * sm_count()), 256, 0, s>>>(a);
-        return check_launch("quantize_rows_kernel");
-    }
-    const dim3 grid(static_cast<unsigned>((a.C + 127) >> 7), static_cast<unsigned>((a.R + 127) >> 7));
-    ATB_REQUIRE((a.R + 127) >> 7 <= 65535, "too many rows");
-    if (square) quantize_tile_kernel<T, E5, VEC, false, true><<<grid, 256, 0, s>>>(a);
-    else quantize_tile_kernel<T, E5, VEC, DROP, false><<<grid, 256, 0, s>>>(a);
-    return check_launch("quantize_tile_kernel");
-}
-
-template <class T>
-static int launch_quantize(const QuantArgs& a, bool e5, bool square, cudaStream_t s)
-{
-    const bool vec = aligned_to(a.x, 16) && (a.ldx * static_cast<long long>(sizeof(T))) % 16 == 0;
+    const long long nbt = (a.R + 127) >> 7;
+    ATB_REQUIRE(nbt <= 65535, "too many rows");
+    ATB_REQUIRE((a.C + 127) >> 7 < (1ll << 31), "too many columns");
+    const dim3 grid(static_cast<unsigned>((a.C + 127) >> 7), static_cast<unsigned>(nbt));
+    a.vec = aligned_to(a.x, 16) && (a.ldx * static_cast<long long>(sizeof(T))) % 16 == 0;
     const bool drop = a.drop.rng != nullptr;
-    if (e5) {
-        if (vec) return drop ? launch_quantize2<T, true, true, true>(a, square, s) : launch_quantize2<T, true, true, false>(a, square, s);
-        return drop ? launch_quantize2<T, true, false, true>(a, square, s) : launch_quantize2<T, true, false, false>(a, square, s);
+    if (square) quantize_kernel<T, E5, false, kSquare><<<grid, kQuantThreads<T>, 0, s>>>(a);
+    else if (a.qt != nullptr) {
+        if (drop) quantize_kernel<T, E5, true, kBoth><<<grid, kQuantThreads<T>, 0, s>>>(a);
+        else quantize_kernel<T, E5, false, kBoth><<<grid, kQuantThreads<T>, 0, s>>>(a);
+    } else {
+        if (drop) quantize_kernel<T, E5, true, kRows><<<grid, kQuantThreads<T>, 0, s>>>(a);
+        else quantize_kernel<T, E5, false, kRows><<<grid, kQuantThreads<T>, 0, s>>>(a);
     }
-    if (vec) return drop ? launch_quantize2<T, false, true, true>(a, square, s) : launch_quantize2<T, false, true, false>(a, square, s);
-    return drop ? launch_quantize2<T, false, false, true>(a, square, s) : launch_quantize2<T, false, false, false>(a, square, s);
+    return check_launch("quantize_kernel");
 }
 
 }  // namespace atb
@@ -290,11 +375,11 @@ extern "C" int atb_fp8_quantize(const void* x, int x_dtype, long long R, long lo
     ATB_REQUIRE(rng == nullptr || block_rows == 1, "dropout goes with blocks of one row");
     ATB_REQUIRE(drop_threshold == 0 || (rng != nullptr && aligned_to(rng, 8)), "dropout needs an 8-byte aligned state");
     QuantArgs a{x, R, C, ldx, static_cast<uint8_t*>(q), ldq, s, lds, static_cast<uint8_t*>(qt), ldqt, st, ldst,
-                DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)}};
+                DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)}, false};
     cudaStream_t stm = static_cast<cudaStream_t>(stream);
     const bool e5 = f8 == ATB_E5M2, square = block_rows == 128;
-    if (x_dtype == ATB_F32) return launch_quantize<float>(a, e5, square, stm);
-    if (x_dtype == ATB_BF16) return launch_quantize<__nv_bfloat16>(a, e5, square, stm);
-    if (x_dtype == ATB_F16) return launch_quantize<__half>(a, e5, square, stm);
+    if (x_dtype == ATB_F32) return e5 ? launch_quantize<float, true>(a, square, stm) : launch_quantize<float, false>(a, square, stm);
+    if (x_dtype == ATB_BF16) return e5 ? launch_quantize<__nv_bfloat16, true>(a, square, stm) : launch_quantize<__nv_bfloat16, false>(a, square, stm);
+    if (x_dtype == ATB_F16) return e5 ? launch_quantize<__half, true>(a, square, stm) : launch_quantize<__half, false>(a, square, stm);
     return fail_invalid("x must be fp32, bf16 or fp16");
 }

@@ -40,7 +40,8 @@ template <class T, bool VEC>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* x, T* y, long long numel, DropState d, float factor)
 {
     constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;
-    const PhiloxKey key(d.rng);
+    PhiloxKey key(d.rng);
+    key.settle();
     const long long whole = VEC ? numel >> 3 : 0, groups = (numel + 7) >> 3;
     const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
     long long g = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;

@@ -24,7 +24,19 @@ struct PhiloxKey {
         k0 = static_cast<uint32_t>(seed); k1 = static_cast<uint32_t>(seed >> 32);
         o0 = static_cast<uint32_t>(off); o1 = static_cast<uint32_t>(off >> 32);
     }
+    // by a converged warp: the key in uniform registers, where the ten round keys are made once for all of a thread's calls
+    __device__ __forceinline__ void settle()
+    {
+        k0 = __reduce_max_sync(0xFFFFFFFFu, k0);
+        k1 = __reduce_max_sync(0xFFFFFFFFu, k1);
+    }
 };
+
+// both halves of a product by one instruction (a 64-bit product in C costs 14.6 us instead of 11.2 us for 2^25 elements)
+__device__ __forceinline__ void philox_product(uint32_t a, uint32_t b, uint32_t& hi, uint32_t& lo)
+{
+    asm("{\n\t.reg .b64 t;\n\tmul.wide.u32 t, %2, %3;\n\tmov.b64 {%0, %1}, t;\n\t}" : "=r"(lo), "=r"(hi) : "r"(a), "r"(b));
+}
 
 __device__ __forceinline__ uint4 philox4x32_10(const PhiloxKey& key, unsigned long long group)
 {
@@ -32,9 +44,9 @@ __device__ __forceinline__ uint4 philox4x32_10(const PhiloxKey& key, unsigned lo
     uint32_t k0 = key.k0, k1 = key.k1;
 #pragma unroll
     for (int r = 0; r < 10; ++r) {
-        // (both halves asked for by name: a 64-bit product in C costs 14.6 us instead of 11.2 us for 2^25 elements)
-        const uint32_t ah = __umulhi(c0, 0xD2511F53u), al = c0 * 0xD2511F53u;
-        const uint32_t bh = __umulhi(c2, 0xCD9E8D57u), bl = c2 * 0xCD9E8D57u;
+        uint32_t ah, al, bh, bl;
+        philox_product(c0, 0xD2511F53u, ah, al);
+        philox_product(c2, 0xCD9E8D57u, bh, bl);
         c0 = bh ^ c1 ^ k0;
         c1 = bl;
         c2 = ah ^ c3 ^ k1;

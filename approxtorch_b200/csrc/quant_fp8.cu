@@ -189,7 +189,8 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
         for (int i = 0; i < 8; ++i) load_piece(base + (i < rows ? i : 0) * a.ldx, i < rows ? c : a.C, a.C, v[i]);
     }
     if (DROP) {
-        const PhiloxKey key(a.drop.rng);
+        PhiloxKey key(a.drop.rng);
+        key.settle();
         const unsigned high = a.drop.threshold << 16;
         if (a.drop.threshold >= 65536u) {
 #pragma unroll

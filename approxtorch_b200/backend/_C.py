@@ -96,6 +96,24 @@ for _name, (_res, _args) in _SIGNATURES.items():
 EXPORTED = tuple(_SIGNATURES)
 
 
+def _load_binding():
+    """The native binding (``csrc/binding/binding.cpp``) of the 8-bit floating point operators and dropout; it finds the
+    library above beside itself."""
+    import importlib.machinery
+    import importlib.util
+    import torch  # noqa: F401  (its libraries have to be in the process)
+    path = os.path.join(_PKG, "lib", "_binding.so")
+    if not os.path.exists(path):
+        raise ImportError(f"{path} is missing: build it first with `python -m approxtorch_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("_binding", path)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
+    loader.exec_module(module)
+    return module
+
+
+binding = _load_binding()
+
+
 def last_error() -> str:
     msg = lib.atb_last_error()
     return msg.decode("utf-8", "replace") if msg else ""

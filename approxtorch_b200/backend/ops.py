@@ -425,104 +425,34 @@ def decode_table(device, offset: int) -> Tensor:
 
 
 # --------------------------------------------------------------------------- 8-bit floating point, counter-based dropout
-_FLOAT_CODE = {torch.float32: F32, torch.bfloat16: 3, torch.float16: 4}
-_F8_CODE = {torch.float8_e4m3fn: 5, torch.float8_e5m2: 6}
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _enqueue(name: str, device: torch.device, *args) -> None:
-    """Call a C-ABI entry on the device's current stream, with that device current."""
-    fn = getattr(_lib, name)
-    if torch.cuda.current_device() == device.index:
-        status = fn(*args, _raw_stream(device.index))
-    else:
-        with torch.cuda.device(device):
-            status = fn(*args, _raw_stream(device.index))
-    if status:
-        _check(status, name)
+# Checks, outputs and launches of these are native (csrc/binding/binding.cpp).  Conventions as above: fresh outputs on the
+# input's device, the current stream, no synchronisation, RuntimeError before any launch; inputs that the kernels can
+# read as they lie (a row pitch, an offset) are not copied.
+_native = _C.binding
 
 
 def drop_threshold(p: float) -> int:
     """The drop rate as the generator holds it: round(p 65536) of 65536."""
-    _require(0.0 <= p <= 1.0, f"the drop rate must lie in [0, 1], got {p}")
-    return round(p * 65536)
+    return _native.drop_threshold(p)
 
 
 def drop_factor(p: float) -> float:
     """1 / (1 - rate) for the rounded rate (0 where everything is dropped)."""
-    t = drop_threshold(p)
-    return 0.0 if t == 65536 else 65536.0 / (65536 - t)
+    return _native.drop_factor(p)
 
 
-def _drop_state(p: float, rng: Tensor | None, device: torch.device):
-    """(threshold, address of {seed, offset}); (0, None) where nothing is dropped."""
-    t = drop_threshold(p)
-    if t == 0:
-        return 0, None
-    _require(isinstance(rng, Tensor) and rng.dtype == torch.int64 and rng.numel() == 2 and rng.is_contiguous()
-             and rng.device == device, "rng must be a contiguous int64 tensor {seed, offset} on the input's device")
-    return t, rng.data_ptr()
-
-
-def dropout(x: Tensor, p: float, rng: Tensor) -> Tensor:
+def dropout(x: Tensor, p: float, rng: Tensor | None) -> Tensor:
     """x / (1 - p) where kept, 0 elsewhere; the mask is drawn from (seed, offset, element number) and never stored.
 
     ``rng``: int64 {seed, offset} on x's device.  The same call on the incoming gradient is the backward pass.  ``p`` is
     rounded to a multiple of 2^-16.  fp32, bf16 or fp16; elements are numbered in row-major order whatever the strides."""
-    _require_cuda(("x", x))
-    _require(x.dtype in _FLOAT_CODE, "x must be float32, bfloat16 or float16")
-    threshold, state = _drop_state(p, rng, x.device)
-    x = x.contiguous()
-    if threshold == 0:
-        return x.clone()
-    y = torch.empty_like(x)
-    if y.numel():
-        _enqueue("atb_dropout", x.device, x.data_ptr(), y.data_ptr(), _FLOAT_CODE[x.dtype], x.numel(), threshold, state)
-    return y
+    return _native.dropout(x, p, rng)
 
 
 def dropout_advance(rng: Tensor) -> Tensor:
     """A copy of ``rng`` = {seed, offset} to draw from, after which the offset in ``rng`` moves on by one.  One launch and
     no host work, so every replay of a captured graph draws anew."""
-    _require_cuda(("rng", rng))
-    _require(rng.dtype == torch.int64 and rng.numel() == 2 and rng.is_contiguous(), "rng must be a contiguous int64 tensor {seed, offset}")
-    taken = torch.empty_like(rng)
-    _enqueue("atb_dropout_advance", rng.device, rng.data_ptr(), taken.data_ptr())
-    return taken
-
-
-def _padded(rows: int, cols: int, multiple: int, dtype: torch.dtype, device) -> Tensor:
-    """[rows, cols] of a 1-byte type whose row pitch is a multiple of ``multiple`` bytes."""
-    if cols % multiple == 0:
-        return torch.empty((rows, cols), dtype=dtype, device=device)
-    pitch = -(-cols // multiple) * multiple
-    return torch.empty((rows, pitch), dtype=torch.uint8, device=device).view(dtype)[:, :cols]
-
-
-def _fp8_quantize(x: Tensor, dtype: torch.dtype, block_rows: int, transposed: bool, drop_p: float, rng: Tensor | None):
-    _require_cuda(("x", x))
-    _require(x.dtype in _FLOAT_CODE, "x must be float32, bfloat16 or float16")
-    _require(dtype in _F8_CODE, "dtype must be torch.float8_e4m3fn or torch.float8_e5m2")
-    _require(x.dim() == 2, "x must have shape [R, C]")
-    dev = x.device
-    threshold, state = _drop_state(drop_p, rng, dev)
-    R, C = x.shape
-    if not ((C == 1 or x.stride(1) == 1) and (R == 1 or x.stride(0) >= C)):
-        x = x.contiguous()
-    nb, nbt = -(-C // 128), -(-R // 128)
-    e8 = torch.float8_e8m0fnu
-    q = _padded(R, C, 16, dtype, dev)
-    s = _padded(R if block_rows == 1 else nbt, nb, 16, e8, dev)
-    qt = st = None
-    if transposed:
-        qt = _padded(C, R, 16, dtype, dev)
-        st = _padded(C if block_rows == 1 else nb, nbt, 16, e8, dev)
-    if R and C:
-        _enqueue("atb_fp8_quantize", dev, x.data_ptr(), _FLOAT_CODE[x.dtype], R, C, x.stride(0) if R > 1 else C,
-                 _F8_CODE[dtype], block_rows, q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0),
-                 None if qt is None else qt.data_ptr(), 0 if qt is None else qt.stride(0),
-                 None if st is None else st.data_ptr(), 0 if st is None else st.stride(0), threshold, state)
-    return (q, s, qt, st) if transposed else (q, s)
+    return _native.dropout_advance(rng)
 
 
 def fp8_quantize_rows(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn, drop_p: float = 0.0, rng: Tensor | None = None):
@@ -531,62 +461,23 @@ def fp8_quantize_rows(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn, drop_
 
     The scale is the smallest power of two (at least 2^-126) under which the block's largest magnitude is at most 448
     (e4m3) or 57344 (e5m2); q = x / scale rounded to nearest even.  A block with a NaN or an infinity becomes NaN, scale
-    and all.  The row pitch of q is a multiple of 16, as ``fp8_gemm`` wants it.
+    and all.  The row pitches of q and scale are multiples of 16, as ``fp8_gemm`` likes them.
 
     ``drop_p`` / ``rng``: x is dropped out first, with the mask of ``dropout`` but without its factor 1 / (1 - p), which is
     left to the product's ``alpha`` so that what is quantised stays exact."""
-    return _fp8_quantize(x, dtype, 1, False, drop_p, rng)
+    return tuple(_native.fp8_quantize(x, dtype, 1, False, drop_p, rng))
 
 
 def fp8_quantize_both(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn, drop_p: float = 0.0, rng: Tensor | None = None):
     """(q, scale, qt, scale_t) in one pass over x [R, C]: ``fp8_quantize_rows(x)`` and ``fp8_quantize_rows(x.t())``, the
     operands of a product along C and of its gradient product along R.  The mask of ``drop_p`` is numbered in x."""
-    return _fp8_quantize(x, dtype, 1, True, drop_p, rng)
+    return tuple(_native.fp8_quantize(x, dtype, 1, True, drop_p, rng))
 
 
 def fp8_quantize_blocks(w: Tensor, dtype: torch.dtype = torch.float8_e4m3fn, transposed: bool = True):
     """Weights w [R, C] with one scale for each 128 x 128 block: (q [R, C], scale [ceil(R / 128), ceil(C / 128)]) and, with
     ``transposed``, the same numbers as (qt [C, R], scale_t) for the product with the transposed weights."""
-    return _fp8_quantize(w, dtype, 128, transposed, 0.0, None)
-
-
-def _room(t: Tensor, pitch: int, width: int) -> bool:
-    """Whether every row of t can be read up to ``width`` elements."""
-    return t.untyped_storage().nbytes() >= (t.storage_offset() + (t.shape[0] - 1) * pitch + width) * t.element_size()
-
-
-def _repacked(t: Tensor, multiple: int):
-    out = _padded(*t.shape, multiple, t.dtype, t.device)
-    out.view(torch.uint8).copy_(t.view(torch.uint8))
-    return out
-
-
-def _fp8_operand(t: Tensor, scale: Tensor, name: str):
-    """(values, pitch, scales, pitch, rows of a block) as the kernel reads them; copies only what lies otherwise."""
-    _require_cuda((name, t), (name + "_scale", scale))
-    _require(t.dtype in _F8_CODE, f"{name} must be torch.float8_e4m3fn or torch.float8_e5m2")
-    _require(scale.dtype in (torch.float8_e8m0fnu, torch.uint8), f"{name}_scale must be torch.float8_e8m0fnu (or its bytes)")
-    _require(t.dim() == 2 and scale.dim() == 2, f"{name} and {name}_scale must have two dimensions")
-    _require(scale.device == t.device, f"{name} and {name}_scale must be on one device")
-    R, K = t.shape
-    nb = -(-K // 128)
-    _require(scale.shape[1] == nb and scale.shape[0] in (R, -(-R // 128)),
-             f"{name}_scale must have shape [{R} or {-(-R // 128)}, {nb}], got {tuple(scale.shape)}")
-    if R == 0 or K == 0:
-        return t, 0, scale, 0, 1
-    ld = t.stride(0) if R > 1 else -(-K // 16) * 16
-    if (K > 1 and t.stride(1) != 1) or ld % 16 or ld < K or t.data_ptr() % 16:
-        t = _repacked(t, 16)
-        ld = -(-K // 16) * 16
-    rows = scale.shape[0]
-    lds = scale.stride(0) if rows > 1 else -(-nb // 4) * 4
-    # the kernel reads words, or 16 bytes at a time where base and pitch allow it
-    unit = 16 if lds % 16 == 0 and scale.data_ptr() % 16 == 0 else 4
-    width = -(-nb // unit) * unit
-    if (nb > 1 and scale.stride(1) != 1) or lds % 4 or lds < nb or scale.data_ptr() % 4 or not _room(scale, lds, width):
-        scale = _repacked(scale, 16)
-        lds = -(-nb // 16) * 16
-    return t, ld, scale, lds, 1 if rows == R else 128
+    return tuple(_native.fp8_quantize(w, dtype, 128, transposed, 0.0, None))
 
 
 def fp8_gemm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Tensor | None = None, alpha: float = 1.0,
@@ -597,28 +488,7 @@ def fp8_gemm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Tenso
     The sum is held in fp32 (the tensor core applies the scales) and rounded once to ``out_dtype`` (fp32, bf16, fp16).
     e4m3 and e5m2 operands may be mixed.  ``drop_p`` / ``rng``: elements of y that ``dropout`` would drop become zero
     (without its factor): the gradient of a product whose input was dropped out."""
-    _require(out_dtype in _FLOAT_CODE, "out_dtype must be float32, bfloat16 or float16")
-    a, lda, a_scale, ldsa, a_rows = _fp8_operand(a, a_scale, "a")
-    b, ldb, b_scale, ldsb, b_rows = _fp8_operand(b, b_scale, "b")
-    dev = a.device
-    _require(b.device == dev, "a and b must be on one device")
-    (M, K), N = a.shape, b.shape[0]
-    _require(b.shape[1] == K, f"a.size(1) must equal b.size(1), got {K} vs {b.shape[1]}")
-    _require(max(M, N, K) < 2 ** 31, "dimension too large")
-    if bias is not None:
-        _require(isinstance(bias, Tensor) and bias.device == dev and bias.dim() == 1 and bias.shape[0] == N and bias.dtype in _FLOAT_CODE,
-                 f"bias must be a float tensor of {N} elements on the operands' device")
-        bias = bias.detach().to(torch.float32).contiguous()
-    threshold, state = _drop_state(drop_p, rng, dev)
-    y = torch.empty((M, N), dtype=out_dtype, device=dev)
-    if M and N:
-        if K == 0:
-            threshold, state = 0, None
-        _enqueue("atb_fp8_gemm", dev, a.data_ptr(), _F8_CODE[a.dtype], lda, a_scale.data_ptr(), ldsa, a_rows,
-                 b.data_ptr(), _F8_CODE[b.dtype], ldb, b_scale.data_ptr(), ldsb, b_rows,
-                 None if bias is None else bias.data_ptr(), float(alpha), y.data_ptr(), _FLOAT_CODE[out_dtype], N, M, N, K,
-                 threshold, state)
-    return y
+    return _native.fp8_gemm(a, a_scale, b, b_scale, bias, alpha, out_dtype, drop_p, rng)
 
 
 # --------------------------------------------------------------------------- operator implementations

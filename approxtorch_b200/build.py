@@ -1,10 +1,12 @@
-"""In-tree build of ``libapproxtorch_b200.so`` (hand-written CUDA for sm_100a, no torch headers).
+"""In-tree build of ``libapproxtorch_b200.so`` (hand-written CUDA for sm_100a, no torch headers) and of ``_binding.so``, the
+native Python binding of the operators that are called where latency counts (torch headers, host code only).
 
     python -m approxtorch_b200.build [--force] [--verbose]
 
 Each ``csrc/*.cu`` is compiled with ``nvcc -gencode arch=compute_100a,code=sm_100a`` into
 ``csrc/_obj/`` and linked into ``approxtorch_b200/lib/libapproxtorch_b200.so``, which the Python
-binding loads with ctypes.  nvcc cross-compiles, so no GPU is needed to build.
+side loads with ctypes; ``csrc/binding/binding.cpp`` is compiled by the host compiler and linked against that
+library and torch's.  nvcc cross-compiles, so no GPU is needed to build.
 """
 
 from __future__ import annotations
@@ -21,6 +23,8 @@ SRC_DIR = os.path.join(PKG, "csrc")
 OBJ_DIR = os.path.join(SRC_DIR, "_obj")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libapproxtorch_b200.so")
+BINDING_SRC = os.path.join(SRC_DIR, "binding", "binding.cpp")
+BINDING_PATH = os.path.join(LIB_DIR, "_binding.so")
 HEADER = os.path.join(os.path.dirname(PKG), "include", "approxtorch_b200.h")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -62,7 +66,9 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     with open(os.path.join(LIB_DIR, ".build.lock"), "w") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
-            return _build_locked(force, verbose)
+            lib = _build_locked(force, verbose)
+            _build_binding(force, verbose)
+            return lib
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
 
@@ -104,6 +110,31 @@ def _build_locked(force: bool, verbose: bool) -> str:
             raise RuntimeError("link of libapproxtorch_b200.so failed")
         os.replace(tmp, LIB_PATH)
     return LIB_PATH
+
+
+def _build_binding(force: bool, verbose: bool) -> str:
+    if not force and not _stale(BINDING_PATH, [BINDING_SRC, HEADER]):
+        return BINDING_PATH
+    import importlib.util
+    import sysconfig
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    include = os.path.join(torch_dir, "include")
+    cuda_include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
+    cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else shutil.which("g++") or "g++"
+    tmp = f"{BINDING_PATH}.{os.getpid()}.tmp"
+    cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_binding", "-isystem", include,
+           "-isystem", os.path.join(include, "torch", "csrc", "api", "include"), "-isystem", sysconfig.get_paths()["include"],
+           "-isystem", cuda_include, BINDING_SRC, "-o", tmp, "-L" + LIB_DIR, "-lapproxtorch_b200", "-Wl,-rpath,$ORIGIN",
+           "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or proc.returncode != 0:
+        sys.stderr.write(f"--- binding.cpp\n{proc.stdout}{proc.stderr}\n")
+    if proc.returncode != 0:
+        if os.path.exists(tmp):
+            os.remove(tmp)
+        raise RuntimeError("build of _binding.so failed")
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
 
 
 if __name__ == "__main__":

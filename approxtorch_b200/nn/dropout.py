@@ -9,29 +9,14 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd import Function
 
-from ..backend import ops as _ops
-
-
-class _counter_dropout(Function):
-
-    @staticmethod
-    def forward(ctx, x, p, rng):
-        ctx.p = p
-        ctx.save_for_backward(rng)
-        return _ops.dropout(x, p, rng)
-
-    @staticmethod
-    def backward(ctx, grad_output):
-        rng, = ctx.saved_tensors
-        return _ops.dropout(grad_output, ctx.p, rng), None, None
+from ..backend import _C, ops as _ops
 
 
 def counter_dropout(x: torch.Tensor, p: float, rng: torch.Tensor) -> torch.Tensor:
     """x / (1 - p) where kept, 0 elsewhere, with gradient.  ``rng``: int64 {seed, offset} on x's device; it is read again in
     the backward pass, so pass a state that stays as it is (``backend.ops.dropout_advance`` hands one out)."""
-    return _counter_dropout.apply(x, p, rng)
+    return _C.binding.counter_dropout(x, p, rng)
 
 
 def new_state(seed: int | None) -> torch.Tensor:

@@ -80,7 +80,8 @@ _SIGNATURES = {
     "atb_custom_conv_bwd": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp] + [_i] * 13 + [_i, _i, _vp]),
     "atb_lut_dwconv_fwd": (_i, [_vp, _i, _vp, _vp, _vp] + [_i] * 12 + [_i, _vp]),
     "atb_lut_dwconv_bwd": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp] + [_i] * 12 + [_i, _vp]),
-    "atb_fp8_quantize": (_i, [_vp, _i, _ll, _ll, _ll, _i, _i, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _i, _vp, _vp]),
+    "atb_fp8_quantize": (_i, [_vp, _i, _ll, _ll, _ll, _i, _i, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _i, _vp, _vp]),
+    "atb_sum_rows": (_i, [_vp, _i, _ll, _vp, _vp]),
     "atb_fp8_gemm": (_i, [_vp, _i, _ll, _vp, _ll, _i] * 2 + [_vp, ctypes.c_float, _vp, _i, _ll, _i, _i, _i, _i, _vp, _vp]),
     "atb_fp8_status": (_i, [ctypes.POINTER(ctypes.c_int)]),
     "atb_dropout": (_i, [_vp, _vp, _i, _ll, _i, _vp, _vp]),

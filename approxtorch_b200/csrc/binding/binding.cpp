@@ -140,12 +140,12 @@ Tensor quantiser_input(const Tensor& x, const char* name = "x")
     return (C == 1 || x.stride(1) == 1) && (R == 1 || x.stride(0) >= C) ? x : x.contiguous();
 }
 
-void quantise(const Tensor& x, int f8, const Held& h, const Held* t, int threshold, const void* state, void* stream)
+void quantise(const Tensor& x, int f8, const Held& h, const Held* t, float* sums, int threshold, const void* state, void* stream)
 {
     const int64_t R = x.size(0), C = x.size(1);
     if (R == 0 || C == 0) return;
     check_status(atb_fp8_quantize(x.const_data_ptr(), float_code(x.scalar_type()), R, C, R > 1 ? x.stride(0) : C, f8, h.block_rows, h.q, h.ldq,
-                                  h.s, h.lds, t ? t->q : nullptr, t ? t->ldq : 0, t ? t->s : nullptr, t ? t->lds : 0, threshold, state, stream),
+                                  h.s, h.lds, t ? t->q : nullptr, t ? t->ldq : 0, t ? t->s : nullptr, t ? t->lds : 0, sums, threshold, state, stream),
                  "atb_fp8_quantize");
 }
 
@@ -180,7 +180,7 @@ std::vector<Tensor> fp8_quantize(const Tensor& x_in, at::ScalarType dtype, int b
         out.push_back(st);
     }
     const On on(x);
-    quantise(x, f8, h, transposed ? &t : nullptr, threshold, state, on.stream);
+    quantise(x, f8, h, transposed ? &t : nullptr, nullptr, threshold, state, on.stream);
     return out;
 }
 
@@ -304,8 +304,8 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
             if (need_w) at = xt.place(at);
             if (need_x) wt.place(at);
         }
-        quantise(x2, ATB_E4M3, xq, need_w ? &xt : nullptr, threshold, state, on.stream);
-        quantise(w, ATB_E4M3, wq, need_x ? &wt : nullptr, 0, nullptr, on.stream);
+        quantise(x2, ATB_E4M3, xq, need_w ? &xt : nullptr, nullptr, threshold, state, on.stream);
+        quantise(w, ATB_E4M3, wq, need_x ? &wt : nullptr, nullptr, 0, nullptr, on.stream);
         std::vector<int64_t> shape = x.sizes().vec();
         shape.back() = N;
         Tensor y = at::empty(shape, x2.options());
@@ -338,15 +338,25 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
         const double alpha = drop_factor(p);
         const On on(go);
         Held gq(M, N, 1), gt(N, M, 1), xt(K, M, 1), wt(K, N, 128);
+        const int64_t b_type = ctx->saved_data["b_type"].toInt();
+        const bool need_b = b_type >= 0 && ctx->needs_input_grad(2);
+        // the bias gradient comes out of the quantiser's pass over the gradient where that makes both layouts
+        const int64_t sum_rows = (M + 127) / 128, sum_bytes = need_b && need_w && M ? up(sum_rows * N * 4, 256) : 0;
         Tensor scratch, dx, dw, db;
         if (need_x || need_w) {
             uint8_t* at = kept.mutable_data_ptr<uint8_t>();
             if (laid_w) at = xt.place(at);
             if (laid_x) wt.place(at);
-            scratch = at::empty({gq.bytes() + (need_w ? gt.bytes() : 0)}, go.options().dtype(at::kByte));
+            scratch = at::empty({gq.bytes() + (need_w ? gt.bytes() : 0) + sum_bytes}, go.options().dtype(at::kByte));
             at = gq.place(scratch.mutable_data_ptr<uint8_t>());
-            if (need_w) gt.place(at);
-            quantise(go, ATB_E4M3, gq, need_w ? &gt : nullptr, 0, nullptr, on.stream);
+            if (need_w) at = gt.place(at);
+            float* sums = sum_bytes ? reinterpret_cast<float*>(at) : nullptr;
+            if (sums) {
+                db = at::empty({N}, go.options().dtype(at::kFloat));
+                if (sum_rows == 1) sums = db.mutable_data_ptr<float>();      // one tile of rows: nothing to add up
+            }
+            quantise(go, ATB_E4M3, gq, need_w ? &gt : nullptr, sums, 0, nullptr, on.stream);
+            if (sums && sum_rows > 1) check_status(atb_sum_rows(sums, static_cast<int>(sum_rows), N, db.mutable_data_ptr<float>(), on.stream), "atb_sum_rows");
         }
         if (need_x) {
             dx = at::empty(x_shape, go.options());
@@ -356,8 +366,10 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
             dw = at::empty({N, K}, go.options().dtype(static_cast<at::ScalarType>(ctx->saved_data["w_type"].toInt())));
             product(gt, ATB_E4M3, xt, ATB_E4M3, nullptr, alpha, dw, 0, nullptr, on.stream);
         }
-        const int64_t b_type = ctx->saved_data["b_type"].toInt();
-        if (b_type >= 0 && ctx->needs_input_grad(2)) db = go.sum(at::IntArrayRef{0}, false, at::kFloat).to(static_cast<at::ScalarType>(b_type));
+        if (need_b) {
+            if (!db.defined()) db = go.sum(at::IntArrayRef{0}, false, at::kFloat);
+            db = db.to(static_cast<at::ScalarType>(b_type));
+        }
         return {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };

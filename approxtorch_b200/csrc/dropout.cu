@@ -35,11 +35,12 @@ __device__ __forceinline__ Eight<T> eight_load(const T* p)
 }
 
 // One thread takes whole groups of 8 elements (one draw each), kAhead of them at a time, requested together.  VEC: 16-byte
-// aligned tensors.
+// aligned tensors.  2^26 bf16 elements: 45.9 us (a copy: 42.5 us, floor 41.0 us); 2^24 fp32: 22.4 us (a copy: 22.4 us).  Measured
+// against it, 1, 2 or 4 groups ahead and 2, 3 or 4 blocks to an SM: 47 to 74 us.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) dropout_kernel(const T* x, T* y, long long numel, DropState d, float factor)
+__global__ void __launch_bounds__(256, 4) dropout_kernel(const T* x, T* y, long long numel, DropState d, float factor)
 {
-    constexpr int kAhead = sizeof(T) == 2 ? 4 : 2;
+    constexpr int kAhead = sizeof(T) == 2 ? 4 : 1;
     PhiloxKey key(d.rng);
     key.settle();
     const long long whole = VEC ? numel >> 3 : 0, groups = (numel + 7) >> 3;
@@ -89,7 +90,7 @@ template <class T>
 static void launch_dropout(const void* x, void* y, long long numel, const DropState& d, float factor, cudaStream_t s)
 {
     const bool vec = aligned_to(x, 16) && aligned_to(y, 16);
-    const int grid = grid_for((numel + 7) / 8, 256, 16 * sm_count());
+    const int grid = grid_for((numel + 7) / 8, 256, 8 * sm_count());
     if (vec) dropout_kernel<T, true><<<grid, 256, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
     else dropout_kernel<T, false><<<grid, 256, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
 }

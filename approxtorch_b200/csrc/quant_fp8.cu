@@ -30,6 +30,7 @@ struct QuantArgs {
     long long ldqt;
     uint8_t* st;      // [C or ceil(C/128), ldst]
     long long ldst;
+    float* sums;      // [ceil(R/128), C]
     DropState drop;
     bool vec;         // rows of x start on 16-byte boundaries
 };
@@ -159,7 +160,8 @@ __device__ __forceinline__ void drop_draws4(unsigned (&w)[4], unsigned d0, unsig
 enum QuantMode { kRows = 0, kBoth = 1, kSquare = 2 };
 template <class T> constexpr int kQuantThreads = 16 * 128 / Piece<T>::kElems;      // 256, fp32: 512
 
-template <class T, bool E5, bool DROP, int MODE>
+// SUM: the columns' sums over the tile's rows besides (a bias gradient reads the same matrix).
+template <class T, bool E5, bool DROP, int MODE, bool SUM = false>
 __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quantize_kernel(const QuantArgs a)
 {
     using P = Piece<T>;
@@ -167,6 +169,7 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
     constexpr int kWarps = kQuantThreads<T> / 32, kWords = 128 * static_cast<int>(sizeof(T)) / 4;   // words of a row
     __shared__ __align__(16) unsigned s_max[MODE == kRows ? 1 : kWarps][MODE == kRows ? 4 : kWords];
     __shared__ __align__(16) float s_inv[MODE == kBoth ? 128 : 4];
+    __shared__ float s_sum[SUM ? kWarps : 1][SUM ? 128 : 1];
     __shared__ __align__(16) uint8_t s_turn[MODE == kRows ? 16 : 128 * 128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, in_row = lane % kLanes;
     const int strip = threadIdx.x / kLanes;                                        // of 8 rows, 0 .. 15
@@ -258,6 +261,17 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
                 for (int j = 0; j < 4; ++j) col[j] = P::larger(col[j], __shfl_xor_sync(0xFFFFFFFFu, col[j], 16));
             }
             if (lane < kLanes) *reinterpret_cast<uint4*>(&s_max[warp][in_row * 4]) = make_uint4(col[0], col[1], col[2], col[3]);
+            if constexpr (SUM) {
+                auto add = [&](int j, float f) {
+                    if (kLanes == 16) f += __shfl_xor_sync(0xFFFFFFFFu, f, 16);
+                    if (lane < kLanes) s_sum[warp][in_row * kElems + j] = f;
+                };
+#define ATB_COLUMN(J) (((P::template get<J>(v[0]) + P::template get<J>(v[1])) + (P::template get<J>(v[2]) + P::template get<J>(v[3]))) + \
+                       ((P::template get<J>(v[4]) + P::template get<J>(v[5])) + (P::template get<J>(v[6]) + P::template get<J>(v[7]))))
+                add(0, ATB_COLUMN(0)); add(1, ATB_COLUMN(1)); add(2, ATB_COLUMN(2)); add(3, ATB_COLUMN(3));
+                if constexpr (kElems == 8) { add(4, ATB_COLUMN(4)); add(5, ATB_COLUMN(5)); add(6, ATB_COLUMN(6)); add(7, ATB_COLUMN(7)); }
+#undef ATB_COLUMN
+            }
         }
         // 8 rows x kLanes lanes: with every step a lane keeps half of its rows, the upper half if its bit is set
 #pragma unroll
@@ -296,6 +310,13 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
 
     if (MODE == kBoth) {
         __syncthreads();
+        if (SUM && threadIdx.x >= kQuantThreads<T> - 128) {  // (not the warps that make the scales)
+            const int cc = threadIdx.x - (kQuantThreads<T> - 128);
+            float f = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) f += s_sum[w][cc];
+            if (c0 + cc < a.C) a.sums[blockIdx.y * a.C + c0 + cc] = f;
+        }
         if (threadIdx.x < kWords) {                          // a word's columns (one, or two halves)
             unsigned m = s_max[0][threadIdx.x];
 #pragma unroll
@@ -334,6 +355,17 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
     }
 }
 
+// out[c] = the sum of column c of p [rows, C], in the order of the rows
+__global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__ p, int rows, long long C, float* __restrict__ out)
+{
+    const long long c = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= C) return;
+    float f = 0.0f;
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) f += p[r * C + c];
+    out[c] = f;
+}
+
 template <class T, bool E5>
 static int launch_quantize(QuantArgs a, bool square, cudaStream_t s)
 {
@@ -345,7 +377,8 @@ static int launch_quantize(QuantArgs a, bool square, cudaStream_t s)
     const bool drop = a.drop.rng != nullptr;
     if (square) quantize_kernel<T, E5, false, kSquare><<<grid, kQuantThreads<T>, 0, s>>>(a);
     else if (a.qt != nullptr) {
-        if (drop) quantize_kernel<T, E5, true, kBoth><<<grid, kQuantThreads<T>, 0, s>>>(a);
+        if (a.sums) quantize_kernel<T, E5, false, kBoth, true><<<grid, kQuantThreads<T>, 0, s>>>(a);
+        else if (drop) quantize_kernel<T, E5, true, kBoth><<<grid, kQuantThreads<T>, 0, s>>>(a);
         else quantize_kernel<T, E5, false, kBoth><<<grid, kQuantThreads<T>, 0, s>>>(a);
     } else {
         if (drop) quantize_kernel<T, E5, true, kRows><<<grid, kQuantThreads<T>, 0, s>>>(a);
@@ -360,7 +393,7 @@ using namespace atb;
 
 extern "C" int atb_fp8_quantize(const void* x, int x_dtype, long long R, long long C, long long ldx, int f8, int block_rows,
                                 void* q, long long ldq, uint8_t* s, long long lds, void* qt, long long ldqt, uint8_t* st,
-                                long long ldst, int drop_threshold, const void* rng, void* stream)
+                                long long ldst, float* column_sums, int drop_threshold, const void* rng, void* stream)
 {
     ATB_REQUIRE(R >= 0 && C >= 0, "negative dimension");
     ATB_REQUIRE(f8 == ATB_E4M3 || f8 == ATB_E5M2, "the result must be e4m3 or e5m2");
@@ -374,8 +407,10 @@ extern "C" int atb_fp8_quantize(const void* x, int x_dtype, long long R, long lo
     ATB_REQUIRE(ldq >= C && ldq % 16 == 0 && aligned_to(q, 16) && lds >= nb, "q needs 16-byte aligned rows, s a column for every block");
     if (qt) ATB_REQUIRE(ldqt >= R && ldqt % 16 == 0 && aligned_to(qt, 16) && ldst >= nbt, "qt needs 16-byte aligned rows, st a column for every block");
     ATB_REQUIRE(rng == nullptr || block_rows == 1, "dropout goes with blocks of one row");
+    ATB_REQUIRE(column_sums == nullptr || (qt && block_rows == 1 && drop_threshold == 0 && aligned_to(column_sums, 4)),
+                "column sums go with both layouts, blocks of one row and no dropout");
     ATB_REQUIRE(drop_threshold == 0 || (rng != nullptr && aligned_to(rng, 8)), "dropout needs an 8-byte aligned state");
-    QuantArgs a{x, R, C, ldx, static_cast<uint8_t*>(q), ldq, s, lds, static_cast<uint8_t*>(qt), ldqt, st, ldst,
+    QuantArgs a{x, R, C, ldx, static_cast<uint8_t*>(q), ldq, s, lds, static_cast<uint8_t*>(qt), ldqt, st, ldst, column_sums,
                 DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)}, false};
     cudaStream_t stm = static_cast<cudaStream_t>(stream);
     const bool e5 = f8 == ATB_E5M2, square = block_rows == 128;
@@ -383,4 +418,14 @@ extern "C" int atb_fp8_quantize(const void* x, int x_dtype, long long R, long lo
     if (x_dtype == ATB_BF16) return e5 ? launch_quantize<__nv_bfloat16, true>(a, square, stm) : launch_quantize<__nv_bfloat16, false>(a, square, stm);
     if (x_dtype == ATB_F16) return e5 ? launch_quantize<__half, true>(a, square, stm) : launch_quantize<__half, false>(a, square, stm);
     return fail_invalid("x must be fp32, bf16 or fp16");
+}
+
+extern "C" int atb_sum_rows(const float* p, int rows, long long C, float* out, void* stream)
+{
+    ATB_REQUIRE(rows >= 0 && C >= 0, "negative dimension");
+    if (C == 0) return ATB_OK;
+    ATB_REQUIRE(out && (p || rows == 0), "null pointer");
+    ATB_REQUIRE((C + 255) / 256 < (1ll << 31), "too many columns");
+    sum_rows_kernel<<<static_cast<unsigned>((C + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(p, rows, C, out);
+    return check_launch("sum_rows_kernel");
 }

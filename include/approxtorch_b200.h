@@ -302,11 +302,15 @@ int atb_lut_dwconv_bwd(const float* go, const void* x, int dtype, const uint8_t*
  *   q  [R, C], row pitch ldq (a multiple of 16, base 16-byte aligned; the pitch's padding may be written)
  *   s  [R or ceil(R/128), ceil(C/128)], row pitch lds
  *   qt [C, R], st [C or ceil(C/128), ceil(R/128)]: x transposed, quantised in blocks along R; both or neither
+ *   column_sums [ceil(R/128), C] or NULL: the sums of x's columns over each 128 rows, fp32 (with qt, block_rows 1, no
+ *     dropout); atb_sum_rows adds them up
  * drop_threshold > 0: x is dropped out first, as atb_dropout does on the contiguous [R, C] tensor, but without its factor
  * (block_rows 1 only). */
 int atb_fp8_quantize(const void* x, int x_dtype, long long R, long long C, long long ldx, int f8, int block_rows,
                      void* q, long long ldq, uint8_t* s, long long lds, void* qt, long long ldqt, uint8_t* st,
-                     long long ldst, int drop_threshold, const void* rng, void* stream);
+                     long long ldst, float* column_sums, int drop_threshold, const void* rng, void* stream);
+/* out[c] = sum over r of p[r, c], p [rows, C] fp32, in the order of the rows. */
+int atb_sum_rows(const float* p, int rows, long long C, float* out, void* stream);
 /* y[m, n] = alpha * sum_k A[m, k] B[n, k] (scales applied) + bias[n], summed in fp32, rounded once to y_dtype
  * (fp32 / bf16 / fp16); A [M, K], B [N, K].  Row pitches lda, ldb: multiples of 16, bases 16-byte aligned; ldsa, ldsb:
  * multiples of 4, bases 4-byte aligned, and every scale row readable up to a multiple of 4 bytes (of 16, where base and

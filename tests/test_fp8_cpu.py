@@ -63,10 +63,11 @@ def test_c_entries_refuse_bad_arguments():
     """Refused on the host before anything is launched (addresses are never touched)."""
     lib, p = _C.lib, 1 << 20
     q = lambda **k: lib.atb_fp8_quantize(*{**dict(x=p, dt=0, R=4, C=200, ldx=200, f8=5, br=1, q=p, ldq=208, s=p, lds=2, qt=None,   # noqa: E731
-                                                  ldqt=0, st=None, ldst=0, t=0, rng=None, stream=None), **k}.values())
+                                                  ldqt=0, st=None, ldst=0, sums=None, t=0, rng=None, stream=None), **k}.values())
     for bad in (dict(f8=3), dict(br=2), dict(R=-1), dict(ldx=100), dict(ldq=200), dict(q=p + 8), dict(lds=1), dict(x=None), dict(dt=1),
                 dict(qt=p), dict(qt=p, st=p, ldqt=4, ldst=1), dict(qt=p, st=p, ldqt=16, ldst=0), dict(t=5), dict(t=70000, rng=p),
-                dict(t=5, rng=p, br=128), dict(t=5, rng=p + 4)):
+                dict(t=5, rng=p, br=128), dict(t=5, rng=p + 4), dict(sums=p), dict(sums=p, qt=p, st=p, ldqt=16, ldst=1, br=128),
+                dict(sums=p, qt=p, st=p, ldqt=16, ldst=1, t=5, rng=p)):
         assert q(**bad) == 1, bad
         assert _C.last_error()
     g = lambda **k: lib.atb_fp8_gemm(*{**dict(a=p, af=5, lda=208, sa=p, ldsa=4, ar=1, b=p, bf=5, ldb=208, sb=p, ldsb=4, br=128, bias=None,   # noqa: E731
@@ -74,6 +75,7 @@ def test_c_entries_refuse_bad_arguments():
     for bad in (dict(a=None), dict(af=0), dict(bf=4), dict(lda=200), dict(ldb=192), dict(a=p + 1), dict(ldsa=2), dict(ldsa=0), dict(sa=p + 2),
                 dict(ar=64), dict(yd=1), dict(ldy=63), dict(M=-1), dict(y=None), dict(bias=p + 2), dict(t=9), dict(t=65537, rng=p)):
         assert g(**bad) == 1, bad
+    assert lib.atb_sum_rows(p, -1, 4, p, None) == 1 and lib.atb_sum_rows(None, 1, 4, p, None) == 1 and lib.atb_sum_rows(None, 0, 0, None, None) == 0
     assert g(M=0) == 0 and g(N=0, ldy=0) == 0 and q(R=0) == 0
     d = lambda **k: lib.atb_dropout(*{**dict(x=p, y=p, dt=0, n=4, t=9, rng=p, stream=None), **k}.values())   # noqa: E731
     for bad in (dict(x=None), dict(y=None), dict(dt=2), dict(n=-1), dict(t=-1), dict(t=65537), dict(rng=None), dict(rng=p + 4)):

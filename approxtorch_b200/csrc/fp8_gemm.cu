@@ -121,15 +121,13 @@ __device__ __forceinline__ uint32_t f8_leader(uint32_t addr)
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
-// An arrival at a barrier of the pair's first block.  MEMORY: it hands over what this block wrote to its shared memory;
-// without, it only says that tensor memory has been read, which the tcgen05 fences on both sides order.
-template <bool MEMORY>
+// An arrival at a barrier of the pair's first block.  It orders no memory by itself: it says that tensor memory has been
+// read (the tcgen05 fences on both sides order that), or follows an f8_release_cluster.
 __device__ __forceinline__ void f8_arrive_leader(uint32_t local_bar)
 {
-    const uint32_t bar = f8_leader(local_bar);
-    if (!MEMORY) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); return; }
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(f8_leader(local_bar)) : "memory");
 }
+__device__ __forceinline__ void f8_release_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 __device__ __forceinline__ void f8_cluster_sync()
 {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -358,12 +356,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
-    if (warp == 2 || warp == 3) {
+    if (warp == 2 || (CG == 1 && warp == 3)) {
+        // the first scales are what the first MMA waits for: asked for before the blocks meet, and without waiting for
+        // them there (this warp has written nothing that others read)
         sf_settle();
         if (sf_turn < my_turns) fetch(sf_turn, sf_run);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    if (CG == 2) f8_cluster_sync(); else __syncthreads();
+    if (CG == 2) {
+        if (warp == 2) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+        else asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    } else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = s_tmem;
     // Two accumulators side by side, or, where they and the scales do not fit, sharing columns: the epilogue then reads the
@@ -467,27 +471,41 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             }
         }
     } else if (warp < kF8EpiWarp) {
-        // Warps 2 and 3 take every other run.  A warp asks for its next run after the last hand-over of the one before (the
-        // fence of a hand-over would wait for loads in flight).
+        // Warps 2 and 3 take every other run.  A warp asks for its next run after the hand-over of the one before (the fence of
+        // a hand-over would wait for loads in flight).
+        if (CG == 2 && warp == 3) {
+            sf_settle();
+            if (sf_turn < my_turns) fetch(sf_turn, sf_run);
+        }
         uint32_t handed = 0;                                 // quads of this warp so far; it fills four slots of its own in turn
         bool ok = true;
         while (ok && sf_turn < my_turns) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 if (4 * sf_run + q >= quads) break;
-                const uint32_t slot = 4 * (warp - 2) + (handed & 3u), dst = sf0 + slot * kF8SfSlotBytes + lane * 16;
-                if (!(ok = f8_wait(sfe0 + 8 * slot, ((handed >> 2) & 1u) ^ 1u, abort_flag))) break;
-                ++handed;
+                const uint32_t n = handed + q, slot = 4 * (warp - 2) + (n & 3u), dst = sf0 + slot * kF8SfSlotBytes + lane * 16;
+                if (!(ok = f8_wait(sfe0 + 8 * slot, ((n >> 2) & 1u) ^ 1u, abort_flag))) break;
 #pragma unroll
                 for (int j = 0; j < 3; ++j)
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + 512 * j), "r"(f8_word(w[4 * j], q)), "r"(f8_word(w[4 * j + 1], q)),
                                  "r"(f8_word(w[4 * j + 2], q)), "r"(f8_word(w[4 * j + 3], q)) : "memory");
+                if (CG == 1) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) f8_arrive(sff0 + 8 * slot);
+                }
+            }
+            if (!ok) break;
+            const int count = min(4, quads - 4 * sf_run);
+            if (CG == 2) {                                   // one hand-over for the run: a release over the cluster takes about 1500 clocks
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    if (CG == 2) f8_arrive_leader<true>(sff0 + 8 * slot); else f8_arrive(sff0 + 8 * slot);
+                    f8_release_cluster();
+                    for (int q = 0; q < count; ++q) f8_arrive_leader(sff0 + 8 * (4 * (warp - 2) + ((handed + q) & 3u)));
                 }
             }
+            handed += count;
             sf_run += 2;
             sf_settle();
             if (ok && sf_turn < my_turns) fetch(sf_turn, sf_run);
@@ -502,10 +520,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             const int cols = min(32, p.N - n);
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] *= p.alpha;
-            if (p.bias != nullptr) {
-                const int top = p.N - 1 - n;
+            if (p.bias != nullptr) {                         // one load a lane, handed around (32 loads a lane cost 650 clocks)
+                const float b = __ldg(p.bias + min(n + lane, p.N - 1));
 #pragma unroll
-                for (int j = 0; j < 32; ++j) f[j] += __ldg(p.bias + n + min(j, top));
+                for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xFFFFFFFFu, b, j);
             }
             if (p.drop.rng != nullptr) f8_mask32(p.drop, static_cast<unsigned long long>(m0 + lane) * p.N + n, f);
             constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer;           // of a 32-element row
@@ -537,7 +555,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         auto release = [&](uint32_t buf) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) { if (CG == 2) f8_arrive_leader<false>(acce0 + 8 * buf); else f8_arrive(acce0 + 8 * buf); }
+            if (lane == 0) { if (CG == 2) f8_arrive_leader(acce0 + 8 * buf); else f8_arrive(acce0 + 8 * buf); }
         };
         uint32_t item = 0;                                   // accumulators read so far
         bool ok = true;
@@ -584,7 +602,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     if (overlap && i == 0) {
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
-                        if (lane == 0) { if (CG == 2) f8_arrive_leader<false>(accp); else f8_arrive(accp); }
+                        if (lane == 0) { if (CG == 2) f8_arrive_leader(accp); else f8_arrive(accp); }
                     }
                     if (!live) continue;
                     float f[32];

@@ -269,7 +269,7 @@ Tensor fp8_gemm(const Tensor& a, const Tensor& a_scale, const Tensor& b, const T
     const On on(a);                                          // before the operands: a repacking copy runs on this stream
     const Operand l = operand(a, a_scale, "a"), r = operand(b, b_scale, "b");
     TORCH_CHECK(l.at.C == r.at.C, "a.size(1) must equal b.size(1), got ", l.at.C, " vs ", r.at.C);
-    TORCH_CHECK(std::max({l.at.R, r.at.R, l.at.C}) < (int64_t(1) << 31), "dimension too large");
+    TORCH_CHECK(std::max({l.at.R, r.at.R, l.at.C}) <= 0x7FFFF000, "dimension too large");
     const Tensor bias32 = bias_vector(bias, r.at.R, a.device());
     const int threshold = drop_threshold(drop_p);
     const void* state = drop_state(threshold, rng, a.device());
@@ -288,7 +288,7 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
         const Tensor x2 = quantiser_input(x.reshape({-1, x.size(-1)})), w = quantiser_input(weight, "weight");
         TORCH_CHECK(w.device() == x2.device(), "x and weight must be on one device");
         const int64_t M = x2.size(0), N = w.size(0), K = w.size(1);
-        TORCH_CHECK(std::max({M, N, K}) < (int64_t(1) << 31), "dimension too large");
+        TORCH_CHECK(std::max({M, N, K}) <= 0x7FFFF000, "dimension too large");
         const Tensor bias32 = bias_vector(bias, N, x2.device());
         const int threshold = drop_threshold(p);
         const void* state = drop_state(threshold, rng, x2.device());

@@ -28,9 +28,8 @@ template <class T>
 __device__ __forceinline__ Eight<T> eight_load(const T* p)
 {
     Eight<T> e;
-    const uint4* src = reinterpret_cast<const uint4*>(p);
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(e) / 16); ++i) reinterpret_cast<uint4*>(&e)[i] = __ldcs(src + i);
+    for (int i = 0; i < static_cast<int>(sizeof(e) / 16); ++i) reinterpret_cast<uint4*>(&e)[i] = read16_once(p + 16 / sizeof(T) * i);
     return e;
 }
 
@@ -41,6 +40,7 @@ template <class T, bool VEC>
 __global__ void __launch_bounds__(256, 4) dropout_kernel(const T* x, T* y, long long numel, DropState d, float factor)
 {
     constexpr int kAhead = sizeof(T) == 2 ? 4 : 1;
+    after_previous();
     PhiloxKey key(d.rng);
     key.settle();
     const long long whole = VEC ? numel >> 3 : 0, groups = (numel + 7) >> 3;
@@ -78,8 +78,9 @@ __global__ void __launch_bounds__(256, 4) dropout_kernel(const T* x, T* y, long 
 
 // state = {seed, offset}: `taken` gets the state that this call draws from, the offset moves on by one.  On the device,
 // so that every replay of a captured graph draws anew.
-__global__ void drop_advance_kernel(unsigned long long* __restrict__ state, unsigned long long* __restrict__ taken)
+__global__ void drop_advance_kernel(unsigned long long* state, unsigned long long* taken)
 {
+    after_previous();
     const unsigned long long seed = state[0], off = state[1];
     taken[0] = seed;
     taken[1] = off;
@@ -91,8 +92,8 @@ static void launch_dropout(const void* x, void* y, long long numel, const DropSt
 {
     const bool vec = aligned_to(x, 16) && aligned_to(y, 16);
     const int grid = grid_for((numel + 7) / 8, 256, 8 * sm_count());
-    if (vec) dropout_kernel<T, true><<<grid, 256, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
-    else dropout_kernel<T, false><<<grid, 256, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
+    if (vec) launch_after(dropout_kernel<T, true>, dim3(grid), dim3(256), 0, s, 0, static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
+    else launch_after(dropout_kernel<T, false>, dim3(grid), dim3(256), 0, s, 0, static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
 }
 
 }  // namespace atb
@@ -119,7 +120,7 @@ extern "C" int atb_dropout(const void* x, void* y, int dtype, long long numel, i
 extern "C" int atb_dropout_advance(void* state, void* taken, void* stream)
 {
     ATB_REQUIRE(state && taken && aligned_to(state, 8) && aligned_to(taken, 8), "state and taken must be 8-byte aligned device pointers");
-    drop_advance_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<unsigned long long*>(state),
-                                                                       static_cast<unsigned long long*>(taken));
+    launch_after(drop_advance_kernel, dim3(1), dim3(1), 0, static_cast<cudaStream_t>(stream), 0, static_cast<unsigned long long*>(state),
+                 static_cast<unsigned long long*>(taken));
     return check_launch("drop_advance_kernel");
 }

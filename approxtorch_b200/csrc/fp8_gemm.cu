@@ -314,10 +314,10 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const uint8_t* b = p.sb + 16 * run;
         if (p.sf_vec) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = __ldg(reinterpret_cast<const uint4*>(a + static_cast<long long>(min(m0 + 32 * j, p.M - 1) >> p.a_shift) * p.ldsa));
+            for (int j = 0; j < 4; ++j) w[j] = read16(a + static_cast<long long>(min(m0 + 32 * j, p.M - 1) >> p.a_shift) * p.ldsa);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (32 * j < p.tile_n) w[4 + j] = __ldg(reinterpret_cast<const uint4*>(b + static_cast<long long>(min(n0 + 32 * j, p.N - 1) >> p.b_shift) * p.ldsb));
+                if (32 * j < p.tile_n) w[4 + j] = read16(b + static_cast<long long>(min(n0 + 32 * j, p.N - 1) >> p.b_shift) * p.ldsb);
         } else {
             const int words = quads - 4 * run;               // that this run has left
             for (int i = 0; i < 4 && i < words; ++i) {
@@ -325,7 +325,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 for (int j = 0; j < 12; ++j) {
                     const uint8_t* src = j < 4 ? a + static_cast<long long>(min(m0 + 32 * j, p.M - 1) >> p.a_shift) * p.ldsa
                                                : b + static_cast<long long>(min(n0 + 32 * (j - 4), p.N - 1) >> p.b_shift) * p.ldsb;
-                    const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(src) + i);
+                    const uint32_t v = read4(src + 4 * i);
                     if (i == 0) w[j].x = v; else if (i == 1) w[j].y = v; else if (i == 2) w[j].z = v; else w[j].w = v;
                 }
             }
@@ -359,6 +359,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     if (warp == 2 || (CG == 1 && warp == 3)) {
         // the first scales are what the first MMA waits for: asked for before the blocks meet, and without waiting for
         // them there (this warp has written nothing that others read)
+        after_previous();
         sf_settle();
         if (sf_turn < my_turns) fetch(sf_turn, sf_run);
     }
@@ -369,6 +370,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     } else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    after_previous();
     const uint32_t tmem = s_tmem;
     // Two accumulators side by side, or, where they and the scales do not fit, sharing columns: the epilogue then reads the
     // shared ones first and says so, and the next tile's MMAs start.
@@ -521,7 +523,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] *= p.alpha;
             if (p.bias != nullptr) {                         // one load a lane, handed around (32 loads a lane cost 650 clocks)
-                const float b = __ldg(p.bias + min(n + lane, p.N - 1));
+                const float b = __uint_as_float(read4(p.bias + min(n + lane, p.N - 1)));
 #pragma unroll
                 for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xFFFFFFFFu, b, j);
             }
@@ -697,6 +699,7 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    after_previous();
     const uint32_t tmem = s_tmem;
     const int q0 = kb0 >> 2, quads = ((kb1 + 3) >> 2) - q0;      // of this block, by place in a scale row
 
@@ -756,7 +759,7 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
             for (int j = 0; j < 8; ++j) {
                 const uint8_t* src = j < 4 ? p.sb + static_cast<long long>(min(n0 + lane + 32 * j, p.N - 1) >> p.b_shift) * p.ldsb
                                            : p.sa + static_cast<long long>(min(m0 + lane + 32 * (j - 4), p.M - 1) >> p.a_shift) * p.ldsa;
-                w[j] = j < 4 || 32 * (j - 4) < p.tile_c ? __ldg(reinterpret_cast<const uint32_t*>(src) + q0 + q) : 0x7F7F7F7Fu;
+                w[j] = j < 4 || 32 * (j - 4) < p.tile_c ? read4(src + 4 * (q0 + q)) : 0x7F7F7F7Fu;
             }
             const uint32_t dst = sf0 + q * 1024 + lane * 16;
 #pragma unroll
@@ -782,7 +785,7 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
         if (f8_wait(acc0, 0, abort_flag)) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int row = (warp & 3) * 32 + lane, n = n0 + row;
-            const float bias = p.splits == 1 && p.bias != nullptr && n < p.N ? __ldg(p.bias + n) : 0.0f;
+            const float bias = p.splits == 1 && p.bias != nullptr && n < p.N ? __uint_as_float(read4(p.bias + n)) : 0.0f;
             for (int c = 0; c < cols; c += 16) {
                 uint32_t v[16];
                 f8_tmem_ld16(v, tmem + c + (static_cast<uint32_t>((warp & 3) * 32) << 16));
@@ -809,7 +812,7 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
     // ---- every block finishes its share of the columns, four at a time so that the reads overlap
     const int row = tid & (kF8TileM - 1), n = n0 + row;
     if (n < p.N) {
-        const float bias = p.bias != nullptr ? __ldg(p.bias + n) : 0.0f;
+        const float bias = p.bias != nullptr ? __uint_as_float(read4(p.bias + n)) : 0.0f;
         const int step = 2 * p.splits;
         for (int c = static_cast<int>(rank) + p.splits * (tid >> 7); c < cols; c += 4 * step) {
             float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -827,8 +830,9 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
 
 // y = bias (a product over nothing)
 template <class T>
-__global__ void fp8_bias_kernel(T* __restrict__ y, long long ldy, const float* __restrict__ bias, int M, int N)
+__global__ void fp8_bias_kernel(T* y, long long ldy, const float* bias, int M, int N)
 {
+    after_previous();
     const long long total = static_cast<long long>(M) * N, stride = static_cast<long long>(gridDim.x) * blockDim.x;
     for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
         const long long m = i / N, n = i - m * N;
@@ -932,18 +936,9 @@ static int launch_fp8(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Par
     static bool done[64];
     cudaError_t e = allow_smem(fp8_gemm_kernel<T, CG, SUMS>, done);
     const int tiles = p.mt * p.nt, fit = sm_count() / CG;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(CG * (tiles < fit ? tiles : fit));
-    cfg.blockDim = dim3(SUMS ? kF8SumThreads : kF8Threads);
-    cfg.dynamicSmemBytes = kF8Smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = CG;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = CG == 2 ? 1 : 0;
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, fp8_gemm_kernel<T, CG, SUMS>, ma, mb, p);
+    if (e == cudaSuccess)
+        e = launch_after(fp8_gemm_kernel<T, CG, SUMS>, dim3(CG * (tiles < fit ? tiles : fit)), dim3(SUMS ? kF8SumThreads : kF8Threads), kF8Smem, s,
+                         CG == 2 ? 2 : 0, ma, mb, p);
     if (e != cudaSuccess) { set_error("fp8_gemm_kernel: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
     return check_launch("fp8_gemm_kernel");
 }
@@ -959,18 +954,7 @@ static int launch_split(const CUtensorMap& mb, const CUtensorMap& ma, const Fp8S
 {
     static bool done[64];
     cudaError_t e = allow_smem(fp8_split_kernel<T>, done);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(tiles * p.splits);
-    cfg.blockDim = dim3(kF8Threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = p.splits;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, fp8_split_kernel<T>, mb, ma, p);
+    if (e == cudaSuccess) e = launch_after(fp8_split_kernel<T>, dim3(tiles * p.splits), dim3(kF8Threads), smem, s, p.splits, mb, ma, p);
     if (e != cudaSuccess) { set_error("fp8_split_kernel: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
     return check_launch("fp8_split_kernel");
 }
@@ -978,7 +962,7 @@ static int launch_split(const CUtensorMap& mb, const CUtensorMap& ma, const Fp8S
 template <class T>
 static int launch_bias(void* y, long long ldy, const float* bias, int M, int N, cudaStream_t s)
 {
-    fp8_bias_kernel<T><<<grid_for(static_cast<long long>(M) * N, 256, 16 * sm_count()), 256, 0, s>>>(static_cast<T*>(y), ldy, bias, M, N);
+    launch_after(fp8_bias_kernel<T>, dim3(grid_for(static_cast<long long>(M) * N, 256, 16 * sm_count())), dim3(256), 0, s, 0, static_cast<T*>(y), ldy, bias, M, N);
     return check_launch("fp8_bias_kernel");
 }
 
@@ -992,6 +976,7 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
                             int drop_threshold, const void* rng, void* stream)
 {
     ATB_REQUIRE(M >= 0 && N >= 0 && K >= 0, "negative dimension");
+    ATB_REQUIRE(M <= 0x7FFFF000 && N <= 0x7FFFF000 && K <= 0x7FFFF000, "dimension too large");   // tile coordinates are 32-bit
     ATB_REQUIRE((a_f8 == ATB_E4M3 || a_f8 == ATB_E5M2) && (b_f8 == ATB_E4M3 || b_f8 == ATB_E5M2), "operands must be e4m3 or e5m2");
     ATB_REQUIRE((a_block_rows == 1 || a_block_rows == 128) && (b_block_rows == 1 || b_block_rows == 128), "block rows must be 1 or 128");
     ATB_REQUIRE(y_dtype == ATB_F32 || y_dtype == ATB_BF16 || y_dtype == ATB_F16, "y must be fp32, bf16 or fp16");

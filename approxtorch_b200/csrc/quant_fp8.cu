@@ -33,6 +33,7 @@ struct QuantArgs {
     float* sums;      // [ceil(R/128), C]
     DropState drop;
     bool vec;         // rows of x start on 16-byte boundaries
+    unsigned ct;      // tiles of 128 columns
 };
 
 // What a lane holds of a row: 16 bytes in the input's own type (8 bf16 or fp16, 4 fp32).  Magnitudes are compared in that
@@ -81,7 +82,7 @@ template <> struct Piece<__half> {
 
 // elements c ... of a row (beyond the row's end: zeros)
 template <class T>
-__device__ __forceinline__ void load_piece(const T* __restrict__ row, long long c, long long C, unsigned (&w)[4])
+__device__ __forceinline__ void load_piece(const T* row, long long c, long long C, unsigned (&w)[4])
 {
     constexpr int kElems = Piece<T>::kElems;
 #pragma unroll
@@ -173,17 +174,19 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
     __shared__ __align__(16) uint8_t s_turn[MODE == kRows ? 16 : 128 * 128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, in_row = lane % kLanes;
     const int strip = threadIdx.x / kLanes;                                        // of 8 rows, 0 .. 15
-    const long long r0 = static_cast<long long>(blockIdx.y) * 128 + strip * 8, c0 = static_cast<long long>(blockIdx.x) * 128;
+    const unsigned tile_r = blockIdx.x / a.ct, tile_c = blockIdx.x - tile_r * a.ct;
+    const long long r0 = static_cast<long long>(tile_r) * 128 + strip * 8, c0 = static_cast<long long>(tile_c) * 128;
     const long long c = c0 + in_row * kElems;
     const int rows = static_cast<int>(max(0ll, min(8ll, a.R - r0)));
     if (MODE == kRows && a.R <= r0 - (strip * 8) % (32 / kLanes * 8)) return;      // nothing for this warp
     const T* const x = static_cast<const T*>(a.x) + r0 * a.ldx + c;
+    after_previous();
 
     unsigned v[8][4];
     if (a.vec && rows == 8 && c0 + 128 <= a.C) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint4 q = __ldcs(reinterpret_cast<const uint4*>(x + i * a.ldx));
+            const uint4 q = read16_once(x + i * a.ldx);
             v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
         }
     } else {
@@ -251,8 +254,8 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
 #pragma unroll
         for (int i = 1; i < 8; ++i) inv[i] = inv[0];
         if (threadIdx.x == 0) {
-            a.s[blockIdx.y * a.lds + blockIdx.x] = static_cast<uint8_t>(byte);
-            if (a.st) a.st[blockIdx.x * a.ldst + blockIdx.y] = static_cast<uint8_t>(byte);
+            a.s[tile_r * a.lds + tile_c] = static_cast<uint8_t>(byte);
+            if (a.st) a.st[tile_c * a.ldst + tile_r] = static_cast<uint8_t>(byte);
         }
     } else {
         if (MODE == kBoth) {
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
         const int row = in_row / (kLanes / 8);               // the one this lane is left with
         const unsigned byte = scale_byte<E5>(P::fp32_bits(top[0]));
         const float mine = inverse_scale(byte);
-        if (in_row % (kLanes / 8) == 0 && row < rows) a.s[(r0 + row) * a.lds + blockIdx.x] = static_cast<uint8_t>(byte);
+        if (in_row % (kLanes / 8) == 0 && row < rows) a.s[(r0 + row) * a.lds + tile_c] = static_cast<uint8_t>(byte);
 #pragma unroll
         for (int i = 0; i < 8; ++i) inv[i] = __shfl_sync(0xFFFFFFFFu, mine, i * (kLanes / 8), kLanes);
     }
@@ -315,7 +318,7 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
             float f = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) f += s_sum[w][cc];
-            if (c0 + cc < a.C) a.sums[blockIdx.y * a.C + c0 + cc] = f;
+            if (c0 + cc < a.C) a.sums[tile_r * a.C + c0 + cc] = f;
         }
         if (threadIdx.x < kWords) {                          // a word's columns (one, or two halves)
             unsigned m = s_max[0][threadIdx.x];
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
                 const unsigned one = kPer == 1 ? m : h ? m >> 16 : m & 0xFFFFu;
                 const unsigned byte = scale_byte<E5>(P::fp32_bits(one));
                 s_inv[cc] = inverse_scale(byte);
-                if (c0 + cc < a.C) a.st[(c0 + cc) * a.ldst + blockIdx.y] = static_cast<uint8_t>(byte);
+                if (c0 + cc < a.C) a.st[(c0 + cc) * a.ldst + tile_r] = static_cast<uint8_t>(byte);
             }
         }
         __syncthreads();
@@ -345,7 +348,7 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
     if constexpr (kElems == 8) { ATB_TURN(4); ATB_TURN(5); ATB_TURN(6); ATB_TURN(7); }
 #undef ATB_TURN
     __syncthreads();
-    const long long rt = static_cast<long long>(blockIdx.y) * 128;
+    const long long rt = static_cast<long long>(tile_r) * 128;
 #pragma unroll
     for (int i = 0; i < 1024 / kQuantThreads<T>; ++i) {
         const int cc = (threadIdx.x >> 3) + kQuantThreads<T> / 8 * i, piece = threadIdx.x & 7, by = cc / kElems % 16;
@@ -356,8 +359,9 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
 }
 
 // out[c] = the sum of column c of p [rows, C], in the order of the rows
-__global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__ p, int rows, long long C, float* __restrict__ out)
+__global__ void __launch_bounds__(256) sum_rows_kernel(const float* p, int rows, long long C, float* out)
 {
+    after_previous();
     const long long c = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
     if (c >= C) return;
     float f = 0.0f;
@@ -369,20 +373,20 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const float* __restrict__
 template <class T, bool E5>
 static int launch_quantize(QuantArgs a, bool square, cudaStream_t s)
 {
-    const long long nbt = (a.R + 127) >> 7;
-    ATB_REQUIRE(nbt <= 65535, "too many rows");
-    ATB_REQUIRE((a.C + 127) >> 7 < (1ll << 31), "too many columns");
-    const dim3 grid(static_cast<unsigned>((a.C + 127) >> 7), static_cast<unsigned>(nbt));
+    const long long ct = (a.C + 127) >> 7, tiles = ((a.R + 127) >> 7) * ct;
+    ATB_REQUIRE(tiles < (1ll << 31), "matrix too large");
+    const dim3 grid(static_cast<unsigned>(tiles));
+    a.ct = static_cast<unsigned>(ct);
     a.vec = aligned_to(a.x, 16) && (a.ldx * static_cast<long long>(sizeof(T))) % 16 == 0;
     const bool drop = a.drop.rng != nullptr;
-    if (square) quantize_kernel<T, E5, false, kSquare><<<grid, kQuantThreads<T>, 0, s>>>(a);
+    if (square) launch_after(quantize_kernel<T, E5, false, kSquare>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
     else if (a.qt != nullptr) {
-        if (a.sums) quantize_kernel<T, E5, false, kBoth, true><<<grid, kQuantThreads<T>, 0, s>>>(a);
-        else if (drop) quantize_kernel<T, E5, true, kBoth><<<grid, kQuantThreads<T>, 0, s>>>(a);
-        else quantize_kernel<T, E5, false, kBoth><<<grid, kQuantThreads<T>, 0, s>>>(a);
+        if (a.sums) launch_after(quantize_kernel<T, E5, false, kBoth, true>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
+        else if (drop) launch_after(quantize_kernel<T, E5, true, kBoth>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
+        else launch_after(quantize_kernel<T, E5, false, kBoth>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
     } else {
-        if (drop) quantize_kernel<T, E5, true, kRows><<<grid, kQuantThreads<T>, 0, s>>>(a);
-        else quantize_kernel<T, E5, false, kRows><<<grid, kQuantThreads<T>, 0, s>>>(a);
+        if (drop) launch_after(quantize_kernel<T, E5, true, kRows>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
+        else launch_after(quantize_kernel<T, E5, false, kRows>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
     }
     return check_launch("quantize_kernel");
 }
@@ -411,7 +415,7 @@ extern "C" int atb_fp8_quantize(const void* x, int x_dtype, long long R, long lo
                 "column sums go with both layouts, blocks of one row and no dropout");
     ATB_REQUIRE(drop_threshold == 0 || (rng != nullptr && aligned_to(rng, 8)), "dropout needs an 8-byte aligned state");
     QuantArgs a{x, R, C, ldx, static_cast<uint8_t*>(q), ldq, s, lds, static_cast<uint8_t*>(qt), ldqt, st, ldst, column_sums,
-                DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)}, false};
+                DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)}, false, 0};
     cudaStream_t stm = static_cast<cudaStream_t>(stream);
     const bool e5 = f8 == ATB_E5M2, square = block_rows == 128;
     if (x_dtype == ATB_F32) return e5 ? launch_quantize<float, true>(a, square, stm) : launch_quantize<float, false>(a, square, stm);
@@ -426,6 +430,6 @@ extern "C" int atb_sum_rows(const float* p, int rows, long long C, float* out, v
     if (C == 0) return ATB_OK;
     ATB_REQUIRE(out && (p || rows == 0), "null pointer");
     ATB_REQUIRE((C + 255) / 256 < (1ll << 31), "too many columns");
-    sum_rows_kernel<<<static_cast<unsigned>((C + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(p, rows, C, out);
+    launch_after(sum_rows_kernel, dim3(static_cast<unsigned>((C + 255) / 256)), dim3(256), 0, static_cast<cudaStream_t>(stream), 0, p, rows, C, out);
     return check_launch("sum_rows_kernel");
 }

@@ -320,13 +320,21 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (32 * j < p.tile_n) w[4 + j] = read16(b + static_cast<long long>(min(n0 + 32 * j, p.N - 1) >> p.b_shift) * p.ldsb);
         } else {
             const int words = quads - 4 * run;               // that this run has left
-            for (int i = 0; i < 4 && i < words; ++i) {
+            const uint8_t* src[12];
+#pragma unroll
+            for (int j = 0; j < 12; ++j) {
+                src[j] = j < 4 ? a + static_cast<long long>(min(m0 + 32 * j, p.M - 1) >> p.a_shift) * p.ldsa
+                               : b + static_cast<long long>(min(n0 + 32 * (j - 4), p.N - 1) >> p.b_shift) * p.ldsb;
+                if (j < 4 || 32 * (j - 4) < p.tile_n) w[j].x = read4(src[j]);
+            }
+#pragma unroll
+            for (int i = 1; i < 4; ++i) {
+                if (i >= words) break;
 #pragma unroll
                 for (int j = 0; j < 12; ++j) {
-                    const uint8_t* src = j < 4 ? a + static_cast<long long>(min(m0 + 32 * j, p.M - 1) >> p.a_shift) * p.ldsa
-                                               : b + static_cast<long long>(min(n0 + 32 * (j - 4), p.N - 1) >> p.b_shift) * p.ldsb;
-                    const uint32_t v = read4(src + 4 * i);
-                    if (i == 0) w[j].x = v; else if (i == 1) w[j].y = v; else if (i == 2) w[j].z = v; else w[j].w = v;
+                    if (j >= 4 && 32 * (j - 4) >= p.tile_n) continue;
+                    const uint32_t v = read4(src[j] + 4 * i);
+                    if (i == 1) w[j].y = v; else if (i == 2) w[j].z = v; else w[j].w = v;
                 }
             }
         }
@@ -517,15 +525,16 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const uint32_t stage = stage0 + (warp - kF8EpiWarp) * 32 * kPitch;
         const uint32_t lanes = static_cast<uint32_t>(row0) << 16;
         T* const y = static_cast<T*>(p.y);
-        // 32 x 32 results: f holds this lane's row, columns n ...
-        auto emit = [&](float (&f)[32], int m0, int n, int rows) {
+        // the bias of column n + lane
+        auto bias_of = [&](int n) { return p.bias != nullptr ? __uint_as_float(read4(p.bias + min(n + lane, p.N - 1))) : 0.0f; };
+        // 32 x 32 results: f holds this lane's row, columns n ..., bias is bias_of(n), asked for ahead
+        auto emit = [&](float (&f)[32], int m0, int n, int rows, float bias) {
             const int cols = min(32, p.N - n);
 #pragma unroll
             for (int j = 0; j < 32; ++j) f[j] *= p.alpha;
             if (p.bias != nullptr) {                         // one load a lane, handed around (32 loads a lane cost 650 clocks)
-                const float b = __uint_as_float(read4(p.bias + min(n + lane, p.N - 1)));
 #pragma unroll
-                for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xFFFFFFFFu, b, j);
+                for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xFFFFFFFFu, bias, j);
             }
             if (p.drop.rng != nullptr) f8_mask32(p.drop, static_cast<unsigned long long>(m0 + lane) * p.N + n, f);
             constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer;           // of a 32-element row
@@ -588,16 +597,20 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 for (int i = 0; i < kF8SumTileN / 64; ++i) {
                     if (32 * i >= half) break;
                     const int n = n0 + c0 + 32 * i;
-                    if (n < p.N && rows > 0) emit(sums[i], m0, n, rows);
+                    if (n < p.N && rows > 0) emit(sums[i], m0, n, rows, bias_of(n));
                 }
             } else {
                 const int chunks = p.tile_n / 32;
                 const uint32_t buf = item & 1u;
+                auto column = [&](int i) { return 32 * (overlap && buf == 0 ? (i == 0 ? chunks - 1 : i - 1) : i); };
+                float bias_next = bias_of(n0 + column(0));
                 if (!(ok = f8_wait(accf0 + 8 * buf, (item >> 1) & 1u, abort_flag))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + buf * d_step + lanes;
                 for (int i = 0; i < chunks; ++i) {
-                    const int c = 32 * (overlap && buf == 0 ? (i == 0 ? chunks - 1 : i - 1) : i), n = n0 + c;
+                    const int c = column(i), n = n0 + c;
+                    const float bias = bias_next;
+                    if (i + 1 < chunks) bias_next = bias_of(n0 + column(i + 1));
                     const bool live = n < p.N && rows > 0;   // the same for the whole warp
                     uint32_t v[32];
                     if (live) f8_tmem_ld32(v, src + c);
@@ -610,7 +623,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     float f[32];
 #pragma unroll
                     for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-                    emit(f, m0, n, rows);
+                    emit(f, m0, n, rows, bias);
                 }
                 release(buf);
                 ++item;

@@ -113,11 +113,11 @@ def _build_locked(force: bool, verbose: bool) -> str:
 
 
 def _build_binding(force: bool, verbose: bool) -> str:
-    if not force and not _stale(BINDING_PATH, [BINDING_SRC, HEADER]):
-        return BINDING_PATH
     import importlib.util
     import sysconfig
     torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    if not force and not _stale(BINDING_PATH, [BINDING_SRC, HEADER, os.path.join(torch_dir, "version.py")]):
+        return BINDING_PATH
     include = os.path.join(torch_dir, "include")
     cuda_include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
     cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else shutil.which("g++") or "g++"

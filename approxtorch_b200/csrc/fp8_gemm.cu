@@ -18,9 +18,14 @@
 //               i + 32 j (warp 3 also owns the tensor-memory allocation);
 //   warps 4-7   read finished accumulators, scale, add the bias and store, 32 x 32 elements at a time through shared
 //               memory so that a row's bytes leave together.
-// Two accumulators let the epilogue of a tile run under the MMAs of the next.  Why pairs: each block of a pair holds its
-// own 128 rows of A and half the rows of B and the tensor core reads both halves, so a slice of a 256 x 224 tile costs
-// each SM 30 KB instead of the 44 KB of a 128 x 224 tile, and what bounds the product is the path from L2 to the SMs.
+// Two accumulators let the epilogue of a tile run under the MMAs of the next; where two of 256 columns and the scales do
+// not fit the 512 columns of tensor memory, they share 24 columns, which the epilogue reads first.  Why pairs: each block of
+// a pair holds its own 128 rows of A and half the rows of B and the tensor core reads both halves, so a slice of a 256 x 256
+// tile costs each SM 32 KB from L2 instead of the 48 KB of a 128 x 256 tile.  What bounds it: 8192^3 in 376 us (2.92 PFLOP/s, a
+// library product of the same operands with a scale for each 32: 404 us), 510 clocks for a slice of a 256 x 256 tile that
+// the tensor core needs 512 for at its nominal rate; kept up for long, the power limit (445 us).  What it took to get there, and
+// what a change should not lose: the issuing warp runs converged and walks uniform values (a branch on the lane number cost
+// 40 %), the scales arrive a quad ahead, and only hand-overs of memory between the blocks pay for cluster scope.
 //
 // fp8_split_kernel, for products of few tiles (serving, small heads): see there.
 //
@@ -81,10 +86,11 @@ __device__ __forceinline__ void f8_expect(uint32_t bar, uint32_t bytes)
 // Bounded wait that also gives up when another role of the block has.  CLUSTER: the arrivals it waits for order another
 // block's writes (an acquire over the cluster costs far more than one over the block; only the hand-overs that need it
 // pay for it).
+constexpr int kF8Patience = 1 << 18;                      // looks at a barrier: about a second
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag)
+__device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int patience = kF8Patience)
 {
-    for (int i = 0; i < (1 << 18); ++i) {        // about a second
+    for (int i = 0; i < patience; ++i) {
         uint32_t ok;
         if (CLUSTER)
             asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -568,6 +574,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             __syncwarp();
             if (lane == 0) { if (CG == 2) f8_arrive_leader(acce0 + 8 * buf); else f8_arrive(acce0 + 8 * buf); }
         };
+        // an accumulator may take long where the reduction is: a second for every 65536 slices, which take 26 ms
+        const int patience = kF8Patience * (1 + (kb_n >> 16));
         uint32_t item = 0;                                   // accumulators read so far
         bool ok = true;
         for (int t = first; t < ntiles && ok; t += step) {
@@ -580,7 +588,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 float sums[kF8SumTileN / 64][32];
                 for (int q = 0; q < quads; q += kF8SumQuads, ++item) {
                     const uint32_t buf = item & 1u;
-                    if (!(ok = f8_wait(accf0 + 8 * buf, (item >> 1) & 1u, abort_flag))) break;
+                    if (!(ok = f8_wait(accf0 + 8 * buf, (item >> 1) & 1u, abort_flag, patience))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
                     for (int i = 0; i < kF8SumTileN / 64; ++i) {
@@ -604,7 +612,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 const uint32_t buf = item & 1u;
                 auto column = [&](int i) { return 32 * (overlap && buf == 0 ? (i == 0 ? chunks - 1 : i - 1) : i); };
                 float bias_next = bias_of(n0 + column(0));
-                if (!(ok = f8_wait(accf0 + 8 * buf, (item >> 1) & 1u, abort_flag))) break;
+                if (!(ok = f8_wait(accf0 + 8 * buf, (item >> 1) & 1u, abort_flag, patience))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + buf * d_step + lanes;
                 for (int i = 0; i < chunks; ++i) {

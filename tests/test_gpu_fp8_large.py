@@ -106,6 +106,32 @@ def test_operands_beyond_32_bit_offsets(dev):
         _check(y[part], (a[part], sa[part]), (b, sb), alpha=2.0 ** -10)
 
 
+def test_result_beyond_32_bit_offsets(dev):
+    """A result of 4.6e9 elements: rows past 2^32 elements."""
+    from approxtorch_b200.backend import ops
+    M, N, K = 70000, 65600, 130
+    a, b = _operands(dev, M, N, K, 1)
+    bias = torch.randn(N, device=dev)
+    y = ops.fp8_gemm(*a, *b, bias=bias)
+    for part in (slice(0, 100), slice(65500, 65600), slice(M - 100, M)):
+        _check(y[part], (a[0][part], a[1][part]), b, bias)
+
+
+def test_one_sum_of_seconds(dev):
+    """2^30 steps into one element take seconds; no wait of the kernel may run out over them.  960 ones among zeros, their
+    sum exact in bf16."""
+    from approxtorch_b200.backend import _C, ops
+    K = (1 << 30) - 5
+    a = torch.zeros((1, K + 5), dtype=torch.uint8, device=dev)
+    a[0, torch.randperm(K // 997, device=dev)[:959] * 997] = 0x38
+    a[0, K - 1] = 0x38
+    a = a.view(E4)[:, :K]
+    s = torch.full((1, -(-K // 128)), 127, dtype=torch.uint8, device=dev)
+    assert ops.fp8_gemm(a, s, a, s).item() == 960.0
+    status = ctypes.c_int(-1)
+    assert _C.lib.atb_fp8_status(ctypes.byref(status)) == 0 and status.value == 0
+
+
 def test_quantiser_beyond_32_bit_offsets(dev):
     from approxtorch_b200.backend import ops
     R, C = 36000, 65544                                    # 2.36e9 elements of bf16, rows past 2^31 elements

@@ -32,7 +32,6 @@ struct QuantArgs {
     long long ldst;
     float* sums;      // [ceil(R/128), C]
     DropState drop;
-    bool vec;         // rows of x start on 16-byte boundaries
     unsigned ct;      // tiles of 128 columns
 };
 
@@ -80,18 +79,36 @@ template <> struct Piece<__half> {
     }
 };
 
-// elements c ... of a row (beyond the row's end: zeros)
-template <class T>
-__device__ __forceinline__ void load_piece(const T* row, long long c, long long C, unsigned (&w)[4])
+// the 16 bytes from byte `by` (even, 0 .. 14) of lo, hi on
+__device__ __forceinline__ void shifted(const uint4& lo, const uint4& hi, unsigned by, unsigned (&out)[4])
 {
-    constexpr int kElems = Piece<T>::kElems;
+    unsigned w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int i = 0; i < 7; ++i) w[i] = by & 4u ? w[i + 1] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = by & 8u ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = __funnelshift_r(w[i], w[i + 1], 8u * (by & 3u));
+}
+__device__ __forceinline__ uint4 from_next_lane(const uint4& v)
+{
+    return make_uint4(__shfl_down_sync(0xFFFFFFFFu, v.x, 1), __shfl_down_sync(0xFFFFFFFFu, v.y, 1), __shfl_down_sync(0xFFFFFFFFu, v.z, 1),
+                      __shfl_down_sync(0xFFFFFFFFu, v.w, 1));
+}
+
+// `left` elements from p on (zeros beyond), wherever p lies; WHOLE: there are enough.  Element by element: 16-byte loads of the
+// aligned words around them, shifted into place, took 52.6 us where these take 39.0 (8191 x 4095 bf16, both layouts; fp32 of
+// 4095 x 4095: 35 and 23 us).
+template <class T, bool WHOLE>
+__device__ __forceinline__ void load_piece(const T* p, long long left, unsigned (&w)[4])
+{
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = 0;
 #pragma unroll
-    for (int i = 0; i < kElems; ++i) {
-        if (c + i >= C) continue;
-        if constexpr (kElems == 4) w[i] = __float_as_uint(row[c + i]);
-        else w[i / 2] |= static_cast<unsigned>(reinterpret_cast<const unsigned short*>(row)[c + i]) << (16 * (i & 1));
+    for (int i = 0; i < Piece<T>::kElems; ++i) {
+        if (!WHOLE && i >= left) continue;
+        if constexpr (Piece<T>::kElems == 4) w[i] = __float_as_uint(p[i]);
+        else w[i / 2] |= static_cast<unsigned>(reinterpret_cast<const unsigned short*>(p)[i]) << (16 * (i & 1));
     }
 }
 
@@ -118,18 +135,7 @@ __device__ __forceinline__ unsigned pack4(float a, float b, float c, float d)
     return lo | (hi << 16);
 }
 
-// clears what is dropped: bit j of keep stands for element j of the piece
-template <class T>
-__device__ __forceinline__ void drop_bits(unsigned (&w)[4], unsigned keep)
-{
-#pragma unroll
-    for (int j = 0; j < Piece<T>::kElems; ++j) {
-        if ((keep >> j) & 1u) continue;
-        if (Piece<T>::kElems == 4) w[j] = 0;
-        else w[j / 2] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-    }
-}
-// the same from the draws: word i of d holds the 16 bits of elements 2 i and 2 i + 1 of a group of 8
+// clears what is dropped: word i of d holds the 16 bits of elements 2 i and 2 i + 1 of a group of 8
 __device__ __forceinline__ void drop_draws8(unsigned (&w)[4], const uint4& d, unsigned high)      // high = threshold << 16
 {
     const unsigned v[4] = {d.x, d.y, d.z, d.w};
@@ -158,11 +164,16 @@ __device__ __forceinline__ void drop_draws4(unsigned (&w)[4], unsigned d0, unsig
 // are what bounds this kernel besides memory, and a scale made by every lane for every row was a third of them.
 // The transposed image turns through shared memory so that it leaves in 128-byte rows: column c is row c of s_turn, its
 // 8-byte pieces (8 rows of one lane) permuted by the column so that the lanes of a write spread over all banks.
+//
+// Measured, bf16 8192 x 8192: kRows 32.5 us (floor 30.7), kBoth 51.4 us (41.0), with dropout 50 and 64 us (the draws take 22 us of
+// the multiply pipe); fp32 4096 x 4096 kSquare, both layouts, 19.0 us (15.4).  Rows that start anywhere (8191 x 4095): kRows
+// 27.8 us (15.4), kBoth 39 us (20.5).
 enum QuantMode { kRows = 0, kBoth = 1, kSquare = 2 };
 template <class T> constexpr int kQuantThreads = 16 * 128 / Piece<T>::kElems;      // 256, fp32: 512
 
-// SUM: the columns' sums over the tile's rows besides (a bias gradient reads the same matrix).
-template <class T, bool E5, bool DROP, int MODE, bool SUM = false>
+// SUM: the columns' sums over the tile's rows besides (a bias gradient reads the same matrix).  ALIGNED: rows start on
+// 16-byte boundaries and have a multiple of 8 elements, so that a lane's 16 bytes are one load and one draw.
+template <class T, bool E5, bool ALIGNED, bool DROP, int MODE, bool SUM = false>
 __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quantize_kernel(const QuantArgs a)
 {
     using P = Piece<T>;
@@ -183,16 +194,25 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
     after_previous();
 
     unsigned v[8][4];
-    if (a.vec && rows == 8 && c0 + 128 <= a.C) {
+    const bool whole = rows == 8 && c0 + 128 <= a.C;         // the same for the block's warps but in the last tiles
+    if (ALIGNED && whole) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const uint4 q = read16_once(x + i * a.ldx);
             v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
         }
-    } else {
-        const T* const base = static_cast<const T*>(a.x) + (rows ? r0 : 0) * a.ldx;
+    } else if (ALIGNED) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) load_piece(base + (i < rows ? i : 0) * a.ldx, i < rows ? c : a.C, a.C, v[i]);
+        for (int i = 0; i < 8; ++i) {
+            const uint4 q = i < rows && c < a.C ? read16_once(x + i * a.ldx) : make_uint4(0, 0, 0, 0);
+            v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
+        }
+    } else if (whole) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) load_piece<T, true>(x + i * a.ldx, kElems, v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) load_piece<T, false>(x + i * a.ldx, i < rows ? a.C - c : 0, v[i]);
     }
     if (DROP) {
         PhiloxKey key(a.drop.rng);
@@ -203,7 +223,7 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
             for (int i = 0; i < 8; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[i][j] = 0;
-        } else if ((a.C & 7) == 0) {
+        } else if (ALIGNED) {
             const unsigned long long g = static_cast<unsigned long long>(r0 * a.C + c) >> 3, row = static_cast<unsigned long long>(a.C) >> 3;
             if (kElems == 8) {
 #pragma unroll
@@ -220,11 +240,24 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quan
                 }
             }
         } else {
-#pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-                const unsigned keep = philox_keep8_at(key, static_cast<unsigned long long>((r0 + i) * a.C + c), a.drop.threshold);
+            // Pieces straddle groups of 8 draws: a lane draws the group of its first element and takes the next group from the
+            // next lane.  What the last lanes of the 8 (16) rows are short of, a lane each draws for one row, in one call.
+            const int extra_row = lane % 8, extra_strip = strip - lane / kLanes + lane / 8 % (32 / kLanes);
+            const unsigned long long e_extra = static_cast<unsigned long long>((static_cast<long long>(tile_r) * 128 + extra_strip * 8 + extra_row) * a.C + c0 + 128 - kElems);
+            const uint4 extra = philox4x32_10(key, (e_extra >> 3) + 1);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) if (k == i) drop_bits<T>(v[k], keep);
+            for (int i = 0; i < 8; ++i) {
+                const unsigned long long e = static_cast<unsigned long long>((r0 + i) * a.C + c);
+                const uint4 own = philox4x32_10(key, e >> 3);
+                uint4 next = from_next_lane(own);
+                const int from = lane / kLanes * 8 + i;      // of the lane that drew for this row
+                const uint4 x = make_uint4(__shfl_sync(0xFFFFFFFFu, extra.x, from), __shfl_sync(0xFFFFFFFFu, extra.y, from),
+                                           __shfl_sync(0xFFFFFFFFu, extra.z, from), __shfl_sync(0xFFFFFFFFu, extra.w, from));
+                if (in_row == kLanes - 1) next = x;
+                unsigned d[4];
+                shifted(own, next, 2u * static_cast<unsigned>(e & 7u), d);
+                if (kElems == 8) drop_draws8(v[i], make_uint4(d[0], d[1], d[2], d[3]), high);
+                else drop_draws4(v[i], d[0], d[1], high);
             }
         }
     }
@@ -370,25 +403,30 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const float* p, int rows,
     out[c] = f;
 }
 
+template <class T, bool E5, bool ALIGNED>
+static int launch_quantize_as(const QuantArgs& a, bool square, unsigned tiles, cudaStream_t s)
+{
+    const dim3 grid(tiles), block(kQuantThreads<T>);
+    const bool drop = a.drop.rng != nullptr;
+    if (square) launch_after(quantize_kernel<T, E5, ALIGNED, false, kSquare>, grid, block, 0, s, 0, a);
+    else if (a.qt == nullptr) {
+        if (drop) launch_after(quantize_kernel<T, E5, ALIGNED, true, kRows>, grid, block, 0, s, 0, a);
+        else launch_after(quantize_kernel<T, E5, ALIGNED, false, kRows>, grid, block, 0, s, 0, a);
+    } else if (a.sums) launch_after(quantize_kernel<T, E5, ALIGNED, false, kBoth, true>, grid, block, 0, s, 0, a);
+    else if (drop) launch_after(quantize_kernel<T, E5, ALIGNED, true, kBoth>, grid, block, 0, s, 0, a);
+    else launch_after(quantize_kernel<T, E5, ALIGNED, false, kBoth>, grid, block, 0, s, 0, a);
+    return check_launch("quantize_kernel");
+}
+
 template <class T, bool E5>
 static int launch_quantize(QuantArgs a, bool square, cudaStream_t s)
 {
     const long long ct = (a.C + 127) >> 7, tiles = ((a.R + 127) >> 7) * ct;
     ATB_REQUIRE(tiles < (1ll << 31), "matrix too large");
-    const dim3 grid(static_cast<unsigned>(tiles));
     a.ct = static_cast<unsigned>(ct);
-    a.vec = aligned_to(a.x, 16) && (a.ldx * static_cast<long long>(sizeof(T))) % 16 == 0;
-    const bool drop = a.drop.rng != nullptr;
-    if (square) launch_after(quantize_kernel<T, E5, false, kSquare>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
-    else if (a.qt != nullptr) {
-        if (a.sums) launch_after(quantize_kernel<T, E5, false, kBoth, true>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
-        else if (drop) launch_after(quantize_kernel<T, E5, true, kBoth>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
-        else launch_after(quantize_kernel<T, E5, false, kBoth>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
-    } else {
-        if (drop) launch_after(quantize_kernel<T, E5, true, kRows>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
-        else launch_after(quantize_kernel<T, E5, false, kRows>, grid, dim3(kQuantThreads<T>), 0, s, 0, a);
-    }
-    return check_launch("quantize_kernel");
+    const bool aligned = aligned_to(a.x, 16) && (a.ldx * static_cast<long long>(sizeof(T))) % 16 == 0 && a.C % 8 == 0;
+    return aligned ? launch_quantize_as<T, E5, true>(a, square, static_cast<unsigned>(tiles), s)
+                   : launch_quantize_as<T, E5, false>(a, square, static_cast<unsigned>(tiles), s);
 }
 
 }  // namespace atb
@@ -415,7 +453,7 @@ extern "C" int atb_fp8_quantize(const void* x, int x_dtype, long long R, long lo
                 "column sums go with both layouts, blocks of one row and no dropout");
     ATB_REQUIRE(drop_threshold == 0 || (rng != nullptr && aligned_to(rng, 8)), "dropout needs an 8-byte aligned state");
     QuantArgs a{x, R, C, ldx, static_cast<uint8_t*>(q), ldq, s, lds, static_cast<uint8_t*>(qt), ldqt, st, ldst, column_sums,
-                DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)}, false, 0};
+                DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)}, 0};
     cudaStream_t stm = static_cast<cudaStream_t>(stream);
     const bool e5 = f8 == ATB_E5M2, square = block_rows == 128;
     if (x_dtype == ATB_F32) return e5 ? launch_quantize<float, true>(a, square, stm) : launch_quantize<float, false>(a, square, stm);

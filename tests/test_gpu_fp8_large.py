@@ -106,6 +106,26 @@ def test_operands_beyond_32_bit_offsets(dev):
         _check(y[part], (a[part], sa[part]), (b, sb), alpha=2.0 ** -10)
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,C,pitch,off", [(130, 257, 257, 0), (300, 1001, 1001, 0), (129, 136, 136, 0), (129, 136, 137, 3), (17, 264, 300, 8), (257, 129, 136, 8),
+                                           (128, 127, 128, 1), (3, 5, 5, 0)])
+def test_quantiser_draws_wherever_rows_start(dev, R, C, pitch, off, dt):
+    """Dropout inside the quantiser for rows on and off 16-byte boundaries: both layouts against the oracle, bit for bit."""
+    from approxtorch_b200.backend import ops
+    g = torch.Generator(dev).manual_seed(R + C)
+    x = torch.randn(off + R * pitch + 8, generator=g, device=dev).to(dt)[off:off + R * pitch].view(R, pitch)[:, :C]
+    state = torch.tensor([-5, 1 << 50], dtype=torch.int64, device=dev)
+    keep = fo.keep_mask((R, C), 0.4, -5, 1 << 50)
+    x64 = np.where(keep, x.double().cpu().numpy(), 0.0)
+    out = ops.fp8_quantize_both(x, drop_p=0.4, rng=state)
+    rows = ops.fp8_quantize_rows(x, drop_p=0.4, rng=state)
+    assert all(torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8)) for a, b in zip(rows, out))
+    for q, s, ref in ((*out[:2], x64), (*out[2:], x64.T)):
+        rq, rs = fo.quantise(ref)
+        np.testing.assert_array_equal(q.contiguous().float().double().cpu().numpy(), rq)
+        np.testing.assert_array_equal(np.exp2(s.contiguous().view(torch.uint8).cpu().numpy().astype(np.float64) - 127), rs)
+
+
 def test_result_beyond_32_bit_offsets(dev):
     """A result of 4.6e9 elements: rows past 2^32 elements."""
     from approxtorch_b200.backend import ops

@@ -259,18 +259,19 @@ __device__ __forceinline__ T f8_get(uint32_t addr)
 }
 // zeros where 32 consecutive elements are dropped.  Out of line: rare, and long enough to push the loop out of the
 // instruction cache.
-__device__ __noinline__ unsigned f8_keep8(const unsigned long long* rng, unsigned threshold, unsigned long long element)
+__device__ __noinline__ unsigned f8_keep8(const unsigned long long* rng, unsigned threshold, unsigned long long group)
 {
-    return philox_keep8_at(PhiloxKey(rng), element, threshold);
+    return philox_keep8(PhiloxKey(rng), group, threshold);
 }
 __device__ __forceinline__ void f8_mask32(const DropState& d, unsigned long long element, float (&f)[32])
 {
+    const unsigned shift = static_cast<unsigned>(element & 7u);
+    unsigned long long keep = 0;                             // of the four or five groups that the elements lie in
+    for (int g = 0; g < (shift ? 5 : 4); ++g)
+        keep |= static_cast<unsigned long long>(f8_keep8(d.rng, d.threshold, (element >> 3) + g)) << (8 * g);
+    const unsigned m = static_cast<unsigned>(keep >> shift);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const unsigned keep = f8_keep8(d.rng, d.threshold, element + 8 * g);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[8 * g + j] = (keep >> j) & 1u ? f[8 * g + j] : 0.0f;
-    }
+    for (int j = 0; j < 32; ++j) f[j] = (m >> j) & 1u ? f[j] : 0.0f;
 }
 
 __device__ __forceinline__ uint32_t f8_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
@@ -798,7 +799,7 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
         float f = p.alpha * v + bias;
         if (p.drop.rng != nullptr) {
             const unsigned long long e = static_cast<unsigned long long>(m0 + c) * p.N + n;
-            if (!((f8_keep8(p.drop.rng, p.drop.threshold, e & ~7ull) >> (e & 7u)) & 1u)) f = 0.0f;
+            if (!((f8_keep8(p.drop.rng, p.drop.threshold, e >> 3) >> (e & 7u)) & 1u)) f = 0.0f;
         }
         y[c * p.ldy + n] = f8_out<T>(f);
     };

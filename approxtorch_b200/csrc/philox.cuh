@@ -71,14 +71,4 @@ __device__ __forceinline__ unsigned philox_keep8(const PhiloxKey& key, unsigned 
     return m;
 }
 
-// the same for 8 elements that start anywhere: two groups where they straddle a boundary
-__device__ __forceinline__ unsigned philox_keep8_at(const PhiloxKey& key, unsigned long long element, unsigned threshold)
-{
-    const unsigned shift = static_cast<unsigned>(element & 7u);
-    const unsigned long long g = element >> 3;
-    unsigned m = philox_keep8(key, g, threshold);
-    if (shift != 0) m = (m | (philox_keep8(key, g + 1, threshold) << 8)) >> shift;
-    return m & 0xFFu;
-}
-
 }  // namespace atb

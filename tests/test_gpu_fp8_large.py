@@ -39,7 +39,9 @@ def _check(y, a, b, bias=None, alpha=1.0, keep=None):
     if keep is not None:
         ref = torch.where(keep, ref, 0.0)
     tol = (K * 2.0 ** -23 + 2 * 2.0 ** -24) * mag
-    tol = tol + half * (ref.abs() + tol)
+    # half a step of the result: eps / 2 of the value, and below the smallest normal number, where the steps stay as they are
+    # (fp16: 2^-24 apart below 2^-14), eps / 2 of that number (2^-11 2^-14 = 2^-25, half of 2^-24)
+    tol = tol + half * (ref.abs() + tol) + half * torch.finfo(y.dtype).smallest_normal
     worst = ((y.double() - ref).abs() / tol.clamp(min=1e-300)).max().item()
     assert worst <= 1.0, worst
 

@@ -3,6 +3,7 @@
 // are called where latency counts: checking and calling one from Python took 17 to 26 us, several times what the kernels
 // take for one token or a small head, and a layer's forward and backward 300 us.
 #include <ATen/cuda/CUDAContextLight.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -44,6 +45,12 @@ struct On {
     }
 };
 
+// an uninitialised contiguous tensor on the device of `like` (without the dispatcher: half the time of at::empty)
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like)
+{
+    return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt));
+}
+
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // ---- dropout -------------------------------------------------------------------------------------------------------
@@ -75,7 +82,7 @@ Tensor dropout(const Tensor& x, double p, const std::optional<Tensor>& rng)
     const void* state = drop_state(threshold, rng, x.device());
     const Tensor xc = x.contiguous();
     if (threshold == 0) return xc.clone();
-    Tensor y = at::empty(xc.sizes(), xc.options());
+    Tensor y = fresh(xc.sizes(), xc.scalar_type(), xc);
     if (y.numel()) {
         const On on(x);
         check_status(atb_dropout(xc.const_data_ptr(), y.mutable_data_ptr(), code, xc.numel(), threshold, state, on.stream), "atb_dropout");
@@ -87,7 +94,7 @@ Tensor dropout_advance(const Tensor& rng)
 {
     TORCH_CHECK(rng.is_cuda(), "rng must be a CUDA tensor");
     TORCH_CHECK(rng.scalar_type() == at::kLong && rng.numel() == 2 && rng.is_contiguous(), "rng must be a contiguous int64 tensor {seed, offset}");
-    Tensor taken = at::empty({2}, rng.options());
+    Tensor taken = fresh({2}, at::kLong, rng);
     const On on(rng);
     check_status(atb_dropout_advance(rng.mutable_data_ptr(), taken.mutable_data_ptr(), on.stream), "atb_dropout_advance");
     return taken;
@@ -152,9 +159,9 @@ void quantise(const Tensor& x, int f8, const Held& h, const Held* t, float* sums
 // [rows, cols] of a 1-byte type with a pitch of whole 16 bytes
 Tensor padded(int64_t rows, int64_t cols, at::ScalarType dtype, const Tensor& like)
 {
-    const auto options = like.options().dtype(dtype);
-    if (cols % 16 == 0) return at::empty({rows, cols}, options);
-    return at::empty({rows, up(cols, 16)}, options).narrow(1, 0, cols);
+    Tensor t = fresh({rows, up(cols, 16)}, dtype, like);
+    if (cols % 16) t.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef({rows, cols}), at::IntArrayRef({up(cols, 16), 1}));
+    return t;
 }
 
 std::vector<Tensor> fp8_quantize(const Tensor& x_in, at::ScalarType dtype, int block_rows, bool transposed, double drop_p,
@@ -273,7 +280,7 @@ Tensor fp8_gemm(const Tensor& a, const Tensor& a_scale, const Tensor& b, const T
     const Tensor bias32 = bias_vector(bias, r.at.R, a.device());
     const int threshold = drop_threshold(drop_p);
     const void* state = drop_state(threshold, rng, a.device());
-    Tensor y = at::empty({l.at.R, r.at.R}, a.options().dtype(out_dtype));
+    Tensor y = fresh({l.at.R, r.at.R}, out_dtype, a);
     product(l.at, l.f8, r.at, r.f8, bias_pointer(bias32), alpha, y, threshold, state, on.stream);
     return y;
 }
@@ -295,11 +302,10 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
         const On on(x2);
         // operands in one allocation, what the backward pass reads in another
         Held xq(M, K, 1), wq(N, K, 128), xt(K, M, 1), wt(K, N, 128);
-        const auto bytes = x2.options().dtype(at::kByte);
-        Tensor scratch = at::empty({xq.bytes() + wq.bytes()}, bytes), kept;
+        Tensor scratch = fresh({xq.bytes() + wq.bytes()}, at::kByte, x2), kept;
         wq.place(xq.place(scratch.mutable_data_ptr<uint8_t>()));
         if (need_x || need_w) {
-            kept = at::empty({(need_w ? xt.bytes() : 0) + (need_x ? wt.bytes() : 0)}, bytes);
+            kept = fresh({(need_w ? xt.bytes() : 0) + (need_x ? wt.bytes() : 0)}, at::kByte, x2);
             uint8_t* at = kept.mutable_data_ptr<uint8_t>();
             if (need_w) at = xt.place(at);
             if (need_x) wt.place(at);
@@ -308,7 +314,7 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
         quantise(w, ATB_E4M3, wq, need_x ? &wt : nullptr, nullptr, 0, nullptr, on.stream);
         std::vector<int64_t> shape = x.sizes().vec();
         shape.back() = N;
-        Tensor y = at::empty(shape, x2.options());
+        Tensor y = fresh(shape, x2.scalar_type(), x2);
         product(xq, ATB_E4M3, wq, ATB_E4M3, bias_pointer(bias32), drop_factor(p), y, 0, nullptr, on.stream);
         if (need_x || need_w || (bias.has_value() && bias->defined())) {
             ctx->save_for_backward({kept, threshold ? *rng : Tensor()});
@@ -347,23 +353,23 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
             uint8_t* at = kept.mutable_data_ptr<uint8_t>();
             if (laid_w) at = xt.place(at);
             if (laid_x) wt.place(at);
-            scratch = at::empty({gq.bytes() + (need_w ? gt.bytes() : 0) + sum_bytes}, go.options().dtype(at::kByte));
+            scratch = fresh({gq.bytes() + (need_w ? gt.bytes() : 0) + sum_bytes}, at::kByte, go);
             at = gq.place(scratch.mutable_data_ptr<uint8_t>());
             if (need_w) at = gt.place(at);
             float* sums = sum_bytes ? reinterpret_cast<float*>(at) : nullptr;
             if (sums) {
-                db = at::empty({N}, go.options().dtype(at::kFloat));
+                db = fresh({N}, at::kFloat, go);
                 if (sum_rows == 1) sums = db.mutable_data_ptr<float>();      // one tile of rows: nothing to add up
             }
             quantise(go, ATB_E4M3, gq, need_w ? &gt : nullptr, sums, 0, nullptr, on.stream);
             if (sums && sum_rows > 1) check_status(atb_sum_rows(sums, static_cast<int>(sum_rows), N, db.mutable_data_ptr<float>(), on.stream), "atb_sum_rows");
         }
         if (need_x) {
-            dx = at::empty(x_shape, go.options());
+            dx = fresh(x_shape, go.scalar_type(), go);
             product(gq, ATB_E4M3, wt, ATB_E4M3, nullptr, alpha, dx, threshold, rng.defined() ? rng.const_data_ptr() : nullptr, on.stream);
         }
         if (need_w) {
-            dw = at::empty({N, K}, go.options().dtype(static_cast<at::ScalarType>(ctx->saved_data["w_type"].toInt())));
+            dw = fresh({N, K}, static_cast<at::ScalarType>(ctx->saved_data["w_type"].toInt()), go);
             product(gt, ATB_E4M3, xt, ATB_E4M3, nullptr, alpha, dw, 0, nullptr, on.stream);
         }
         if (need_b) {

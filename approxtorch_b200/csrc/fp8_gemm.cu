@@ -30,7 +30,7 @@
 // fp8_split_kernel, for products of few tiles (serving, small heads): see there.
 //
 // Operand rows beyond M or N and steps beyond K are zeros that TMA fills in; scale bytes beyond the last block are
-// never selected, and rows beyond the last get 1.
+// never selected, and rows beyond the last take its scales: a row's products go to its own row of the result alone.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -29,7 +29,8 @@ def new_state(seed: int | None) -> torch.Tensor:
 class CounterDropout(nn.Module):
     """Dropout layer on ``counter_dropout``.  Its state {seed, offset} is a buffer: it moves on by one on the device with
     every training forward (also in replays of a captured graph), is saved in checkpoints, and decides the masks, so a
-    resumed run draws what the interrupted one would have drawn.  Give every rank its own seed."""
+    resumed run draws what the interrupted one would have drawn.  Give every rank its own seed, and wrap the model with
+    ``broadcast_buffers=False`` (DistributedDataParallel otherwise hands rank 0's state to all)."""
 
     def __init__(self, p: float = 0.5, seed: int | None = None):
         super().__init__()

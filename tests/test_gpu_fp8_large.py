@@ -343,6 +343,18 @@ def test_linear_fp8_takes_what_autograd_hands_it(dev):
             bad()
 
 
+def test_linear_fp8_with_everything_dropped(dev):
+    """p = 1: the product is over nothing, whatever x holds; the gradients of x and W are zero."""
+    import approxtorch_b200 as at
+    state = torch.tensor([1, 1], dtype=torch.int64, device=dev)
+    x = torch.full((150, 200), float("inf"), device=dev, requires_grad=True)
+    w, b = torch.randn(70, 200, device=dev, requires_grad=True), torch.randn(70, device=dev, requires_grad=True)
+    y = at.nn.gemm_fp8.linear_fp8(x, w, b, drop_p=1.0, rng=state)
+    assert torch.equal(y, b.expand(150, 70))
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    assert (gx == 0).all() and (gw == 0).all() and (gb == 150).all()
+
+
 def test_dropout_differentiates_twice(dev):
     import approxtorch_b200 as at
     state = torch.tensor([8, 8], dtype=torch.int64, device=dev)

@@ -655,7 +655,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 // instead of 32.  B supplies the MMA's 128 rows whatever M is, so no tensor-core row is wasted on a missing token; each
 // block requests its whole share of B at once (up to kF8MaxStages slices).  The S partial tiles meet in shared memory: every
 // block adds up its share of the columns over the cluster in the order of the blocks (bit for bit repeatable) and stores
-// it.  No workspace, no counters, one launch.
+// it.  No workspace, no counters, one launch.  Measured back to back, bf16 results, against the best tile of
+// fp8_gemm_kernel: 1 x 4096 x 4096 5.4 us (12.3; the weights' 17 MB pass at 3.1 TB/s), 64 x 4096 x 4096 7.8 us (11.5),
+// 256 x 1000 x 2048 6.1 us (7.3).
 struct Fp8SplitParams {
     const uint8_t* sa;
     const uint8_t* sb;
@@ -895,11 +897,55 @@ static int operand_map(CUtensorMap* map, const void* base, long long R, long lon
     return ATB_OK;
 }
 
+// the kernels' shared memory is above the default limit: allowed once per device
+template <class K>
+static cudaError_t allow_smem(K kernel, bool (&done)[64])
+{
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev])) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    return e;
+}
+
+// blocks of clusters of `size` that the device runs at a time, one to an SM (148 SMs hold 132 blocks of clusters of 4)
+static int fp8_cluster_blocks(int size)
+{
+    static int known[64][9];
+    static bool done[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sm_count() / size * size;
+    if (known[dev][size] == 0) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(size);
+        cfg.blockDim = dim3(kF8Threads);
+        cfg.dynamicSmemBytes = kF8Smem;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = size;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (allow_smem(fp8_split_kernel<float>, done) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, fp8_split_kernel<float>, &cfg) != cudaSuccess || n <= 0) {
+            cudaGetLastError();                              // an estimate does; the launch reports what is wrong
+            n = sm_count() / size;
+        }
+        known[dev][size] = n * size;
+    }
+    return known[dev][size];
+}
+
 // How a product is cut: the kernel, tile and number of blocks to a tile with the least estimated time.  Microseconds as
 // measured on B200 (8-bit operands of random numbers): a slice (128 steps) of a tile costs 0.06 + 0.0013 per column to a
 // pair of blocks (the MMAs; 0.22 at least, the issue), 0.165 + 0.00106 per column to a single block; a tile besides, 0.4 +
-// 0.003 per column; a launch with a first load, 3.9 (pairs: 5.0).  The split kernel: 0.14 + 0.0016 per row of A for a slice,
-// 0.8 + 0.025 per row of A and 0.06 per block of the cluster for a tile, 3.2 for the launch.
+// 0.003 per column; a launch with a first load, 3.5 (pairs: 4.6).  The split kernel: 0.14 + 0.0016 per row of A for a slice,
+// 0.8 + 0.025 per row of A and 0.06 per block of the cluster for a tile, 2.0 for the launch, 2.3 with clusters (blocks that
+// share an SM take nearly as long as one after the other, so they count as further rounds).  Over 200 products drawn at
+// random (rows 1 to 4000, columns and reduction 64 to 8192, bf16 and fp32 results) the choice took 1.02 of the time of the
+// best choice on average and 1.24 at worst.
 struct Fp8Plan {
     int cg, tile;            // fp8_gemm_kernel: blocks to a tile, columns
     int splits;              // fp8_split_kernel where not 0: blocks to a tile; tile = rows of A
@@ -920,7 +966,7 @@ static Fp8Plan fp8_plan(int M, int N, int kblocks, bool fp32)
             if (tile > unit && tile - unit >= N) break;
             const double nt = (N + tile - 1) / tile, waves = ceil(mt * nt / (sms / cg));
             const double slice = cg == 2 ? fmax(0.22, 0.06 + 0.0013 * tile) : 0.165 + 0.00106 * tile;
-            const double t = waves * (kblocks * slice + 0.4 + 0.003 * tile) + (cg == 2 ? 5.0 : 3.9);
+            const double t = waves * (kblocks * slice + 0.4 + 0.003 * tile) + (cg == 2 ? 4.6 : 3.5);
             if (t < least) { least = t; best = Fp8Plan{cg, tile, 0}; }
         }
     }
@@ -930,26 +976,14 @@ static Fp8Plan fp8_plan(int M, int N, int kblocks, bool fp32)
         const double mt = (M + tile - 1) / tile;
         if (mt * nt > 16.0 * sms) continue;                  // many tiles: never the better kernel
         for (int splits = 1; splits <= 8 && splits <= kblocks; ++splits) {
-            const int kbs = (kblocks + splits - 1) / splits;
-            if (kbs / 4 + 2 > kF8MaxQuads || (fp32 && kbs > kF8SumsFrom)) continue;
-            const double waves = ceil(mt * nt * splits / sms);
-            const double t = waves * (kbs * (0.14 + 0.0016 * tile) + 0.8 + 0.025 * tile + 0.06 * splits) + 3.2;
+            const int slices = (kblocks + splits - 1) / splits;
+            if (slices / 4 + 2 > kF8MaxQuads || (fp32 && slices > kF8SumsFrom)) continue;
+            const double waves = ceil(mt * nt * splits / fp8_cluster_blocks(splits));
+            const double t = waves * (slices * (0.14 + 0.0016 * tile) + 0.8 + 0.025 * tile + 0.06 * splits) + (splits > 1 ? 2.3 : 2.0);
             if (t < least) { least = t; best = Fp8Plan{1, tile, splits}; }
         }
     }
     return best;
-}
-
-// the kernels' shared memory is above the default limit: allowed once per device
-template <class K>
-static cudaError_t allow_smem(K kernel, bool (&done)[64])
-{
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev])) return e;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
-    if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
-    return e;
 }
 
 template <class T, int CG, bool SUMS>

@@ -17,7 +17,11 @@ from .gemm_fp8 import linear_fp8
 
 class Linear_fp8(nn.Module):
     """y = dropout(x) W^T + b.  ``dropout`` is applied in training only, its state {seed, offset} is the buffer ``rng`` (see
-    ``CounterDropout``); ``state_dict`` keys of ``weight`` and ``bias`` are those of ``nn.Linear``."""
+    ``CounterDropout``, also for forwards that are run twice); ``state_dict`` keys of ``weight`` and ``bias`` are those of
+    ``nn.Linear``.
+
+    A training step can be captured into a CUDA graph.  As with torch's own layers, let go of every result that was computed
+    from the same parameters outside the capture first: their gradient nodes belong to the stream of that computation."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, dropout: float = 0.0, seed: int | None = None):
         super().__init__()
@@ -50,11 +54,12 @@ class Linear_fp8(nn.Module):
         self._frozen = None
         return super()._load_from_state_dict(*args, **kwargs)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, rng: torch.Tensor | None = None) -> torch.Tensor:
         if x.dim() == 0 or x.shape[-1] != self.in_features:
             raise RuntimeError(f"expected last dimension {self.in_features}, got {tuple(x.shape)}")
         p = self.dropout if self.training else 0.0
-        rng = _ops.dropout_advance(self.rng) if p > 0.0 else None
+        if p > 0.0 and rng is None:
+            rng = _ops.dropout_advance(self.rng)
         wants_grad = torch.is_grad_enabled() and (
             x.requires_grad or self.weight.requires_grad or (self.bias is not None and self.bias.requires_grad))
         if self._frozen is not None and not wants_grad:

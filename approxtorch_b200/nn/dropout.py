@@ -30,7 +30,11 @@ class CounterDropout(nn.Module):
     """Dropout layer on ``counter_dropout``.  Its state {seed, offset} is a buffer: it moves on by one on the device with
     every training forward (also in replays of a captured graph), is saved in checkpoints, and decides the masks, so a
     resumed run draws what the interrupted one would have drawn.  Give every rank its own seed, and wrap the model with
-    ``broadcast_buffers=False`` (DistributedDataParallel otherwise hands rank 0's state to all)."""
+    ``broadcast_buffers=False`` (DistributedDataParallel otherwise hands rank 0's state to all).
+
+    A forward that is run again for the backward pass (``torch.utils.checkpoint``) has to draw what it drew the first time:
+    take the state before, ``rng = backend.ops.dropout_advance(layer.rng)``, and hand it to ``layer(x, rng)``.  Without it
+    the second run draws anew, and the gradient is that of another mask."""
 
     def __init__(self, p: float = 0.5, seed: int | None = None):
         super().__init__()
@@ -39,10 +43,10 @@ class CounterDropout(nn.Module):
         self.p = p
         self.register_buffer('rng', new_state(seed))
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, rng: torch.Tensor | None = None) -> torch.Tensor:
         if not self.training or self.p == 0.0:
             return x
-        return counter_dropout(x, self.p, _ops.dropout_advance(self.rng))
+        return counter_dropout(x, self.p, _ops.dropout_advance(self.rng) if rng is None else rng)
 
     def extra_repr(self) -> str:
         return f"p={self.p}"

@@ -355,6 +355,32 @@ def test_linear_fp8_with_everything_dropped(dev):
     assert (gx == 0).all() and (gw == 0).all() and (gb == 150).all()
 
 
+def test_layers_recomputed_with_a_given_state(dev):
+    """Activation checkpointing runs the forward twice; with the state handed in, results and gradients are those of one run."""
+    import approxtorch_b200 as at
+    from torch.utils.checkpoint import checkpoint
+    drop, lin = at.nn.CounterDropout(0.4, seed=5).to(dev), at.nn.Linear_fp8(96, 50, dropout=0.3, seed=6).to(dev)
+    x, go = torch.randn(140, 96, device=dev, requires_grad=True), torch.randn(140, 50, device=dev)
+    r1, r2 = at.backend.ops.dropout_advance(drop.rng), at.backend.ops.dropout_advance(lin.rng)
+    run = lambda t: lin(drop(t, r1), r2)                                     # noqa: E731
+    leaves = (x, lin.weight, lin.bias)
+    y = run(x)
+    want = torch.autograd.grad(y, leaves, go)
+    for reentrant in (False, True):
+        z = checkpoint(run, x, use_reentrant=reentrant)
+        assert torch.equal(z, y)
+        for t in leaves:
+            t.grad = None
+        z.backward(go)
+        assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+    assert drop.rng.tolist() == [5, 1] and lin.rng.tolist() == [6, 1]        # a given state leaves the layer's own as it is
+    with torch.autograd.graph.save_on_cpu():
+        z = run(x)
+    assert all(torch.equal(g, w) for g, w in zip(torch.autograd.grad(z, leaves, go), want))
+    with torch.inference_mode():
+        assert torch.equal(run(x), y)
+
+
 def test_dropout_differentiates_twice(dev):
     import approxtorch_b200 as at
     state = torch.tensor([8, 8], dtype=torch.int64, device=dev)

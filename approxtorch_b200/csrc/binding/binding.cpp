@@ -4,8 +4,10 @@
 // take for one token or a small head, and a layer's forward and backward 300 us.
 #include <ATen/cuda/CUDAContextLight.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -52,6 +54,23 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like)
 }
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// The gradient node of a leaf belongs to the stream on which an operator first asked for it, for as long as a result of that
+// operator lives.  Where that is the default stream and a backward pass is being captured, the engine would make the default
+// stream wait for the captured one, which CUDA refuses at a point where an exception ends the process: refused here, before.
+void check_captured_backward()
+{
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    for (size_t i = 0; node && i < node->num_outputs(); ++i) {
+        const auto& next = node->next_edge(i).function;
+        if (!next || !node->task_should_compute_output(i)) continue;
+        const auto stream = next->stream();
+        TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(stream->device_index()).unwrap(),
+                    "a captured backward pass reaches a gradient node of the default stream: let go of all results that were computed from "
+                    "the same tensors outside the capture (or compute them on a side stream)");
+    }
+}
 
 // ---- dropout -------------------------------------------------------------------------------------------------------
 int drop_threshold(double p)
@@ -110,6 +129,7 @@ struct CounterDropout : torch::autograd::Function<CounterDropout> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
+        check_captured_backward();
         const Tensor rng = ctx->get_saved_variables()[0];
         const double p = ctx->saved_data["p"].toDouble();
         return {CounterDropout::apply(grads[0], p, rng.defined() ? std::optional<Tensor>(rng) : std::nullopt), Tensor(), Tensor()};
@@ -331,6 +351,7 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         TORCH_CHECK(!at::GradMode::is_enabled(), "linear_fp8 has no second derivative (create_graph=True)");
+        check_captured_backward();
         const auto saved = ctx->get_saved_variables();
         const Tensor kept = saved[0], rng = saved[1];
         const double p = ctx->saved_data["p"].toDouble();

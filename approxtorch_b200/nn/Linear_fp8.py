@@ -20,8 +20,8 @@ class Linear_fp8(nn.Module):
     ``CounterDropout``, also for forwards that are run twice); ``state_dict`` keys of ``weight`` and ``bias`` are those of
     ``nn.Linear``.
 
-    A training step can be captured into a CUDA graph.  As with torch's own layers, let go of every result that was computed
-    from the same parameters outside the capture first: their gradient nodes belong to the stream of that computation."""
+    A training step can be captured into a CUDA graph.  Let go of every result that was computed from the same parameters on
+    the default stream first (warm up on a side stream): while one lives, a captured backward pass raises RuntimeError."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, dropout: float = 0.0, seed: int | None = None):
         super().__init__()

@@ -381,6 +381,29 @@ def test_layers_recomputed_with_a_given_state(dev):
         assert torch.equal(run(x), y)
 
 
+def test_captured_backward_beside_an_eager_graph_is_refused(dev):
+    """While a result computed on the default stream holds the leaves' gradient nodes, capturing their backward pass raises;
+    once it is let go the same capture works."""
+    import approxtorch_b200 as at
+    state = torch.tensor([3, 0], dtype=torch.int64, device=dev)
+    x, w, go = torch.randn(64, 96, device=dev), torch.randn(50, 96, device=dev, requires_grad=True), torch.randn(64, 50, device=dev)
+    for run, leaf, g in ((lambda: at.nn.gemm_fp8.linear_fp8(x, w), w, go),
+                         (lambda: at.nn.dropout.counter_dropout(w, 0.5, state), w, torch.randn_like(w))):
+        want, = torch.autograd.grad(run(), leaf, g)
+        alive = run()
+        with pytest.raises(RuntimeError, match="let go of all results"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(run(), leaf, g)
+        torch.cuda.synchronize()
+        assert torch.equal(torch.autograd.grad(alive, leaf, g)[0], want)     # the eager one is whole
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(run(), leaf, g)
+        graph.replay()
+        assert torch.equal(got, want)
+
+
 def test_dropout_differentiates_twice(dev):
     import approxtorch_b200 as at
     state = torch.tensor([8, 8], dtype=torch.int64, device=dev)

@@ -32,7 +32,7 @@ struct QuantArgs {
     long long ldst;
     float* sums;      // [ceil(R/128), C]
     DropState drop;
-    unsigned ct;      // tiles of 128 columns
+    unsigned ct, tiles;      // tiles of 128 columns; of the matrix
 };
 
 // What a lane holds of a row: 16 bytes in the input's own type (8 bf16 or fp16, 4 fp32).  Magnitudes are compared in that
@@ -165,7 +165,7 @@ __device__ __forceinline__ void drop_draws4(unsigned (&w)[4], unsigned d0, unsig
 // The transposed image turns through shared memory so that it leaves in 128-byte rows: column c is row c of s_turn, its
 // 8-byte pieces (8 rows of one lane) permuted by the column so that the lanes of a write spread over all banks.
 //
-// Measured, bf16 8192 x 8192: kRows 32.5 us (floor 30.7), kBoth 51.4 us (41.0), with dropout 50 and 64 us (the draws take 22 us of
+// Measured, bf16 8192 x 8192: kRows 32.5 us (floor 30.7), kBoth 47.8 us (41.0), with dropout 50 and 64 us (the draws take 22 us of
 // the multiply pipe); fp32 4096 x 4096 kSquare, both layouts, 19.0 us (15.4).  Rows that start anywhere (8191 x 4095): kRows
 // 27.8 us (15.4), kBoth 39 us (20.5).
 enum QuantMode { kRows = 0, kBoth = 1, kSquare = 2 };
@@ -173,222 +173,257 @@ template <class T> constexpr int kQuantThreads = 16 * 128 / Piece<T>::kElems;   
 
 // SUM: the columns' sums over the tile's rows besides (a bias gradient reads the same matrix).  ALIGNED: rows start on
 // 16-byte boundaries and have a multiple of 8 elements, so that a lane's 16 bytes are one load and one draw.
-template <class T, bool E5, bool ALIGNED, bool DROP, int MODE, bool SUM = false>
-__global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 ? 3 : 2) quantize_kernel(const QuantArgs a)
+//
+// AHEAD: two blocks to an SM that go from tile to tile and ask for the next one (cp.async into the lane's own places) while
+// they work on this one.  For both layouts of 2-byte types without draws, where more tiles than that are waiting: bf16
+// 8192 x 8192 47.7 us instead of 51.4, 8192 x 4096 25.0 instead of 27.0.  Elsewhere it costs more than it hides (same size:
+// rows 34.1 instead of 32.6 us, squares 45.7 and 45.0, both layouts with draws 73 instead of 64, bound by instructions; fp32
+// 4096 x 4096 both layouts 20.3 and 20.2).
+template <class T, bool E5, bool ALIGNED, bool DROP, int MODE, bool SUM = false, bool AHEAD = false>
+__global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 && !AHEAD ? 3 : 2) quantize_kernel(const QuantArgs a)
 {
+    static_assert(!AHEAD || (ALIGNED && MODE == kBoth), "the next tile is asked for 16 aligned bytes at a time");
     using P = Piece<T>;
     constexpr int kElems = P::kElems, kLanes = 128 / kElems;                       // of a row
     constexpr int kWarps = kQuantThreads<T> / 32, kWords = 128 * static_cast<int>(sizeof(T)) / 4;   // words of a row
+    extern __shared__ __align__(16) uint4 s_ahead[];         // AHEAD: [8][kQuantThreads], a lane's rows
     __shared__ __align__(16) unsigned s_max[MODE == kRows ? 1 : kWarps][MODE == kRows ? 4 : kWords];
     __shared__ __align__(16) float s_inv[MODE == kBoth ? 128 : 4];
     __shared__ float s_sum[SUM ? kWarps : 1][SUM ? 128 : 1];
     __shared__ __align__(16) uint8_t s_turn[MODE == kRows ? 16 : 128 * 128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, in_row = lane % kLanes;
     const int strip = threadIdx.x / kLanes;                                        // of 8 rows, 0 .. 15
-    const unsigned tile_r = blockIdx.x / a.ct, tile_c = blockIdx.x - tile_r * a.ct;
-    const long long r0 = static_cast<long long>(tile_r) * 128 + strip * 8, c0 = static_cast<long long>(tile_c) * 128;
-    const long long c = c0 + in_row * kElems;
-    const int rows = static_cast<int>(max(0ll, min(8ll, a.R - r0)));
-    if (MODE == kRows && a.R <= r0 - (strip * 8) % (32 / kLanes * 8)) return;      // nothing for this warp
-    const T* const x = static_cast<const T*>(a.x) + r0 * a.ldx + c;
-    after_previous();
-
-    unsigned v[8][4];
-    const bool whole = rows == 8 && c0 + 128 <= a.C;         // the same for the block's warps but in the last tiles
-    if (ALIGNED && whole) {
+    auto ask = [&](unsigned tile) {                          // zeros for what lies outside the matrix
+        const unsigned tile_r = tile / a.ct, tile_c = tile - tile_r * a.ct;
+        const long long r0 = static_cast<long long>(tile_r) * 128 + strip * 8, c = static_cast<long long>(tile_c) * 128 + in_row * kElems;
+        const T* const x = static_cast<const T*>(a.x) + r0 * a.ldx + c;
+        const long long rows = c < a.C ? a.R - r0 : 0;
+        const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(s_ahead + threadIdx.x));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint4 q = read16_once(x + i * a.ldx);
-            v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
-        }
-    } else if (ALIGNED) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint4 q = i < rows && c < a.C ? read16_once(x + i * a.ldx) : make_uint4(0, 0, 0, 0);
-            v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
-        }
-    } else if (whole) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) load_piece<T, true>(x + i * a.ldx, kElems, v[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) load_piece<T, false>(x + i * a.ldx, i < rows ? a.C - c : 0, v[i]);
+        for (int i = 0; i < 8; ++i)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * kQuantThreads<T> * 16),
+                         "l"(i < rows ? x + i * a.ldx : static_cast<const T*>(a.x)), "r"(i < rows ? 16 : 0) : "memory");
+    };
+    unsigned tile = blockIdx.x;
+    if (AHEAD) {
+        after_previous();
+        ask(tile);
     }
-    if (DROP) {
-        PhiloxKey key(a.drop.rng);
-        key.settle();
-        const unsigned high = a.drop.threshold << 16;
-        if (a.drop.threshold >= 65536u) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[i][j] = 0;
-        } else if (ALIGNED) {
-            const unsigned long long g = static_cast<unsigned long long>(r0 * a.C + c) >> 3, row = static_cast<unsigned long long>(a.C) >> 3;
-            if (kElems == 8) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) drop_draws8(v[i], philox4x32_10(key, g + i * row), high);
-            } else {
-                // a group of 8 elements is two lanes' share of a row: each draws for four rows and they exchange halves
-                const bool odd = lane & 1;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint4 d = philox4x32_10(key, g + (odd ? i + 4 : i) * row);
-                    const unsigned e0 = __shfl_xor_sync(0xFFFFFFFFu, odd ? d.x : d.z, 1), e1 = __shfl_xor_sync(0xFFFFFFFFu, odd ? d.y : d.w, 1);
-                    drop_draws4(v[i], odd ? e0 : d.x, odd ? e1 : d.y, high);
-                    drop_draws4(v[i + 4], odd ? d.z : e0, odd ? d.w : e1, high);
-                }
-            }
-        } else {
-            // Pieces straddle groups of 8 draws: a lane draws the group of its first element and takes the next group from the
-            // next lane.  What the last lanes of the 8 (16) rows are short of, a lane each draws for one row, in one call.
-            const int extra_row = lane % 8, extra_strip = strip - lane / kLanes + lane / 8 % (32 / kLanes);
-            const unsigned long long e_extra = static_cast<unsigned long long>((static_cast<long long>(tile_r) * 128 + extra_strip * 8 + extra_row) * a.C + c0 + 128 - kElems);
-            const uint4 extra = philox4x32_10(key, (e_extra >> 3) + 1);
+    do {
+        const unsigned tile_r = tile / a.ct, tile_c = tile - tile_r * a.ct;
+        const long long r0 = static_cast<long long>(tile_r) * 128 + strip * 8, c0 = static_cast<long long>(tile_c) * 128;
+        const long long c = c0 + in_row * kElems;
+        const int rows = static_cast<int>(max(0ll, min(8ll, a.R - r0)));
+        if (MODE == kRows && a.R <= r0 - (strip * 8) % (32 / kLanes * 8)) return;      // nothing for this warp
+        const T* const x = static_cast<const T*>(a.x) + r0 * a.ldx + c;
+        if (!AHEAD) after_previous();
+
+        unsigned v[8][4];
+        const bool whole = rows == 8 && c0 + 128 <= a.C;         // the same for the block's warps but in the last tiles
+        if (AHEAD) {
+            asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const unsigned long long e = static_cast<unsigned long long>((r0 + i) * a.C + c);
-                const uint4 own = philox4x32_10(key, e >> 3);
-                uint4 next = from_next_lane(own);
-                const int from = lane / kLanes * 8 + i;      // of the lane that drew for this row
-                const uint4 x = make_uint4(__shfl_sync(0xFFFFFFFFu, extra.x, from), __shfl_sync(0xFFFFFFFFu, extra.y, from),
-                                           __shfl_sync(0xFFFFFFFFu, extra.z, from), __shfl_sync(0xFFFFFFFFu, extra.w, from));
-                if (in_row == kLanes - 1) next = x;
-                unsigned d[4];
-                shifted(own, next, 2u * static_cast<unsigned>(e & 7u), d);
-                if (kElems == 8) drop_draws8(v[i], make_uint4(d[0], d[1], d[2], d[3]), high);
-                else drop_draws4(v[i], d[0], d[1], high);
+                const uint4 q = s_ahead[i * kQuantThreads<T> + threadIdx.x];
+                v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
             }
-        }
-    }
-
-    // maxima of the rows, and of the columns over this lane's rows
-    unsigned top[8], col[4];
+        } else if (ALIGNED && whole) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const unsigned m0 = P::mag(v[i][0]), m1 = P::mag(v[i][1]), m2 = P::mag(v[i][2]), m3 = P::mag(v[i][3]);
-        top[i] = P::larger(P::larger(m0, m1), P::larger(m2, m3));
-        if (MODE == kBoth) {
-            col[0] = i ? P::larger(col[0], m0) : m0; col[1] = i ? P::larger(col[1], m1) : m1;
-            col[2] = i ? P::larger(col[2], m2) : m2; col[3] = i ? P::larger(col[3], m3) : m3;
-        }
-    }
-    float inv[8];                                            // 1 / scale of this lane's rows
-    if (MODE == kSquare) {
-        unsigned m = top[0];
-#pragma unroll
-        for (int i = 1; i < 8; ++i) m = P::larger(m, top[i]);
-        m = __reduce_max_sync(0xFFFFFFFFu, P::fp32_bits(m));
-        if (lane == 0) s_max[warp][0] = m;
-        __syncthreads();
-        m = __reduce_max_sync(0xFFFFFFFFu, lane < kWarps ? s_max[lane][0] : 0u);
-        const unsigned byte = scale_byte<E5>(m);
-        inv[0] = inverse_scale(byte);
-#pragma unroll
-        for (int i = 1; i < 8; ++i) inv[i] = inv[0];
-        if (threadIdx.x == 0) {
-            a.s[tile_r * a.lds + tile_c] = static_cast<uint8_t>(byte);
-            if (a.st) a.st[tile_c * a.ldst + tile_r] = static_cast<uint8_t>(byte);
-        }
-    } else {
-        if (MODE == kBoth) {
-            if (kLanes == 16) {                              // the warp's two strips
-#pragma unroll
-                for (int j = 0; j < 4; ++j) col[j] = P::larger(col[j], __shfl_xor_sync(0xFFFFFFFFu, col[j], 16));
+            for (int i = 0; i < 8; ++i) {
+                const uint4 q = read16_once(x + i * a.ldx);
+                v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
             }
-            if (lane < kLanes) *reinterpret_cast<uint4*>(&s_max[warp][in_row * 4]) = make_uint4(col[0], col[1], col[2], col[3]);
-            if constexpr (SUM) {
-                auto add = [&](int j, float f) {
-                    if (kLanes == 16) f += __shfl_xor_sync(0xFFFFFFFFu, f, 16);
-                    if (lane < kLanes) s_sum[warp][in_row * kElems + j] = f;
-                };
-#define ATB_COLUMN(J) (((P::template get<J>(v[0]) + P::template get<J>(v[1])) + (P::template get<J>(v[2]) + P::template get<J>(v[3]))) + \
-                       ((P::template get<J>(v[4]) + P::template get<J>(v[5])) + (P::template get<J>(v[6]) + P::template get<J>(v[7]))))
-                add(0, ATB_COLUMN(0)); add(1, ATB_COLUMN(1)); add(2, ATB_COLUMN(2)); add(3, ATB_COLUMN(3));
-                if constexpr (kElems == 8) { add(4, ATB_COLUMN(4)); add(5, ATB_COLUMN(5)); add(6, ATB_COLUMN(6)); add(7, ATB_COLUMN(7)); }
-#undef ATB_COLUMN
+        } else if (ALIGNED) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint4 q = i < rows && c < a.C ? read16_once(x + i * a.ldx) : make_uint4(0, 0, 0, 0);
+                v[i][0] = q.x; v[i][1] = q.y; v[i][2] = q.z; v[i][3] = q.w;
             }
-        }
-        // 8 rows x kLanes lanes: with every step a lane keeps half of its rows, the upper half if its bit is set
+        } else if (whole) {
 #pragma unroll
-        for (int half = 4, bit = kLanes / 2; half >= 1; half >>= 1, bit >>= 1) {
-            const bool upper = lane & bit;
-#pragma unroll
-            for (int i = 0; i < half; ++i) {
-                const unsigned keep = upper ? top[i + half] : top[i], give = upper ? top[i] : top[i + half];
-                top[i] = P::larger(keep, __shfl_xor_sync(0xFFFFFFFFu, give, bit));
-            }
-        }
-#pragma unroll
-        for (int bit = kLanes / 16; bit >= 1; bit >>= 1) top[0] = P::larger(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], bit));
-        const int row = in_row / (kLanes / 8);               // the one this lane is left with
-        const unsigned byte = scale_byte<E5>(P::fp32_bits(top[0]));
-        const float mine = inverse_scale(byte);
-        if (in_row % (kLanes / 8) == 0 && row < rows) a.s[(r0 + row) * a.lds + tile_c] = static_cast<uint8_t>(byte);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) inv[i] = __shfl_sync(0xFFFFFFFFu, mine, i * (kLanes / 8), kLanes);
-    }
-    // the image as it lies
-    uint8_t* const q = a.q + r0 * a.ldq + c;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const unsigned lo = pack4<E5>(P::template get<0>(v[i]) * inv[i], P::template get<1>(v[i]) * inv[i],
-                                      P::template get<2>(v[i]) * inv[i], P::template get<3>(v[i]) * inv[i]);
-        if constexpr (kElems == 8) {
-            const unsigned hi = pack4<E5>(P::template get<4>(v[i]) * inv[i], P::template get<5>(v[i]) * inv[i],
-                                          P::template get<6>(v[i]) * inv[i], P::template get<7>(v[i]) * inv[i]);
-            if (i < rows && c < a.ldq) *reinterpret_cast<uint2*>(q + i * a.ldq) = make_uint2(lo, hi);
+            for (int i = 0; i < 8; ++i) load_piece<T, true>(x + i * a.ldx, kElems, v[i]);
         } else {
-            if (i < rows && c < a.ldq) *reinterpret_cast<unsigned*>(q + i * a.ldq) = lo;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) load_piece<T, false>(x + i * a.ldx, i < rows ? a.C - c : 0, v[i]);
         }
-    }
-    if (MODE == kRows || a.qt == nullptr) return;
-
-    if (MODE == kBoth) {
-        __syncthreads();
-        if (SUM && threadIdx.x >= kQuantThreads<T> - 128) {  // (not the warps that make the scales)
-            const int cc = threadIdx.x - (kQuantThreads<T> - 128);
-            float f = 0.0f;
+        if (DROP) {
+            PhiloxKey key(a.drop.rng);
+            key.settle();
+            const unsigned high = a.drop.threshold << 16;
+            if (a.drop.threshold >= 65536u) {
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) f += s_sum[w][cc];
-            if (c0 + cc < a.C) a.sums[tile_r * a.C + c0 + cc] = f;
-        }
-        if (threadIdx.x < kWords) {                          // a word's columns (one, or two halves)
-            unsigned m = s_max[0][threadIdx.x];
+                for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) m = P::larger(m, s_max[w][threadIdx.x]);
-            constexpr int kPer = 128 / kWords;
+                    for (int j = 0; j < 4; ++j) v[i][j] = 0;
+            } else if (ALIGNED) {
+                const unsigned long long g = static_cast<unsigned long long>(r0 * a.C + c) >> 3, row = static_cast<unsigned long long>(a.C) >> 3;
+                if (kElems == 8) {
 #pragma unroll
-            for (int h = 0; h < kPer; ++h) {
-                const int cc = threadIdx.x * kPer + h;
-                const unsigned one = kPer == 1 ? m : h ? m >> 16 : m & 0xFFFFu;
-                const unsigned byte = scale_byte<E5>(P::fp32_bits(one));
-                s_inv[cc] = inverse_scale(byte);
-                if (c0 + cc < a.C) a.st[(c0 + cc) * a.ldst + tile_r] = static_cast<uint8_t>(byte);
+                    for (int i = 0; i < 8; ++i) drop_draws8(v[i], philox4x32_10(key, g + i * row), high);
+                } else {
+                    // a group of 8 elements is two lanes' share of a row: each draws for four rows and they exchange halves
+                    const bool odd = lane & 1;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 d = philox4x32_10(key, g + (odd ? i + 4 : i) * row);
+                        const unsigned e0 = __shfl_xor_sync(0xFFFFFFFFu, odd ? d.x : d.z, 1), e1 = __shfl_xor_sync(0xFFFFFFFFu, odd ? d.y : d.w, 1);
+                        drop_draws4(v[i], odd ? e0 : d.x, odd ? e1 : d.y, high);
+                        drop_draws4(v[i + 4], odd ? d.z : e0, odd ? d.w : e1, high);
+                    }
+                }
+            } else {
+                // Pieces straddle groups of 8 draws: a lane draws the group of its first element and takes the next group from the
+                // next lane.  What the last lanes of the 8 (16) rows are short of, a lane each draws for one row, in one call.
+                const int extra_row = lane % 8, extra_strip = strip - lane / kLanes + lane / 8 % (32 / kLanes);
+                const unsigned long long e_extra = static_cast<unsigned long long>((static_cast<long long>(tile_r) * 128 + extra_strip * 8 + extra_row) * a.C + c0 + 128 - kElems);
+                const uint4 extra = philox4x32_10(key, (e_extra >> 3) + 1);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const unsigned long long e = static_cast<unsigned long long>((r0 + i) * a.C + c);
+                    const uint4 own = philox4x32_10(key, e >> 3);
+                    uint4 next = from_next_lane(own);
+                    const int from = lane / kLanes * 8 + i;      // of the lane that drew for this row
+                    const uint4 x = make_uint4(__shfl_sync(0xFFFFFFFFu, extra.x, from), __shfl_sync(0xFFFFFFFFu, extra.y, from),
+                                               __shfl_sync(0xFFFFFFFFu, extra.z, from), __shfl_sync(0xFFFFFFFFu, extra.w, from));
+                    if (in_row == kLanes - 1) next = x;
+                    unsigned d[4];
+                    shifted(own, next, 2u * static_cast<unsigned>(e & 7u), d);
+                    if (kElems == 8) drop_draws8(v[i], make_uint4(d[0], d[1], d[2], d[3]), high);
+                    else drop_draws4(v[i], d[0], d[1], high);
+                }
             }
         }
-        __syncthreads();
-    }
-    auto turn = [&](int j, float f0, float f1, float f2, float f3, float f4, float f5, float f6, float f7) {
-        const float by = MODE == kBoth ? s_inv[in_row * kElems + j] : inv[0];
-        const int cc = in_row * kElems + j;
-        *reinterpret_cast<uint2*>(s_turn + cc * 128 + ((strip ^ in_row % 16) << 3)) =
-            make_uint2(pack4<E5>(f0 * by, f1 * by, f2 * by, f3 * by), pack4<E5>(f4 * by, f5 * by, f6 * by, f7 * by));
-    };
-#define ATB_TURN(J) turn(J, P::template get<J>(v[0]), P::template get<J>(v[1]), P::template get<J>(v[2]), P::template get<J>(v[3]), \
-                         P::template get<J>(v[4]), P::template get<J>(v[5]), P::template get<J>(v[6]), P::template get<J>(v[7]))
-    ATB_TURN(0); ATB_TURN(1); ATB_TURN(2); ATB_TURN(3);
-    if constexpr (kElems == 8) { ATB_TURN(4); ATB_TURN(5); ATB_TURN(6); ATB_TURN(7); }
-#undef ATB_TURN
-    __syncthreads();
-    const long long rt = static_cast<long long>(tile_r) * 128;
+
+        // maxima of the rows, and of the columns over this lane's rows
+        unsigned top[8], col[4];
 #pragma unroll
-    for (int i = 0; i < 1024 / kQuantThreads<T>; ++i) {
-        const int cc = (threadIdx.x >> 3) + kQuantThreads<T> / 8 * i, piece = threadIdx.x & 7, by = cc / kElems % 16;
-        uint4 o = *reinterpret_cast<const uint4*>(s_turn + cc * 128 + ((piece ^ (by >> 1)) << 4));
-        if (by & 1) o = make_uint4(o.z, o.w, o.x, o.y);
-        if (c0 + cc < a.C && rt + piece * 16 < a.ldqt) *reinterpret_cast<uint4*>(a.qt + (c0 + cc) * a.ldqt + rt + piece * 16) = o;
-    }
+        for (int i = 0; i < 8; ++i) {
+            const unsigned m0 = P::mag(v[i][0]), m1 = P::mag(v[i][1]), m2 = P::mag(v[i][2]), m3 = P::mag(v[i][3]);
+            top[i] = P::larger(P::larger(m0, m1), P::larger(m2, m3));
+            if (MODE == kBoth) {
+                col[0] = i ? P::larger(col[0], m0) : m0; col[1] = i ? P::larger(col[1], m1) : m1;
+                col[2] = i ? P::larger(col[2], m2) : m2; col[3] = i ? P::larger(col[3], m3) : m3;
+            }
+        }
+        float inv[8];                                            // 1 / scale of this lane's rows
+        if (MODE == kSquare) {
+            unsigned m = top[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) m = P::larger(m, top[i]);
+            m = __reduce_max_sync(0xFFFFFFFFu, P::fp32_bits(m));
+            if (lane == 0) s_max[warp][0] = m;
+            __syncthreads();
+            m = __reduce_max_sync(0xFFFFFFFFu, lane < kWarps ? s_max[lane][0] : 0u);
+            const unsigned byte = scale_byte<E5>(m);
+            inv[0] = inverse_scale(byte);
+#pragma unroll
+            for (int i = 1; i < 8; ++i) inv[i] = inv[0];
+            if (threadIdx.x == 0) {
+                a.s[tile_r * a.lds + tile_c] = static_cast<uint8_t>(byte);
+                if (a.st) a.st[tile_c * a.ldst + tile_r] = static_cast<uint8_t>(byte);
+            }
+        } else {
+            if (MODE == kBoth) {
+                if (kLanes == 16) {                              // the warp's two strips
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) col[j] = P::larger(col[j], __shfl_xor_sync(0xFFFFFFFFu, col[j], 16));
+                }
+                if (lane < kLanes) *reinterpret_cast<uint4*>(&s_max[warp][in_row * 4]) = make_uint4(col[0], col[1], col[2], col[3]);
+                if constexpr (SUM) {
+                    auto add = [&](int j, float f) {
+                        if (kLanes == 16) f += __shfl_xor_sync(0xFFFFFFFFu, f, 16);
+                        if (lane < kLanes) s_sum[warp][in_row * kElems + j] = f;
+                    };
+#define ATB_COLUMN(J) (((P::template get<J>(v[0]) + P::template get<J>(v[1])) + (P::template get<J>(v[2]) + P::template get<J>(v[3]))) + \
+                           ((P::template get<J>(v[4]) + P::template get<J>(v[5])) + (P::template get<J>(v[6]) + P::template get<J>(v[7]))))
+                    add(0, ATB_COLUMN(0)); add(1, ATB_COLUMN(1)); add(2, ATB_COLUMN(2)); add(3, ATB_COLUMN(3));
+                    if constexpr (kElems == 8) { add(4, ATB_COLUMN(4)); add(5, ATB_COLUMN(5)); add(6, ATB_COLUMN(6)); add(7, ATB_COLUMN(7)); }
+#undef ATB_COLUMN
+                }
+            }
+            // 8 rows x kLanes lanes: with every step a lane keeps half of its rows, the upper half if its bit is set
+#pragma unroll
+            for (int half = 4, bit = kLanes / 2; half >= 1; half >>= 1, bit >>= 1) {
+                const bool upper = lane & bit;
+#pragma unroll
+                for (int i = 0; i < half; ++i) {
+                    const unsigned keep = upper ? top[i + half] : top[i], give = upper ? top[i] : top[i + half];
+                    top[i] = P::larger(keep, __shfl_xor_sync(0xFFFFFFFFu, give, bit));
+                }
+            }
+#pragma unroll
+            for (int bit = kLanes / 16; bit >= 1; bit >>= 1) top[0] = P::larger(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], bit));
+            if (AHEAD && tile + gridDim.x < a.tiles) ask(tile + gridDim.x);          // the maxima have used every value: all are in registers
+            const int row = in_row / (kLanes / 8);               // the one this lane is left with
+            const unsigned byte = scale_byte<E5>(P::fp32_bits(top[0]));
+            const float mine = inverse_scale(byte);
+            if (in_row % (kLanes / 8) == 0 && row < rows) a.s[(r0 + row) * a.lds + tile_c] = static_cast<uint8_t>(byte);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) inv[i] = __shfl_sync(0xFFFFFFFFu, mine, i * (kLanes / 8), kLanes);
+        }
+        // the image as it lies
+        uint8_t* const q = a.q + r0 * a.ldq + c;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const unsigned lo = pack4<E5>(P::template get<0>(v[i]) * inv[i], P::template get<1>(v[i]) * inv[i],
+                                          P::template get<2>(v[i]) * inv[i], P::template get<3>(v[i]) * inv[i]);
+            if constexpr (kElems == 8) {
+                const unsigned hi = pack4<E5>(P::template get<4>(v[i]) * inv[i], P::template get<5>(v[i]) * inv[i],
+                                              P::template get<6>(v[i]) * inv[i], P::template get<7>(v[i]) * inv[i]);
+                if (i < rows && c < a.ldq) *reinterpret_cast<uint2*>(q + i * a.ldq) = make_uint2(lo, hi);
+            } else {
+                if (i < rows && c < a.ldq) *reinterpret_cast<unsigned*>(q + i * a.ldq) = lo;
+            }
+        }
+        if (MODE == kRows || a.qt == nullptr) return;
+
+        if (MODE == kBoth) {
+            __syncthreads();
+            if (SUM && threadIdx.x >= kQuantThreads<T> - 128) {  // (not the warps that make the scales)
+                const int cc = threadIdx.x - (kQuantThreads<T> - 128);
+                float f = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) f += s_sum[w][cc];
+                if (c0 + cc < a.C) a.sums[tile_r * a.C + c0 + cc] = f;
+            }
+            if (threadIdx.x < kWords) {                          // a word's columns (one, or two halves)
+                unsigned m = s_max[0][threadIdx.x];
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) m = P::larger(m, s_max[w][threadIdx.x]);
+                constexpr int kPer = 128 / kWords;
+#pragma unroll
+                for (int h = 0; h < kPer; ++h) {
+                    const int cc = threadIdx.x * kPer + h;
+                    const unsigned one = kPer == 1 ? m : h ? m >> 16 : m & 0xFFFFu;
+                    const unsigned byte = scale_byte<E5>(P::fp32_bits(one));
+                    s_inv[cc] = inverse_scale(byte);
+                    if (c0 + cc < a.C) a.st[(c0 + cc) * a.ldst + tile_r] = static_cast<uint8_t>(byte);
+                }
+            }
+            __syncthreads();
+        }
+        auto turn = [&](int j, float f0, float f1, float f2, float f3, float f4, float f5, float f6, float f7) {
+            const float by = MODE == kBoth ? s_inv[in_row * kElems + j] : inv[0];
+            const int cc = in_row * kElems + j;
+            *reinterpret_cast<uint2*>(s_turn + cc * 128 + ((strip ^ in_row % 16) << 3)) =
+                make_uint2(pack4<E5>(f0 * by, f1 * by, f2 * by, f3 * by), pack4<E5>(f4 * by, f5 * by, f6 * by, f7 * by));
+        };
+#define ATB_TURN(J) turn(J, P::template get<J>(v[0]), P::template get<J>(v[1]), P::template get<J>(v[2]), P::template get<J>(v[3]), \
+                             P::template get<J>(v[4]), P::template get<J>(v[5]), P::template get<J>(v[6]), P::template get<J>(v[7]))
+        ATB_TURN(0); ATB_TURN(1); ATB_TURN(2); ATB_TURN(3);
+        if constexpr (kElems == 8) { ATB_TURN(4); ATB_TURN(5); ATB_TURN(6); ATB_TURN(7); }
+#undef ATB_TURN
+        __syncthreads();
+        const long long rt = static_cast<long long>(tile_r) * 128;
+#pragma unroll
+        for (int i = 0; i < 1024 / kQuantThreads<T>; ++i) {
+            const int cc = (threadIdx.x >> 3) + kQuantThreads<T> / 8 * i, piece = threadIdx.x & 7, by = cc / kElems % 16;
+            uint4 o = *reinterpret_cast<const uint4*>(s_turn + cc * 128 + ((piece ^ (by >> 1)) << 4));
+            if (by & 1) o = make_uint4(o.z, o.w, o.x, o.y);
+            if (c0 + cc < a.C && rt + piece * 16 < a.ldqt) *reinterpret_cast<uint4*>(a.qt + (c0 + cc) * a.ldqt + rt + piece * 16) = o;
+        }
+        // (what the next tile writes to shared memory is written one barrier at least after this tile's last read of it)
+    } while (AHEAD && (tile += gridDim.x) < a.tiles);
 }
 
 // out[c] = the sum of column c of p [rows, C], in the order of the rows
@@ -403,11 +438,31 @@ __global__ void __launch_bounds__(256) sum_rows_kernel(const float* p, int rows,
     out[c] = f;
 }
 
-template <class T, bool E5, bool ALIGNED>
-static int launch_quantize_as(const QuantArgs& a, bool square, unsigned tiles, cudaStream_t s)
+// both layouts of an aligned matrix of a 2-byte type, more tiles than two blocks an SM
+template <class T, bool E5, bool SUM>
+static int launch_quantize_ahead(const QuantArgs& a, cudaStream_t s)
 {
-    const dim3 grid(tiles), block(kQuantThreads<T>);
+    const int smem = 8 * 16 * kQuantThreads<T>;              // with what is declared in the kernel, above the default limit
+    static bool done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 64 || !done[dev]))
+        e = cudaFuncSetAttribute(quantize_kernel<T, E5, true, false, kBoth, SUM, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return fail_invalid(cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) done[dev] = true;
+    launch_after(quantize_kernel<T, E5, true, false, kBoth, SUM, true>, dim3(2 * sm_count()), dim3(kQuantThreads<T>), smem, s, 0, a);
+    return check_launch("quantize_kernel");
+}
+
+template <class T, bool E5, bool ALIGNED>
+static int launch_quantize_as(const QuantArgs& a, bool square, cudaStream_t s)
+{
+    const dim3 grid(a.tiles), block(kQuantThreads<T>);
     const bool drop = a.drop.rng != nullptr;
+    if constexpr (ALIGNED && sizeof(T) == 2) {
+        if (!square && a.qt != nullptr && !drop && a.tiles > 2u * sm_count())
+            return a.sums ? launch_quantize_ahead<T, E5, true>(a, s) : launch_quantize_ahead<T, E5, false>(a, s);
+    }
     if (square) launch_after(quantize_kernel<T, E5, ALIGNED, false, kSquare>, grid, block, 0, s, 0, a);
     else if (a.qt == nullptr) {
         if (drop) launch_after(quantize_kernel<T, E5, ALIGNED, true, kRows>, grid, block, 0, s, 0, a);
@@ -424,9 +479,10 @@ static int launch_quantize(QuantArgs a, bool square, cudaStream_t s)
     const long long ct = (a.C + 127) >> 7, tiles = ((a.R + 127) >> 7) * ct;
     ATB_REQUIRE(tiles < (1ll << 31), "matrix too large");
     a.ct = static_cast<unsigned>(ct);
+    a.tiles = static_cast<unsigned>(tiles);
     const bool aligned = aligned_to(a.x, 16) && (a.ldx * static_cast<long long>(sizeof(T))) % 16 == 0 && a.C % 8 == 0;
-    return aligned ? launch_quantize_as<T, E5, true>(a, square, static_cast<unsigned>(tiles), s)
-                   : launch_quantize_as<T, E5, false>(a, square, static_cast<unsigned>(tiles), s);
+    return aligned ? launch_quantize_as<T, E5, true>(a, square, s)
+                   : launch_quantize_as<T, E5, false>(a, square, s);
 }
 
 }  // namespace atb
@@ -453,7 +509,7 @@ extern "C" int atb_fp8_quantize(const void* x, int x_dtype, long long R, long lo
                 "column sums go with both layouts, blocks of one row and no dropout");
     ATB_REQUIRE(drop_threshold == 0 || (rng != nullptr && aligned_to(rng, 8)), "dropout needs an 8-byte aligned state");
     QuantArgs a{x, R, C, ldx, static_cast<uint8_t*>(q), ldq, s, lds, static_cast<uint8_t*>(qt), ldqt, st, ldst, column_sums,
-                DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)}, 0};
+                DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)}, 0, 0};
     cudaStream_t stm = static_cast<cudaStream_t>(stream);
     const bool e5 = f8 == ATB_E5M2, square = block_rows == 128;
     if (x_dtype == ATB_F32) return e5 ? launch_quantize<float, true>(a, square, stm) : launch_quantize<float, false>(a, square, stm);

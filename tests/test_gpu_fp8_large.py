@@ -224,6 +224,39 @@ def test_c_quantiser_writes_its_rows_and_nothing_else(dev):
             assert (tail == 0xEE).all()
 
 
+@pytest.mark.parametrize("fmt", [torch.float8_e4m3fn, torch.float8_e5m2], ids=["e4m3", "e5m2"])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,C,pitch", [(2500, 2056, 2056), (128, 128 * 301, 128 * 301), (128 * 331 - 7, 120, 136), (9000, 1000, 1024)])
+def test_both_layouts_of_more_tiles_than_resident_blocks(dev, R, C, pitch, dt, fmt):
+    """Blocks that go from tile to tile write what a block a tile would: equal to the two images made one at a time."""
+    from approxtorch_b200.backend import _C, ops
+    g = torch.Generator(dev).manual_seed(5)
+    x = torch.full((R, pitch), float("nan"), device=dev, dtype=dt)[:, :C]
+    x.copy_(_x(g, R, C))
+    x[R // 2, C // 3], x[R - 1, C - 1], x[0, 5] = float("inf"), float("nan"), 0.0
+    q, s, qt, st = ops.fp8_quantize_both(x, fmt)
+    for got, want in zip((q, s, qt, st), (*ops.fp8_quantize_rows(x, fmt), *ops.fp8_quantize_rows(x.t().contiguous(), fmt))):
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8))
+    # column sums over each 128 rows: 128 values added in fp32, off by at most 127 half steps of the magnitudes' sum
+    x[R // 2, C // 3], x[R - 1, C - 1] = 1.0, 2.0
+    nb, up = -(-R // 128), lambda v: -(-v // 16) * 16                        # noqa: E731
+    sums = torch.full((nb * C + 16,), -7.0, device=dev)
+    bufs = [torch.empty(n, dtype=torch.uint8, device=dev) for n in (R * up(C), R * up(-(-C // 128)), C * up(R), C * up(nb))]
+    code = 3 if dt == torch.bfloat16 else 4
+    assert _C.lib.atb_fp8_quantize(x.data_ptr(), code, R, C, pitch, 5 if fmt == E4 else 6, 1, bufs[0].data_ptr(), up(C), bufs[1].data_ptr(),
+                                   up(-(-C // 128)), bufs[2].data_ptr(), up(R), bufs[3].data_ptr(), up(nb), sums.data_ptr(), 0, None,
+                                   ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    xd = torch.zeros(nb * 128, C, dtype=torch.float64, device=dev)
+    xd[:R] = x.double()
+    xd = xd.view(nb, 128, C)
+    assert (sums[nb * C:] == -7.0).all()
+    assert ((sums[:nb * C].view(nb, C).double() - xd.sum(1)).abs() <= 127 * 2.0 ** -24 * xd.abs().sum(1)).all()
+    want = ops.fp8_quantize_both(x, fmt)
+    for buf, w in zip(bufs, want):
+        rows, width = w.shape
+        assert torch.equal(buf.view(rows, up(width))[:, :width], w.view(torch.uint8))
+
+
 def test_two_streams_at_once(dev):
     """Products, quantisers and dropout of two streams in flight together give what they give alone."""
     from approxtorch_b200.backend import ops

@@ -8,8 +8,8 @@
 // exponent byte e + 127.  A block that holds a NaN or an infinity gets the scale NaN (byte 255) and NaN in every place:
 // it cannot pass unseen.
 //
-// The reduction over magnitudes works on the bit patterns as unsigned integers: |x| orders like its bits, infinities come
-// out above every number and NaNs above them.
+// The reduction over magnitudes takes the maximum of absolute values as one instruction (max.xorsign.abs: the result's sign is
+// the exclusive or of the operands' and is cleared at the end), a NaN winning over everything; scales are made from the bits.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -36,24 +36,28 @@ struct QuantArgs {
 };
 
 // What a lane holds of a row: 16 bytes in the input's own type (8 bf16 or fp16, 4 fp32).  Magnitudes are compared in that
-// type, two halves at a time where it has 16 bits; a NaN is kept as the larger.  Element order: word by word, low half first.
+// type, two halves at a time where it has 16 bits.  Element order: word by word, low half first.
 template <class T> struct Piece;
 template <> struct Piece<float> {
     static constexpr int kElems = 4;
-    static __device__ __forceinline__ unsigned mag(unsigned w) { return w & 0x7FFFFFFFu; }
-    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return max(a, b); }
-    static __device__ __forceinline__ unsigned fp32_bits(unsigned m) { return m; }               // of a whole word's maximum
+    static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b)
+    {
+        float m;
+        asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(m) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+        return __float_as_uint(m);
+    }
+    static __device__ __forceinline__ unsigned fp32_bits(unsigned m) { return m & 0x7FFFFFFFu; }               // of a whole word's maximum
     template <int J> static __device__ __forceinline__ float get(const unsigned (&w)[4]) { return __uint_as_float(w[J]); }
 };
 template <> struct Piece<__nv_bfloat16> {
     static constexpr int kElems = 8;
-    static __device__ __forceinline__ unsigned mag(unsigned w) { return w & 0x7FFF7FFFu; }
     static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b)
     {
-        const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-        return *reinterpret_cast<const unsigned*>(&m);
+        unsigned m;
+        asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+        return m;
     }
-    static __device__ __forceinline__ unsigned fp32_bits(unsigned m) { return max(m << 16, m & 0xFFFF0000u); }   // of both halves
+    static __device__ __forceinline__ unsigned fp32_bits(unsigned m) { return max(m << 16 & 0x7FFFFFFFu, m & 0x7FFF0000u); }   // of both halves
     template <int J> static __device__ __forceinline__ float get(const unsigned (&w)[4])
     {
         return __uint_as_float(J & 1 ? w[J / 2] & 0xFFFF0000u : w[J / 2] << 16);
@@ -61,16 +65,16 @@ template <> struct Piece<__nv_bfloat16> {
 };
 template <> struct Piece<__half> {
     static constexpr int kElems = 8;
-    static __device__ __forceinline__ unsigned mag(unsigned w) { return w & 0x7FFF7FFFu; }
     static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b)
     {
-        const __half2 m = __hmax2_nan(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-        return *reinterpret_cast<const unsigned*>(&m);
+        unsigned m;
+        asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+        return m;
     }
     static __device__ __forceinline__ unsigned fp32_bits(unsigned m)
     {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&m));
-        return max(__float_as_uint(f.x), __float_as_uint(f.y));
+        return max(__float_as_uint(f.x) & 0x7FFFFFFFu, __float_as_uint(f.y) & 0x7FFFFFFFu);
     }
     template <int J> static __device__ __forceinline__ float get(const unsigned (&w)[4])
     {
@@ -165,7 +169,7 @@ __device__ __forceinline__ void drop_draws4(unsigned (&w)[4], unsigned d0, unsig
 // The transposed image turns through shared memory so that it leaves in 128-byte rows: column c is row c of s_turn, its
 // 8-byte pieces (8 rows of one lane) permuted by the column so that the lanes of a write spread over all banks.
 //
-// Measured, bf16 8192 x 8192: kRows 32.5 us (floor 30.7), kBoth 47.8 us (41.0), with dropout 50 and 64 us (the draws take 22 us of
+// Measured, bf16 8192 x 8192: kRows 32.5 us (floor 30.7), kBoth 47.8 us (41.0), with dropout 49 and 64 us (the draws take 22 us of
 // the multiply pipe); fp32 4096 x 4096 kSquare, both layouts, 19.0 us (15.4).  Rows that start anywhere (8191 x 4095): kRows
 // 27.8 us (15.4), kBoth 39 us (20.5).
 enum QuantMode { kRows = 0, kBoth = 1, kSquare = 2 };
@@ -298,11 +302,10 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 && !AHEAD ? 3
         unsigned top[8], col[4];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const unsigned m0 = P::mag(v[i][0]), m1 = P::mag(v[i][1]), m2 = P::mag(v[i][2]), m3 = P::mag(v[i][3]);
-            top[i] = P::larger(P::larger(m0, m1), P::larger(m2, m3));
+            top[i] = P::larger(P::larger(v[i][0], v[i][1]), P::larger(v[i][2], v[i][3]));
             if (MODE == kBoth) {
-                col[0] = i ? P::larger(col[0], m0) : m0; col[1] = i ? P::larger(col[1], m1) : m1;
-                col[2] = i ? P::larger(col[2], m2) : m2; col[3] = i ? P::larger(col[3], m3) : m3;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) col[j] = i ? P::larger(col[j], v[i][j]) : v[i][j];
             }
         }
         float inv[8];                                            // 1 / scale of this lane's rows

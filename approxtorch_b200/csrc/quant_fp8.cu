@@ -100,12 +100,22 @@ __device__ __forceinline__ uint4 from_next_lane(const uint4& v)
                       __shfl_down_sync(0xFFFFFFFFu, v.w, 1));
 }
 
-// `left` elements from p on (zeros beyond), wherever p lies; WHOLE: there are enough.  Element by element: 16-byte loads of the
-// aligned words around them, shifted into place, took 52.6 us where these take 39.0 (8191 x 4095 bf16, both layouts; fp32 of
-// 4095 x 4095: 35 and 23 us).
+// `left` elements from p on (zeros beyond), wherever p lies; WHOLE: there are enough.  Whole pieces of 2-byte types come as the
+// words that hold them (the first may begin, the last end, with an element that is not theirs), shifted into place: 8191 x 4095
+// bf16, rows 21.9 us, both layouts 31.8 us, where element by element took 28.1 and 39.1, aligned 16-byte words with any shift
+// 52.6 (both), 8-byte words 20.8 and 30.9 but with draws 40.3 instead of 39.4 (rows).
 template <class T, bool WHOLE>
 __device__ __forceinline__ void load_piece(const T* p, long long left, unsigned (&w)[4])
 {
+    if constexpr (WHOLE && sizeof(T) == 2) {
+        const unsigned odd = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)) & 2u;
+        const unsigned* const q = reinterpret_cast<const unsigned*>(reinterpret_cast<uintptr_t>(p) - odd);
+        unsigned v[5] = {q[0], q[1], q[2], q[3], 0u};        // each holds an element of the piece
+        if (odd) v[4] = q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(v[i], v[i + 1], 8u * odd);
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = 0;
 #pragma unroll
@@ -171,7 +181,7 @@ __device__ __forceinline__ void drop_draws4(unsigned (&w)[4], unsigned d0, unsig
 //
 // Measured, bf16 8192 x 8192: kRows 32.5 us (floor 30.7), kBoth 47.8 us (41.0), with dropout 49 and 64 us (the draws take 22 us of
 // the multiply pipe); fp32 4096 x 4096 kSquare, both layouts, 19.0 us (15.4).  Rows that start anywhere (8191 x 4095): kRows
-// 27.8 us (15.4), kBoth 39 us (20.5).
+// 21.9 us (15.4), kBoth 31.8 us (20.5).
 enum QuantMode { kRows = 0, kBoth = 1, kSquare = 2 };
 template <class T> constexpr int kQuantThreads = 16 * 128 / Piece<T>::kElems;      // 256, fp32: 512
 

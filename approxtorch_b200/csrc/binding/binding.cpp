@@ -273,7 +273,7 @@ void product(const Held& a, int a_f8, const Held& b, int b_f8, const float* bias
     if (M == 0 || N == 0) return;
     check_status(atb_fp8_gemm(a.q, a_f8, a.ldq, a.s, a.lds, a.block_rows, b.q, b_f8, b.ldq, b.s, b.lds, b.block_rows, bias,
                               static_cast<float>(alpha), y.mutable_data_ptr(), float_code(y.scalar_type()), N, static_cast<int>(M),
-                              static_cast<int>(N), static_cast<int>(K), K ? threshold : 0, K ? state : nullptr, stream),
+                              static_cast<int>(N), static_cast<int>(K), threshold, state, stream),
                  "atb_fp8_gemm");
 }
 

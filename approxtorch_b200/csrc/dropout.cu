@@ -106,7 +106,8 @@ extern "C" int atb_dropout(const void* x, void* y, int dtype, long long numel, i
     ATB_REQUIRE(threshold >= 0 && threshold <= 65536, "threshold must lie in [0, 65536]");
     if (numel == 0) return ATB_OK;
     ATB_REQUIRE(x && y && rng, "null pointer");
-    ATB_REQUIRE(aligned_to(rng, 8), "rng must be 8-byte aligned");
+    ATB_REQUIRE(aligned_to(rng, 8) && aligned_to(x, dtype == ATB_F32 ? 4 : 2) && aligned_to(y, dtype == ATB_F32 ? 4 : 2),
+                "rng must be 8-byte aligned, x and y aligned to their elements");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const DropState d{static_cast<const unsigned long long*>(rng), static_cast<unsigned>(threshold)};
     const float factor = threshold == 65536 ? 0.0f : static_cast<float>(65536.0 / (65536 - threshold));

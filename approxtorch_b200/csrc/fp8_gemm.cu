@@ -1042,8 +1042,9 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     ATB_REQUIRE(y != nullptr && ldy >= N, "null y, or its row pitch below N");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int size = y_dtype == ATB_F32 ? 4 : 2;
+    ATB_REQUIRE(aligned_to(y, size) && aligned_to(bias, 4), "y and bias must be aligned to their elements");
     if (K == 0) {
-        ATB_REQUIRE(drop_threshold == 0, "dropout needs a product");
+        ATB_REQUIRE(drop_threshold == 0 || bias == nullptr, "dropout needs a product");
         if (y_dtype == ATB_F32) return launch_bias<float>(y, ldy, bias, M, N, s);
         if (y_dtype == ATB_BF16) return launch_bias<__nv_bfloat16>(y, ldy, bias, M, N, s);
         return launch_bias<__half>(y, ldy, bias, M, N, s);
@@ -1054,7 +1055,6 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     const int kblocks = (K + 127) / 128;
     ATB_REQUIRE(aligned_to(sa, 4) && aligned_to(sb, 4) && ldsa >= kblocks && ldsb >= kblocks && ldsa % 4 == 0 && ldsb % 4 == 0,
                 "scale rows must start on 4-byte boundaries");
-    ATB_REQUIRE(bias == nullptr || aligned_to(bias, 4), "bias must be 4-byte aligned");
 
     Fp8Params p{};
     p.sa = sa; p.sb = sb; p.ldsa = ldsa; p.ldsb = ldsb;

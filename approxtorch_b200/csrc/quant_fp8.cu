@@ -512,6 +512,7 @@ extern "C" int atb_fp8_quantize(const void* x, int x_dtype, long long R, long lo
     ATB_REQUIRE(drop_threshold >= 0 && drop_threshold <= 65536, "threshold must lie in [0, 65536]");
     if (R == 0 || C == 0) return ATB_OK;
     ATB_REQUIRE(x && q && s, "null pointer");
+    ATB_REQUIRE(aligned_to(x, x_dtype == ATB_F32 ? 4 : 2), "x must be aligned to its elements");
     ATB_REQUIRE((qt == nullptr) == (st == nullptr), "the transposed image and its scales come together");
     ATB_REQUIRE(ldx >= C || R == 1, "row pitch of x below its width");
     const long long nb = (C + 127) / 128, nbt = (R + 127) / 128;
@@ -535,7 +536,7 @@ extern "C" int atb_sum_rows(const float* p, int rows, long long C, float* out, v
 {
     ATB_REQUIRE(rows >= 0 && C >= 0, "negative dimension");
     if (C == 0) return ATB_OK;
-    ATB_REQUIRE(out && (p || rows == 0), "null pointer");
+    ATB_REQUIRE(out && (p || rows == 0) && aligned_to(p, 4) && aligned_to(out, 4), "p and out must be 4-byte aligned pointers");
     ATB_REQUIRE((C + 255) / 256 < (1ll << 31), "too many columns");
     launch_after(sum_rows_kernel, dim3(static_cast<unsigned>((C + 255) / 256)), dim3(256), 0, static_cast<cudaStream_t>(stream), 0, p, rows, C, out);
     return check_launch("sum_rows_kernel");

@@ -84,6 +84,18 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.atb_dropout_advance(None, p, None) == 1 and lib.atb_dropout_advance(p, p + 4, None) == 1
 
 
+def test_c_entries_refuse_misaligned_elements():
+    lib, p = _C.lib, 1 << 20
+    quant = lambda x, dt: lib.atb_fp8_quantize(x, dt, 4, 200, 200, 5, 1, p, 208, p, 2, None, 0, None, 0, None, 0, None, None)   # noqa: E731
+    gemm = lambda y, yd, K=200, bias=None, t=0: lib.atb_fp8_gemm(p, 5, 208, p, 4, 1, p, 5, 208, p, 4, 128, bias, 1.0, y, yd, 64, 4, 64, K, t, p, None)   # noqa: E731
+    drop = lambda x, y, dt: lib.atb_dropout(x, y, dt, 4, 9, p, None)         # noqa: E731
+    for code, size in ((0, 4), (3, 2), (4, 2)):
+        assert quant(p + size // 2, code) == 1 and gemm(p + size // 2, code) == 1
+        assert drop(p + size // 2, p, code) == 1 and drop(p, p + size // 2, code) == 1
+    assert gemm(p, 0, 0, p + 2) == 1 and gemm(p, 0, 0, p, 9) == 1            # without a reduction too; a masked bias alone is refused
+    assert lib.atb_sum_rows(p + 2, 2, 4, p, None) == 1 and lib.atb_sum_rows(p, 2, 4, p + 2, None) == 1
+
+
 def test_layer_surface():
     layer = at.nn.Linear_fp8(12, 5, dropout=0.25, seed=3)
     assert set(layer.state_dict()) == {"weight", "bias", "rng"} and layer.rng.tolist() == [3, 0]

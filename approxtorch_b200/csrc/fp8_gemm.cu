@@ -257,21 +257,21 @@ __device__ __forceinline__ T f8_get(uint32_t addr)
     }
     return r;
 }
-// zeros where 32 consecutive elements are dropped.  Out of line: rare, and long enough to push the loop out of the
-// instruction cache.
-__device__ __noinline__ unsigned f8_keep8(const unsigned long long* rng, unsigned threshold, unsigned long long group)
+// bit j set: element + j is kept (j < 32).  Out of line: long enough to push the loop out of the instruction cache, and not
+// every product has a mask.  The four (five) draws are independent of one another, so that they fill each other's latency.
+__device__ __noinline__ unsigned f8_keep32(PhiloxKey key, unsigned threshold, unsigned long long element)
 {
-    return philox_keep8(PhiloxKey(rng), group, threshold);
-}
-__device__ __forceinline__ void f8_mask32(const DropState& d, unsigned long long element, float (&f)[32])
-{
+    const unsigned long long group = element >> 3;
     const unsigned shift = static_cast<unsigned>(element & 7u);
-    unsigned long long keep = 0;                             // of the four or five groups that the elements lie in
-    for (int g = 0; g < (shift ? 5 : 4); ++g)
-        keep |= static_cast<unsigned long long>(f8_keep8(d.rng, d.threshold, (element >> 3) + g)) << (8 * g);
-    const unsigned m = static_cast<unsigned>(keep >> shift);
+    unsigned keep[4];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) f[j] = (m >> j) & 1u ? f[j] : 0.0f;
+    for (int g = 0; g < 4; ++g) keep[g] = philox_keep8(key, group + g, threshold);
+    const unsigned m = keep[0] | keep[1] << 8 | keep[2] << 16 | keep[3] << 24;
+    return shift ? __funnelshift_r(m, philox_keep8(key, group + 4, threshold), shift) : m;
+}
+__device__ __noinline__ unsigned f8_keep8(PhiloxKey key, unsigned threshold, unsigned long long group)
+{
+    return philox_keep8(key, group, threshold);
 }
 
 __device__ __forceinline__ uint32_t f8_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
@@ -532,6 +532,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         const uint32_t stage = stage0 + (warp - kF8EpiWarp) * 32 * kPitch;
         const uint32_t lanes = static_cast<uint32_t>(row0) << 16;
         T* const y = static_cast<T*>(p.y);
+        PhiloxKey key;
+        if (p.drop.rng != nullptr) key = PhiloxKey(p.drop.rng);
         // the bias of column n + lane
         auto bias_of = [&](int n) { return p.bias != nullptr ? __uint_as_float(read4(p.bias + min(n + lane, p.N - 1))) : 0.0f; };
         // 32 x 32 results: f holds this lane's row, columns n ..., bias is bias_of(n), asked for ahead
@@ -543,7 +545,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
                 for (int j = 0; j < 32; ++j) f[j] += __shfl_sync(0xFFFFFFFFu, bias, j);
             }
-            if (p.drop.rng != nullptr) f8_mask32(p.drop, static_cast<unsigned long long>(m0 + lane) * p.N + n, f);
+            if (p.drop.rng != nullptr) {
+                const unsigned m = f8_keep32(key, p.drop.threshold, static_cast<unsigned long long>(m0 + lane) * p.N + n);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) f[j] = (m >> j) & 1u ? f[j] : 0.0f;
+            }
             constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer;           // of a 32-element row
             __syncwarp();                                                       // the last chunk's readers are through
 #pragma unroll
@@ -797,11 +803,13 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
     }
     const int cols = min(p.tile_c, p.M - m0);
     T* const y = static_cast<T*>(p.y) + static_cast<long long>(m0) * p.ldy;
+    PhiloxKey key;
+    if (p.drop.rng != nullptr) key = PhiloxKey(p.drop.rng);
     auto store = [&](int n, int c, float v, float bias) {
         float f = p.alpha * v + bias;
         if (p.drop.rng != nullptr) {
             const unsigned long long e = static_cast<unsigned long long>(m0 + c) * p.N + n;
-            if (!((f8_keep8(p.drop.rng, p.drop.threshold, e >> 3) >> (e & 7u)) & 1u)) f = 0.0f;
+            if (!((f8_keep8(key, p.drop.threshold, e >> 3) >> (e & 7u)) & 1u)) f = 0.0f;
         }
         y[c * p.ldy + n] = f8_out<T>(f);
     };

@@ -18,6 +18,7 @@ struct DropState {                // what a kernel needs to know of a dropout ca
 
 struct PhiloxKey {
     uint32_t k0, k1, o0, o1;
+    PhiloxKey() = default;
     __device__ __forceinline__ explicit PhiloxKey(const unsigned long long* rng)
     {
         const unsigned long long seed = rng[0], off = rng[1];

@@ -43,12 +43,13 @@ namespace atb {
 
 __device__ int g_fp8_status = 0;                      // 1: a block gave up waiting
 
-constexpr int kF8Threads = 256, kF8EpiWarp = 4, kF8EpiWarps = 4;
-constexpr int kF8SumThreads = 384, kF8SumEpiWarps = 8, kF8SumTileN = 192, kF8SumQuads = 2;   // with fp32 sums of partial products
+constexpr int kF8Threads = 384, kF8EpiWarp = 4, kF8EpiWarps = 8, kF8SplitThreads = 256;
+constexpr int kF8SumTileN = 192, kF8SumQuads = 2;            // with fp32 sums of partial products
 constexpr int kF8TileM = 128, kF8MaxTileN = 256;          // of one block; a pair's tile has twice the rows
 constexpr int kF8SfSlots = 8, kF8SfSlotBytes = 3 * 512;   // a run of quads for each gathering warp; 128 rows of A, up to 256 of B
 constexpr int kF8SfCol = 488, kF8SfCols = 12;             // tensor-memory columns of the two scale buffers
 constexpr int kF8Smem = 226 * 1024, kF8MaxStages = 8;
+constexpr int kF8SplitSmem = kF8Smem - kF8TileM * 16;    // fp8_split_kernel: its mask besides
 constexpr int kF8SumsFrom = 16;                          // slices beyond which an fp32 result is added up from partial sums
 constexpr int kF8MaxQuads = 40;                           // of one block of fp8_split_kernel
 constexpr int kF8Group = 8;                               // row tiles that are walked together (their operands meet in L2)
@@ -269,10 +270,6 @@ __device__ __noinline__ unsigned f8_keep32(PhiloxKey key, unsigned threshold, un
     const unsigned m = keep[0] | keep[1] << 8 | keep[2] << 16 | keep[3] << 24;
     return shift ? __funnelshift_r(m, philox_keep8(key, group + 4, threshold), shift) : m;
 }
-__device__ __noinline__ unsigned f8_keep8(PhiloxKey key, unsigned threshold, unsigned long long group)
-{
-    return philox_keep8(key, group, threshold);
-}
 
 __device__ __forceinline__ uint32_t f8_word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
@@ -289,7 +286,7 @@ __device__ __forceinline__ void f8_tile(int t, int mt, int nt, int& tm, int& tn)
 // long reduction to fp32 the accumulators are read every 1024 steps (kF8SumQuads quads) and added up, rounded, in the
 // registers of eight epilogue warps, the two accumulators taking turns.
 template <class T, int CG, bool SUMS>
-__global__ void __launch_bounds__(SUMS ? kF8SumThreads : kF8Threads, 1)
+__global__ void __launch_bounds__(kF8Threads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp8Params p)
 {
     extern __shared__ uint8_t smem_raw[];
@@ -354,8 +351,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (lane == 0) s_abort = 0;
         for (int i = lane; i < kF8MaxStages; i += 32) { f8_bar_init(full0 + 8 * i, 1); f8_bar_init(empty0 + 8 * i, 1); }
         if (lane < kF8SfSlots) { f8_bar_init(sff0 + 8 * lane, CG); f8_bar_init(sfe0 + 8 * lane, 1); }
-        if (lane < 2) { f8_bar_init(accf0 + 8 * lane, 1); f8_bar_init(acce0 + 8 * lane, (SUMS ? kF8SumEpiWarps : kF8EpiWarps) * CG); }
-        if (lane == 0) f8_bar_init(accp, kF8EpiWarps * CG);
+        if (lane < 2) { f8_bar_init(accf0 + 8 * lane, 1); f8_bar_init(acce0 + 8 * lane, kF8EpiWarps * CG); }
+        if (lane == 0) f8_bar_init(accp, kF8EpiWarps / 2 * CG);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     } else if (warp == 1) {
         if (f8_elect()) {
@@ -618,14 +615,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 const int chunks = p.tile_n / 32;
                 const uint32_t buf = item & 1u;
                 auto column = [&](int i) { return 32 * (overlap && buf == 0 ? (i == 0 ? chunks - 1 : i - 1) : i); };
-                float bias_next = bias_of(n0 + column(0));
+                const int half = (warp - kF8EpiWarp) >> 2;   // the chunks' turn: four warps the even ones, four the odd ones
+                float bias_next = bias_of(n0 + column(half));
                 if (!(ok = f8_wait(accf0 + 8 * buf, (item >> 1) & 1u, abort_flag, patience))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t src = tmem + buf * d_step + lanes;
-                for (int i = 0; i < chunks; ++i) {
+                for (int i = half; i < chunks; i += 2) {
                     const int c = column(i), n = n0 + c;
                     const float bias = bias_next;
-                    if (i + 1 < chunks) bias_next = bias_of(n0 + column(i + 1));
+                    if (i + 2 < chunks) bias_next = bias_of(n0 + column(i + 2));
                     const bool live = n < p.N && rows > 0;   // the same for the whole warp
                     uint32_t v[32];
                     if (live) f8_tmem_ld32(v, src + c);
@@ -695,13 +693,14 @@ __device__ __forceinline__ uint32_t f8_cluster_rank()
 }
 
 template <class T>
-__global__ void __launch_bounds__(kF8Threads)
+__global__ void __launch_bounds__(kF8SplitThreads)
 fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a, const Fp8SplitParams p)
 {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ __align__(8) uint64_t s_full[kF8MaxStages], s_empty[kF8MaxStages], s_sf[kF8MaxQuads], s_acc;
+    __shared__ unsigned s_keep[kF8TileM][4];                 // [row of A]: a bit for each row of B
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
     const uint32_t rank = f8_cluster_rank();
@@ -803,17 +802,20 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
     }
     const int cols = min(p.tile_c, p.M - m0);
     T* const y = static_cast<T*>(p.y) + static_cast<long long>(m0) * p.ldy;
-    PhiloxKey key;
-    if (p.drop.rng != nullptr) key = PhiloxKey(p.drop.rng);
     auto store = [&](int n, int c, float v, float bias) {
         float f = p.alpha * v + bias;
-        if (p.drop.rng != nullptr) {
-            const unsigned long long e = static_cast<unsigned long long>(m0 + c) * p.N + n;
-            if (!((f8_keep8(key, p.drop.threshold, e >> 3) >> (e & 7u)) & 1u)) f = 0.0f;
-        }
+        if (p.drop.rng != nullptr && !((s_keep[c][(n - n0) >> 5] >> ((n - n0) & 31)) & 1u)) f = 0.0f;
         y[c * p.ldy + n] = f8_out<T>(f);
     };
     if (warp >= kF8EpiWarp) {
+        if (p.drop.rng != nullptr) {                         // the mask of this block's share, while the product is made
+            const PhiloxKey key(p.drop.rng);
+            for (int i = tid - 32 * kF8EpiWarp; i < 4 * ((cols - static_cast<int>(rank) + p.splits - 1) / p.splits); i += 128) {
+                const int c = static_cast<int>(rank) + p.splits * (i >> 2), n = n0 + 32 * (i & 3);
+                if (n < p.N) s_keep[c][i & 3] = f8_keep32(key, p.drop.threshold, static_cast<unsigned long long>(m0 + c) * p.N + n);
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
         if (f8_wait(acc0, 0, abort_flag)) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int row = (warp & 3) * 32 + lane, n = n0 + row;
@@ -907,12 +909,12 @@ static int operand_map(CUtensorMap* map, const void* base, long long R, long lon
 
 // the kernels' shared memory is above the default limit: allowed once per device
 template <class K>
-static cudaError_t allow_smem(K kernel, bool (&done)[64])
+static cudaError_t allow_smem(K kernel, int bytes, bool (&done)[64])
 {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev])) return e;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kF8Smem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
     return e;
 }
@@ -927,8 +929,8 @@ static int fp8_cluster_blocks(int size)
     if (known[dev][size] == 0) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(size);
-        cfg.blockDim = dim3(kF8Threads);
-        cfg.dynamicSmemBytes = kF8Smem;
+        cfg.blockDim = dim3(kF8SplitThreads);
+        cfg.dynamicSmemBytes = kF8SplitSmem;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = size;
@@ -936,7 +938,7 @@ static int fp8_cluster_blocks(int size)
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         int n = 0;
-        if (allow_smem(fp8_split_kernel<float>, done) != cudaSuccess ||
+        if (allow_smem(fp8_split_kernel<float>, kF8SplitSmem, done) != cudaSuccess ||
             cudaOccupancyMaxActiveClusters(&n, fp8_split_kernel<float>, &cfg) != cudaSuccess || n <= 0) {
             cudaGetLastError();                              // an estimate does; the launch reports what is wrong
             n = sm_count() / size;
@@ -998,10 +1000,10 @@ template <class T, int CG, bool SUMS>
 static int launch_fp8(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Params& p, cudaStream_t s)
 {
     static bool done[64];
-    cudaError_t e = allow_smem(fp8_gemm_kernel<T, CG, SUMS>, done);
+    cudaError_t e = allow_smem(fp8_gemm_kernel<T, CG, SUMS>, kF8Smem, done);
     const int tiles = p.mt * p.nt, fit = sm_count() / CG;
     if (e == cudaSuccess)
-        e = launch_after(fp8_gemm_kernel<T, CG, SUMS>, dim3(CG * (tiles < fit ? tiles : fit)), dim3(SUMS ? kF8SumThreads : kF8Threads), kF8Smem, s,
+        e = launch_after(fp8_gemm_kernel<T, CG, SUMS>, dim3(CG * (tiles < fit ? tiles : fit)), dim3(kF8Threads), kF8Smem, s,
                          CG == 2 ? 2 : 0, ma, mb, p);
     if (e != cudaSuccess) { set_error("fp8_gemm_kernel: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
     return check_launch("fp8_gemm_kernel");
@@ -1017,8 +1019,8 @@ template <class T>
 static int launch_split(const CUtensorMap& mb, const CUtensorMap& ma, const Fp8SplitParams& p, int tiles, size_t smem, cudaStream_t s)
 {
     static bool done[64];
-    cudaError_t e = allow_smem(fp8_split_kernel<T>, done);
-    if (e == cudaSuccess) e = launch_after(fp8_split_kernel<T>, dim3(tiles * p.splits), dim3(kF8Threads), smem, s, p.splits, mb, ma, p);
+    cudaError_t e = allow_smem(fp8_split_kernel<T>, kF8SplitSmem, done);
+    if (e == cudaSuccess) e = launch_after(fp8_split_kernel<T>, dim3(tiles * p.splits), dim3(kF8SplitThreads), smem, s, p.splits, mb, ma, p);
     if (e != cudaSuccess) { set_error("fp8_split_kernel: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
     return check_launch("fp8_split_kernel");
 }
@@ -1081,7 +1083,7 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
         q.splits = plan.splits;
         const int kbs = (kblocks + plan.splits - 1) / plan.splits, quads = kbs / 4 + 2, stage = (kF8TileM + plan.tile) * 128;
         const int sums = plan.tile * kF8TileM * 4;           // the partial tile takes the stages' place
-        q.stages = (kF8Smem - 1024 - quads * 1024) / stage;
+        q.stages = (kF8SplitSmem - 1024 - quads * 1024) / stage;
         q.stages = q.stages < kbs ? q.stages : kbs;
         q.stages = q.stages < kF8MaxStages ? q.stages : kF8MaxStages;
         q.stages = q.stages * stage >= sums ? q.stages : (sums + stage - 1) / stage;
@@ -1095,7 +1097,7 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
         const size_t share = 456 * static_cast<size_t>(q.tmem_cols) - 1024;
         size_t smem = 1024 + static_cast<size_t>(q.stages) * stage + static_cast<size_t>(quads) * 1024;
         smem = smem < share ? share : smem;
-        smem = smem < kF8Smem ? smem : kF8Smem;              // (which leaves no room for a second block either)
+        smem = smem < kF8SplitSmem ? smem : kF8SplitSmem;    // (which leaves no room for a second block either)
         const int tiles = ((N + kF8TileM - 1) / kF8TileM) * q.ct;
         int rc = operand_map(&mb, b, N, K, ldb, kF8TileM);
         if (rc == ATB_OK) rc = operand_map(&ma, a, M, K, lda, plan.tile);
@@ -1110,7 +1112,7 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     p.nt = (N + p.tile_n - 1) / p.tile_n;
     ATB_REQUIRE(static_cast<long long>(p.mt) * p.nt < (1LL << 30), "too many tiles");
     const int stage = kF8TileM * 128 + p.tile_n / cg * 128;
-    p.stages = (kF8Smem - 1024 - kF8SfSlots * kF8SfSlotBytes - (sums ? kF8SumEpiWarps : kF8EpiWarps) * 32 * (32 * size + 16)) / stage;
+    p.stages = (kF8Smem - 1024 - kF8SfSlots * kF8SfSlotBytes - kF8EpiWarps * 32 * (32 * size + 16)) / stage;
     if (p.stages > kF8MaxStages) p.stages = kF8MaxStages;
     p.idesc = formats | (a_f8 == ATB_E5M2 ? 1u << 7 : 0u) | (b_f8 == ATB_E5M2 ? 1u << 10 : 0u) |
               (static_cast<uint32_t>(p.tile_n >> 3) << 17) | (static_cast<uint32_t>(cg) << 27);

@@ -24,19 +24,36 @@ template <> __device__ __forceinline__ __half drop_store<__half>(float v) { retu
 
 template <class T> struct alignas(16) Eight { T v[8]; };
 
-template <class T>
+// ALIGNED: 16 bytes at a time; else 2-byte types as the words that hold them (the first may begin, the last end, with an element
+// that is not theirs), shifted into place.  2^26 bf16 elements from an odd one on: 54 us (aligned 46), 201 element by element.
+template <class T, bool ALIGNED>
 __device__ __forceinline__ Eight<T> eight_load(const T* p)
 {
     Eight<T> e;
+    if constexpr (!ALIGNED) {
+        unsigned* const w = reinterpret_cast<unsigned*>(&e);
+        if constexpr (sizeof(T) == 2) {
+            const unsigned odd = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p)) & 2u;
+            const unsigned* const q = reinterpret_cast<const unsigned*>(reinterpret_cast<uintptr_t>(p) - odd);
+            unsigned v[5] = {read4(q), read4(q + 1), read4(q + 2), read4(q + 3), 0u};
+            if (odd) v[4] = read4(q + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(v[i], v[i + 1], 8u * odd);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = read4(p + i);
+        }
+        return e;
+    }
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(e) / 16); ++i) reinterpret_cast<uint4*>(&e)[i] = read16_once(p + 16 / sizeof(T) * i);
     return e;
 }
 
-// One thread takes whole groups of 8 elements (one draw each), kAhead of them at a time, requested together.  VEC: 16-byte
-// aligned tensors.  2^26 bf16 elements: 45.9 us (a copy: 42.5 us, floor 41.0 us); 2^24 fp32: 22.4 us (a copy: 22.4 us).  Measured
+// One thread takes whole groups of 8 elements (one draw each), kAhead of them at a time, requested together.  VEC: y is 16-byte
+// aligned; ALIGNED: x too.  2^26 bf16 elements: 45.9 us (a copy: 42.5 us, floor 41.0 us); 2^24 fp32: 22.4 us (a copy: 22.4 us).  Measured
 // against it, 1, 2 or 4 groups ahead and 2, 3 or 4 blocks to an SM: 47 to 74 us.
-template <class T, bool VEC>
+template <class T, bool VEC, bool ALIGNED>
 __global__ void __launch_bounds__(256, 4) dropout_kernel(const T* x, T* y, long long numel, DropState d, float factor)
 {
     constexpr int kAhead = sizeof(T) == 2 ? 4 : 1;
@@ -61,15 +78,15 @@ __global__ void __launch_bounds__(256, 4) dropout_kernel(const T* x, T* y, long 
     for (; g + (kAhead - 1) * stride < whole; g += kAhead * stride) {
         Eight<T> e[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) e[i] = eight_load(x + ((g + i * stride) << 3));
+        for (int i = 0; i < kAhead; ++i) e[i] = eight_load<T, ALIGNED>(x + ((g + i * stride) << 3));
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) finish(g + i * stride, e[i]);
     }
     for (; g < whole; g += stride) {
-        Eight<T> e = eight_load(x + (g << 3));
+        Eight<T> e = eight_load<T, ALIGNED>(x + (g << 3));
         finish(g, e);
     }
-    for (; g < groups; g += stride) {                        // unaligned tensors, and what a last group is short of 8
+    for (; g < groups; g += stride) {                        // an unaligned result, and what a last group is short of 8
         const unsigned m = philox_keep8(key, g, d.threshold);
         for (int j = 0; j < 8 && (g << 3) + j < numel; ++j)
             y[(g << 3) + j] = drop_store<T>((m >> j) & 1u ? drop_load(x[(g << 3) + j]) * factor : 0.0f);
@@ -90,10 +107,13 @@ __global__ void drop_advance_kernel(unsigned long long* state, unsigned long lon
 template <class T>
 static void launch_dropout(const void* x, void* y, long long numel, const DropState& d, float factor, cudaStream_t s)
 {
-    const bool vec = aligned_to(x, 16) && aligned_to(y, 16);
     const int grid = grid_for((numel + 7) / 8, 256, 8 * sm_count());
-    if (vec) launch_after(dropout_kernel<T, true>, dim3(grid), dim3(256), 0, s, 0, static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
-    else launch_after(dropout_kernel<T, false>, dim3(grid), dim3(256), 0, s, 0, static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
+    const auto go = [&](void (*kernel)(const T*, T*, long long, DropState, float)) {
+        launch_after(kernel, dim3(grid), dim3(256), 0, s, 0, static_cast<const T*>(x), static_cast<T*>(y), numel, d, factor);
+    };
+    if (!aligned_to(y, 16)) go(dropout_kernel<T, false, false>);
+    else if (aligned_to(x, 16)) go(dropout_kernel<T, true, true>);
+    else go(dropout_kernel<T, true, false>);
 }
 
 }  // namespace atb

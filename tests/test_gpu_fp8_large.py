@@ -224,6 +224,20 @@ def test_c_quantiser_writes_its_rows_and_nothing_else(dev):
             assert (tail == 0xEE).all()
 
 
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_dropout_of_inputs_that_start_anywhere(dev, dt):
+    """The same elements give the same result wherever they lie, in the loop over many groups, a last group and a short one."""
+    from approxtorch_b200.backend import ops
+    state = torch.tensor([4, 9], dtype=torch.int64, device=dev)
+    for n in (2 ** 24 + 5, 4099, 9, 8, 7, 1):
+        x = torch.randn(n, device=dev).to(dt)
+        want = ops.dropout(x, 0.3, state)
+        for first in (1, 2, 3, 5):
+            buf = torch.full((n + 8,), float("nan"), device=dev, dtype=dt)
+            buf[first:first + n] = x
+            assert torch.equal(ops.dropout(buf[first:first + n], 0.3, state), want)
+
+
 @pytest.mark.parametrize("fmt", [torch.float8_e4m3fn, torch.float8_e5m2], ids=["e4m3", "e5m2"])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("R,C,pitch", [(2500, 2056, 2056), (128, 128 * 301, 128 * 301), (128 * 331 - 7, 120, 136), (9000, 1000, 1024)])

@@ -16,8 +16,9 @@
 //   warps 2-3   gather the scale bytes, 16 slices at a time (one load per row), and hand them over four slices (a quad) at a
 //               time in the order in which tcgen05.cp wants them: 32 rows of 16 bytes, word j of row i = operand row
 //               i + 32 j (warp 3 also owns the tensor-memory allocation);
-//   warps 4-7   read finished accumulators, scale, add the bias and store, 32 x 32 elements at a time through shared
-//               memory so that a row's bytes leave together.
+//   warps 4-11  read finished accumulators, scale, add the bias, mask and store, 32 x 32 elements at a time through shared
+//               memory so that a row's bytes leave together (four warps instead of eight: 4096 x 8192 x 128 24.0 instead of
+//               19.5 us, 4096 x 8192 x 1024 with a mask 58 instead of 46 us).
 // Two accumulators let the epilogue of a tile run under the MMAs of the next; where two of 256 columns and the scales do
 // not fit the 512 columns of tensor memory, they share 24 columns, which the epilogue reads first.  Why pairs: each block of
 // a pair holds its own 128 rows of A and half the rows of B and the tensor core reads both halves, so a slice of a 256 x 256
@@ -284,7 +285,7 @@ __device__ __forceinline__ void f8_tile(int t, int mt, int nt, int& tm, int& tn)
 // SUMS: the tensor core's accumulator cuts what does not fit its 24 bits instead of rounding it, which leaves a bias towards
 // zero that grows with the number of additions (2e-6 of a result over 8192 steps).  A bf16 or fp16 result hides it; for a
 // long reduction to fp32 the accumulators are read every 1024 steps (kF8SumQuads quads) and added up, rounded, in the
-// registers of eight epilogue warps, the two accumulators taking turns.
+// registers of the epilogue warps, the two accumulators taking turns.
 template <class T, int CG, bool SUMS>
 __global__ void __launch_bounds__(kF8Threads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp8Params p)
@@ -952,10 +953,10 @@ static int fp8_cluster_blocks(int size)
 // measured on B200 (8-bit operands of random numbers): a slice (128 steps) of a tile costs 0.06 + 0.0013 per column to a
 // pair of blocks (the MMAs; 0.22 at least, the issue), 0.165 + 0.00106 per column to a single block; a tile besides, 0.4 +
 // 0.003 per column; a launch with a first load, 3.5 (pairs: 4.6).  The split kernel: 0.14 + 0.0016 per row of A for a slice,
-// 0.8 + 0.025 per row of A and 0.06 per block of the cluster for a tile, 2.0 for the launch, 2.3 with clusters (blocks that
-// share an SM take nearly as long as one after the other, so they count as further rounds).  Over 200 products drawn at
+// 0.8 + 0.025 per row of A and 0.06 per block of the cluster for a tile, 2.0 for the launch, 2.8 with clusters (blocks that
+// share an SM take nearly as long as one after the other, so they count as further rounds).  Over 600 products drawn at
 // random (rows 1 to 4000, columns and reduction 64 to 8192, bf16 and fp32 results) the choice took 1.02 of the time of the
-// best choice on average and 1.24 at worst.
+// best choice on average and 1.37 at worst.
 struct Fp8Plan {
     int cg, tile;            // fp8_gemm_kernel: blocks to a tile, columns
     int splits;              // fp8_split_kernel where not 0: blocks to a tile; tile = rows of A
@@ -989,7 +990,7 @@ static Fp8Plan fp8_plan(int M, int N, int kblocks, bool fp32)
             const int slices = (kblocks + splits - 1) / splits;
             if (slices / 4 + 2 > kF8MaxQuads || (fp32 && slices > kF8SumsFrom)) continue;
             const double waves = ceil(mt * nt * splits / fp8_cluster_blocks(splits));
-            const double t = waves * (slices * (0.14 + 0.0016 * tile) + 0.8 + 0.025 * tile + 0.06 * splits) + (splits > 1 ? 2.3 : 2.0);
+            const double t = waves * (slices * (0.14 + 0.0016 * tile) + 0.8 + 0.025 * tile + 0.06 * splits) + (splits > 1 ? 2.8 : 2.0);
             if (t < least) { least = t; best = Fp8Plan{1, tile, splits}; }
         }
     }

@@ -374,8 +374,9 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
             uint8_t* at = kept.mutable_data_ptr<uint8_t>();
             if (laid_w) at = xt.place(at);
             if (laid_x) wt.place(at);
-            scratch = fresh({gq.bytes() + (need_w ? gt.bytes() : 0) + sum_bytes}, at::kByte, go);
-            at = gq.place(scratch.mutable_data_ptr<uint8_t>());
+            scratch = fresh({(need_x ? gq.bytes() : 0) + (need_w ? gt.bytes() : 0) + sum_bytes}, at::kByte, go);
+            at = scratch.mutable_data_ptr<uint8_t>();
+            if (need_x) at = gq.place(at);
             if (need_w) at = gt.place(at);
             float* sums = sum_bytes ? reinterpret_cast<float*>(at) : nullptr;
             if (sums) {

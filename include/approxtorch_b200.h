@@ -301,7 +301,8 @@ int atb_lut_dwconv_bwd(const float* go, const void* x, int dtype, const uint8_t*
  * gets byte 255 (NaN) and NaN everywhere.
  *   q  [R, C], row pitch ldq (a multiple of 16, base 16-byte aligned; the pitch's padding may be written)
  *   s  [R or ceil(R/128), ceil(C/128)], row pitch lds
- *   qt [C, R], st [C or ceil(C/128), ceil(R/128)]: x transposed, quantised in blocks along R; both or neither
+ *   qt [C, R], st [C or ceil(C/128), ceil(R/128)]: x transposed, quantised in blocks along R
+ *   an image is left out where it and its scales are NULL (q only with block_rows 1)
  *   column_sums [ceil(R/128), C] or NULL: the sums of x's columns over each 128 rows, fp32 (with qt, block_rows 1, no
  *     dropout); atb_sum_rows adds them up
  * drop_threshold > 0: x is dropped out first, as atb_dropout does on the contiguous [R, C] tensor, but without its factor

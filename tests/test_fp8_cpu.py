@@ -93,6 +93,9 @@ def test_c_entries_refuse_misaligned_elements():
         assert quant(p + size // 2, code) == 1 and gemm(p + size // 2, code) == 1
         assert drop(p + size // 2, p, code) == 1 and drop(p, p + size // 2, code) == 1
     assert gemm(p, 0, 0, p + 2) == 1 and gemm(p, 0, 0, p, 9) == 1            # without a reduction too; a masked bias alone is refused
+    for q, s, qt, st in ((None, p, p, p), (p, None, p, p), (None, None, None, None), (None, None, p, None), (None, None, None, p)):
+        assert lib.atb_fp8_quantize(p, 0, 4, 200, 200, 5, 1, q, 208, s, 2, qt, 16, st, 1, None, 0, None, None) == 1
+    assert lib.atb_fp8_quantize(p, 0, 4, 200, 200, 5, 128, None, 0, None, 0, p, 16, p, 1, None, 0, None, None) == 1
     assert lib.atb_sum_rows(p + 2, 2, 4, p, None) == 1 and lib.atb_sum_rows(p, 2, 4, p + 2, None) == 1
 
 

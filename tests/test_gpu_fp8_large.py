@@ -271,6 +271,31 @@ def test_both_layouts_of_more_tiles_than_resident_blocks(dev, R, C, pitch, dt, f
         assert torch.equal(buf.view(rows, up(width))[:, :width], w.view(torch.uint8))
 
 
+@pytest.mark.parametrize("R,C,dt", [(5, 130, torch.float32), (200, 72, torch.bfloat16), (129, 257, torch.float16), (2600, 2048, torch.bfloat16)])
+def test_c_quantiser_makes_the_transposed_image_alone(dev, R, C, dt):
+    from approxtorch_b200.backend import _C, ops
+    x = torch.randn(R, C, device=dev).to(dt)
+    want = ops.fp8_quantize_both(x)[2:]
+    ldqt, ldst = -(-R // 16) * 16, -(-R // 128)
+    qt = torch.empty(C, ldqt, dtype=torch.uint8, device=dev)
+    st = torch.empty(C, ldst, dtype=torch.uint8, device=dev)
+    code = {torch.float32: 0, torch.bfloat16: 3, torch.float16: 4}[dt]
+    assert _C.lib.atb_fp8_quantize(x.data_ptr(), code, R, C, C, 5, 1, None, 0, None, 0, qt.data_ptr(), ldqt, st.data_ptr(), ldst, None, 0,
+                                   None, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    assert torch.equal(qt[:, :R], want[0].view(torch.uint8)) and torch.equal(st, want[1].view(torch.uint8))
+
+
+def test_linear_fp8_gradients_without_an_input_gradient(dev):
+    """A first layer: the weight and bias gradients are those of a layer whose input wants one too."""
+    import approxtorch_b200 as at
+    for M, N, K, dt in ((140, 50, 96, torch.float32), (2560, 2048, 256, torch.bfloat16)):
+        x, go = torch.randn(M, K, device=dev).to(dt), torch.randn(M, N, device=dev).to(dt)
+        w, b = torch.randn(N, K, device=dev, requires_grad=True), torch.randn(N, device=dev, requires_grad=True)
+        got = torch.autograd.grad(at.nn.gemm_fp8.linear_fp8(x, w, b), (w, b), go)
+        want = torch.autograd.grad(at.nn.gemm_fp8.linear_fp8(x.clone().requires_grad_(True), w, b), (w, b), go)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_two_streams_at_once(dev):
     """Products, quantisers and dropout of two streams in flight together give what they give alone."""
     from approxtorch_b200.backend import ops

@@ -838,12 +838,16 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
     }
-    __syncwarp();
-    if (p.splits == 1) __syncthreads(); else f8_cluster_sync();
+    // Tensor memory goes back before this block waits for the others of its cluster: tcgen05.alloc waits without a limit, so a
+    // block that kept its columns while it waited for one that still waits for columns could close a circle through a tensor-core
+    // kernel of another stream that shares their SMs.
+    __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
     if (tid == 0 && s_abort) g_fp8_status = 1;
     if (p.splits == 1) return;
+    __syncwarp();
+    f8_cluster_sync();                                       // the parts are in place
     // ---- every block finishes its share of the columns, four at a time so that the reads overlap
     const int row = tid & (kF8TileM - 1), n = n0 + row;
     if (n < p.N) {
@@ -1092,9 +1096,8 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
         while (q.tmem_cols < static_cast<uint32_t>(plan.tile + 8 * quads)) q.tmem_cols *= 2;
         q.idesc = formats | (b_f8 == ATB_E5M2 ? 1u << 7 : 0u) | (a_f8 == ATB_E5M2 ? 1u << 10 : 0u) | (static_cast<uint32_t>(plan.tile >> 3) << 17) | (1u << 27);
         q.drop = drop;
-        // At least the tensor memory's share of an SM's 228 KB: blocks that fit an SM together then find their columns too.  (A
-        // block of one cluster that waited for columns held by another cluster's block, which waits for its own cluster on
-        // an SM where the first cluster holds the columns, would wait for ever.)
+        // At least the tensor memory's share of an SM's 228 KB: blocks that fit an SM together then find their columns at once
+        // instead of waiting for a neighbour's.
         const size_t share = 456 * static_cast<size_t>(q.tmem_cols) - 1024;
         size_t smem = 1024 + static_cast<size_t>(q.stages) * stage + static_cast<size_t>(quads) * 1024;
         smem = smem < share ? share : smem;

@@ -32,6 +32,7 @@ struct QuantArgs {
     long long ldst;
     float* sums;      // [ceil(R/128), C]
     DropState drop;
+    long long wq, wqt;       // what may be written of a row of q, qt: its width up to 16 bytes
     unsigned ct, tiles;      // tiles of 128 columns; of the matrix
 };
 
@@ -384,9 +385,9 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 && !AHEAD ? 3
                 if constexpr (kElems == 8) {
                     const unsigned hi = pack4<E5>(P::template get<4>(v[i]) * inv[i], P::template get<5>(v[i]) * inv[i],
                                                   P::template get<6>(v[i]) * inv[i], P::template get<7>(v[i]) * inv[i]);
-                    if (i < rows && c < a.ldq) *reinterpret_cast<uint2*>(q + i * a.ldq) = make_uint2(lo, hi);
+                    if (i < rows && c < a.wq) *reinterpret_cast<uint2*>(q + i * a.ldq) = make_uint2(lo, hi);
                 } else {
-                    if (i < rows && c < a.ldq) *reinterpret_cast<unsigned*>(q + i * a.ldq) = lo;
+                    if (i < rows && c < a.wq) *reinterpret_cast<unsigned*>(q + i * a.ldq) = lo;
                 }
             }
         }
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kQuantThreads<T>, sizeof(T) == 2 && !AHEAD ? 3
             const int cc = (threadIdx.x >> 3) + kQuantThreads<T> / 8 * i, piece = threadIdx.x & 7, by = cc / kElems % 16;
             uint4 o = *reinterpret_cast<const uint4*>(s_turn + cc * 128 + ((piece ^ (by >> 1)) << 4));
             if (by & 1) o = make_uint4(o.z, o.w, o.x, o.y);
-            if (c0 + cc < a.C && rt + piece * 16 < a.ldqt) *reinterpret_cast<uint4*>(a.qt + (c0 + cc) * a.ldqt + rt + piece * 16) = o;
+            if (c0 + cc < a.C && rt + piece * 16 < a.wqt) *reinterpret_cast<uint4*>(a.qt + (c0 + cc) * a.ldqt + rt + piece * 16) = o;
         }
         // (what the next tile writes to shared memory is written one barrier at least after this tile's last read of it)
     } while (AHEAD && (tile += gridDim.x) < a.tiles);
@@ -525,7 +526,8 @@ extern "C" int atb_fp8_quantize(const void* x, int x_dtype, long long R, long lo
                 "column sums go with both layouts, blocks of one row and no dropout");
     ATB_REQUIRE(drop_threshold == 0 || (rng != nullptr && aligned_to(rng, 8)), "dropout needs an 8-byte aligned state");
     QuantArgs a{x, R, C, ldx, static_cast<uint8_t*>(q), ldq, s, lds, static_cast<uint8_t*>(qt), ldqt, st, ldst, column_sums,
-                DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)}, 0, 0};
+                DropState{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)},
+                (C + 15) / 16 * 16, (R + 15) / 16 * 16, 0, 0};
     cudaStream_t stm = static_cast<cudaStream_t>(stream);
     const bool e5 = f8 == ATB_E5M2, square = block_rows == 128;
     if (x_dtype == ATB_F32) return e5 ? launch_quantize<float, true>(a, square, stm) : launch_quantize<float, false>(a, square, stm);

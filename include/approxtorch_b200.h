@@ -299,9 +299,9 @@ int atb_lut_dwconv_bwd(const float* go, const void* x, int dtype, const uint8_t*
  * Quantise x [R, C] (fp32 / bf16 / fp16, row pitch ldx elements): byte = the smallest in 1..254 with
  * max|x| <= F 2^(byte - 127), F = 448 or 57344; q = x / scale rounded to nearest even.  A block with a NaN or an infinity
  * gets byte 255 (NaN) and NaN everywhere.
- *   q  [R, C], row pitch ldq (a multiple of 16, base 16-byte aligned; the pitch's padding may be written)
+ *   q  [R, C], row pitch ldq (a multiple of 16, base 16-byte aligned); a row is written up to the next multiple of 16 bytes
  *   s  [R or ceil(R/128), ceil(C/128)], row pitch lds
- *   qt [C, R], st [C or ceil(C/128), ceil(R/128)]: x transposed, quantised in blocks along R
+ *   qt [C, R] (as q), st [C or ceil(C/128), ceil(R/128)]: x transposed, quantised in blocks along R
  *   an image is left out where it and its scales are NULL (q only with block_rows 1)
  *   column_sums [ceil(R/128), C] or NULL: the sums of x's columns over each 128 rows, fp32 (with qt, block_rows 1, no
  *     dropout); atb_sum_rows adds them up

@@ -39,3 +39,26 @@ def test_products_beside_other_tensor_core_kernels(dev):
         assert all(torch.equal(p, q) for p, q in zip(out, want))
     for out in got_mats:
         assert all(torch.equal(p, q) for p, q in zip(out, want_mats))
+
+
+@pytest.mark.parametrize("code,dt", [(0, torch.float32), (3, torch.bfloat16), (4, torch.float16)])
+@pytest.mark.parametrize("R,C", [(5, 130), (130, 70), (129, 257), (200, 72), (300, 1001), (2500, 2056)])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_c_quantiser_leaves_a_wider_buffer_around_its_rows(dev, R, C, block_rows, dt, code):
+    """Images in column ranges of wider buffers: a row is written up to the next multiple of 16 bytes and no further."""
+    import ctypes
+    from approxtorch_b200.backend import _C, ops
+    x = torch.randn(R, C, device=dev).to(dt)
+    x[R // 2, C // 2] = float("inf")                         # a block of NaN bytes
+    want = ops.fp8_quantize_both(x) if block_rows == 1 else ops.fp8_quantize_blocks(x)
+    up = lambda v, to: -(-v // to) * to                      # noqa: E731
+    spread = 1 if block_rows == 1 else 128
+    shapes = [(R, C, 16), (-(-R // spread), -(-C // 128), 1), (C, R, 16), (-(-C // spread), -(-R // 128), 1)]
+    bufs = [torch.full((rows, up(cols, 16) + 192), 0xEE, dtype=torch.uint8, device=dev) for rows, cols, _ in shapes]
+    args = [v for b in bufs for v in (b.data_ptr() + 32, b.stride(0))]
+    assert _C.lib.atb_fp8_quantize(x.data_ptr(), code, R, C, C, 5, block_rows, *args, None, 0, None,
+                                   ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    for buf, (rows, cols, to), ref in zip(bufs, shapes, want):
+        before, inside, after = buf[:, :32], buf[:, 32:32 + cols], buf[:, 32 + up(cols, to):]
+        assert torch.equal(inside, ref.view(torch.uint8))
+        assert before.numel() and after.shape[1] >= 160 and (before == 0xEE).all() and (after == 0xEE).all()

@@ -84,6 +84,7 @@ _SIGNATURES = {
     "atb_sum_rows": (_i, [_vp, _i, _ll, _vp, _vp]),
     "atb_fp8_gemm": (_i, [_vp, _i, _ll, _vp, _ll, _i] * 2 + [_vp, ctypes.c_float, _vp, _i, _ll, _i, _i, _i, _i, _vp, _vp]),
     "atb_fp8_status": (_i, [ctypes.POINTER(ctypes.c_int)]),
+    "atb_fp8_patience": (_i, [_i]),
     "atb_dropout": (_i, [_vp, _vp, _i, _ll, _i, _vp, _vp]),
     "atb_dropout_advance": (_i, [_vp, _vp, _vp]),
     "atb_probe_shared_load": (_i, [_vp, _vp, _i, _i, _vp]),

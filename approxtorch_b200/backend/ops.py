@@ -487,7 +487,10 @@ def fp8_gemm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Tenso
 
     The sum is held in fp32 (the tensor core applies the scales) and rounded once to ``out_dtype`` (fp32, bf16, fp16).
     e4m3 and e5m2 operands may be mixed.  ``drop_p`` / ``rng``: elements of y that ``dropout`` would drop become zero
-    (without its factor): the gradient of a product whose input was dropped out."""
+    (without its factor): the gradient of a product whose input was dropped out.
+
+    A product whose blocks waited for their operands in vain (a second without progress) leaves NaN; the next product raises
+    RuntimeError."""
     return _native.fp8_gemm(a, a_scale, b, b_scale, bias, alpha, out_dtype, drop_p, rng)
 
 

@@ -37,12 +37,12 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "philox.cuh"
 
 namespace atb {
-
-__device__ int g_fp8_status = 0;                      // 1: a block gave up waiting
 
 constexpr int kF8Threads = 384, kF8EpiWarp = 4, kF8EpiWarps = 8, kF8SplitThreads = 256;
 constexpr int kF8SumTileN = 192, kF8SumQuads = 2;            // with fp32 sums of partial products
@@ -70,6 +70,8 @@ struct Fp8Params {
     uint32_t idesc;
     bool vec;                            // rows of y start on 16-byte boundaries
     DropState drop;
+    int patience;                        // see f8_wait
+    int* error;                          // pinned host memory
 };
 
 __device__ __forceinline__ uint32_t f8_smem(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -85,12 +87,15 @@ __device__ __forceinline__ void f8_expect(uint32_t bar, uint32_t bytes)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Bounded wait that also gives up when another role of the block has.  CLUSTER: the arrivals it waits for order another
-// block's writes (an acquire over the cluster costs far more than one over the block; only the hand-overs that need it
-// pay for it).
-constexpr int kF8Patience = 1 << 18;                      // looks at a barrier: about a second
+// Bounded wait (`patience` looks at the barrier) that also gives up when another role of the block has.  CLUSTER: the arrivals it
+// waits for order another block's writes (an acquire over the cluster costs far more than one over the block; only the
+// hand-overs that need it pay for it).
+//
+// A block that gave up fills what it has not written with NaN, waits for its copies and MMAs in flight, says so in a word of
+// pinned host memory that the next call looks at, and returns.
+constexpr int kF8Patience = 1 << 18;                      // about a second
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int patience = kF8Patience)
+__device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int patience)
 {
     for (int i = 0; i < patience; ++i) {
         uint32_t ok;
@@ -105,6 +110,17 @@ __device__ __forceinline__ bool f8_wait(uint32_t bar, uint32_t parity, volatile 
     }
     *abort_flag = 1;
     return false;
+}
+// the wait for what is in flight when a block ends, whoever has given up before
+__device__ __forceinline__ bool f8_settle(uint32_t bar, uint32_t parity)
+{
+    int never = 0;
+    return f8_wait(bar, parity, &never, kF8Patience);
+}
+__device__ __forceinline__ void f8_report(int* error)
+{
+    *static_cast<volatile int*>(error) = 1;
+    __threadfence_system();
 }
 // one look at a barrier
 __device__ __forceinline__ bool f8_test(uint32_t bar, uint32_t parity)
@@ -192,6 +208,13 @@ __device__ __forceinline__ void f8_commit(uint32_t bar)
     else
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                      ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+// the same, at this block's barrier alone
+template <int CG>
+__device__ __forceinline__ void f8_commit_here(uint32_t bar)
+{
+    if (CG == 1) asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void f8_tmem_ld32(uint32_t (&v)[32], uint32_t addr)
 {
@@ -282,18 +305,37 @@ __device__ __forceinline__ void f8_tile(int t, int mt, int nt, int& tm, int& tn)
     tm = g * kF8Group + (in - tn * rows);
 }
 
+// NaN for what an epilogue warp still had to write when it gave up: its part of the tiles t, t + step, ...  Out of line, for the
+// loop's sake (inside it: 0.3 to 0.6 us of 5 to 14 us of a small product).
+template <class T, bool SUMS>
+__device__ __noinline__ void f8_blank(const Fp8Params& p, int t, int step, int cg, int rank)
+{
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = (warp - kF8EpiWarp) >> 2;
+    const int c0 = SUMS ? p.tile_n / 2 * group : 32 * group, c1 = SUMS ? c0 + p.tile_n / 2 : p.tile_n, by = SUMS ? 32 : 64;
+    for (; t < p.mt * p.nt; t += step) {
+        int tm, tn;
+        f8_tile(t, p.mt, p.nt, tm, tn);
+        const int m0 = (tm * cg + rank) * kF8TileM + (warp & 3) * 32, m1 = min(m0 + 32, p.M);
+        for (int c = c0; c < c1; c += by) {
+            const int n = tn * p.tile_n + c + lane;
+            if (n < p.N)
+                for (int m = m0; m < m1; ++m) static_cast<T*>(p.y)[m * p.ldy + n] = f8_out<T>(__uint_as_float(0x7FC00000u));
+        }
+    }
+}
+
 // SUMS: the tensor core's accumulator cuts what does not fit its 24 bits instead of rounding it, which leaves a bias towards
 // zero that grows with the number of additions (2e-6 of a result over 8192 steps).  A bf16 or fp16 result hides it; for a
 // long reduction to fp32 the accumulators are read every 1024 steps (kF8SumQuads quads) and added up, rounded, in the
 // registers of the epilogue warps, the two accumulators taking turns.
 template <class T, int CG, bool SUMS>
 __global__ void __launch_bounds__(kF8Threads, 1)
-fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Fp8Params p)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Fp8Params p)
 {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    __shared__ __align__(8) uint64_t s_full[kF8MaxStages], s_empty[kF8MaxStages], s_sf_full[kF8SfSlots], s_sf_empty[kF8SfSlots], s_acc_full[2], s_acc_empty[2], s_acc_part;
+    __shared__ __align__(8) uint64_t s_full[kF8MaxStages], s_empty[kF8MaxStages], s_sf_full[kF8SfSlots], s_sf_empty[kF8SfSlots], s_acc_full[2], s_acc_empty[2], s_acc_part, s_mma_done;
     constexpr int kPitch = 32 * sizeof(T) + 16;              // of a staged row: 16-byte accesses without bank conflicts
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);  // the same for a warp, and the compiler knows it
@@ -304,7 +346,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const uint32_t stage_bytes = kF8TileM * 128 + b_rows * 128;
     const uint32_t sf0 = smem0 + p.stages * stage_bytes, stage0 = sf0 + kF8SfSlots * kF8SfSlotBytes;
     const uint32_t full0 = f8_smem(s_full), empty0 = f8_smem(s_empty), sff0 = f8_smem(s_sf_full), sfe0 = f8_smem(s_sf_empty);
-    const uint32_t accf0 = f8_smem(s_acc_full), acce0 = f8_smem(s_acc_empty), accp = f8_smem(&s_acc_part);
+    const uint32_t accf0 = f8_smem(s_acc_full), acce0 = f8_smem(s_acc_empty), accp = f8_smem(&s_acc_part), done0 = f8_smem(&s_mma_done);
     const int ntiles = p.mt * p.nt, kb_n = p.kblocks, quads = (kb_n + 3) >> 2, runs = (kb_n + 15) >> 4;
     volatile int* abort_flag = &s_abort;
 
@@ -353,7 +395,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         for (int i = lane; i < kF8MaxStages; i += 32) { f8_bar_init(full0 + 8 * i, 1); f8_bar_init(empty0 + 8 * i, 1); }
         if (lane < kF8SfSlots) { f8_bar_init(sff0 + 8 * lane, CG); f8_bar_init(sfe0 + 8 * lane, 1); }
         if (lane < 2) { f8_bar_init(accf0 + 8 * lane, 1); f8_bar_init(acce0 + 8 * lane, kF8EpiWarps * CG); }
-        if (lane == 0) f8_bar_init(accp, kF8EpiWarps / 2 * CG);
+        if (lane == 0) { f8_bar_init(accp, kF8EpiWarps / 2 * CG); f8_bar_init(done0, 1); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     } else if (warp == 1) {
         if (f8_elect()) {
@@ -398,7 +440,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             f8_tile(t, p.mt, p.nt, tm, tn);
             const int m0 = (tm * CG + rank) * kF8TileM, n0 = tn * p.tile_n + rank * b_rows;
             for (int kb = 0; kb < kb_n; ++kb, ++issued) {
-                if (!(ok = f8_wait(empty0 + 8 * s, parity, abort_flag))) break;
+                if (!(ok = f8_wait(empty0 + 8 * s, parity, abort_flag, p.patience))) break;
                 if (f8_elect()) {
                     if (rank == 0) f8_expect(full0 + 8 * s, CG * stage_bytes);
                     const uint32_t bar = CG == 2 ? f8_leader(full0 + 8 * s) : full0 + 8 * s;
@@ -409,12 +451,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (++s == static_cast<uint32_t>(p.stages)) { s = 0; parity ^= 1u; }
             }
         }
-        // nothing may be in flight when the block ends (all of it has landed unless a role gave up)
-        if (rank == 0)
-            for (uint32_t j = issued > static_cast<uint32_t>(p.stages) ? issued - p.stages : 0; j < issued; ++j) {
-                int never = 0;
-                f8_wait(full0 + 8 * (j % p.stages), (j / p.stages) & 1u, &never);
-            }
+        // nothing may be in flight when the block ends (all of it has landed unless a role gave up); the second block of a pair
+        // has no barrier for its own share, which lands in microseconds: it waits a millisecond
+        if (rank == 0) {
+            for (uint32_t j = issued > static_cast<uint32_t>(p.stages) ? issued - p.stages : 0; j < issued; ++j)
+                if (!f8_settle(full0 + 8 * (j % p.stages), (j / p.stages) & 1u)) break;
+        } else if (!ok) {
+            for (int i = 0; i < 100; ++i) __nanosleep(10000);
+        }
     } else if (warp == 1) {
         if (rank == 0) {
             uint32_t parity = 0, quad = 0, tile = 0;         // tile: accumulators used so far
@@ -428,8 +472,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (tile_left == 0) tile_left = quads;
                 if (run_left == 0) { run_left = min(tile_left, 4u); ++run; }
                 const uint32_t from = (run - 1) & 1u, n = from ? taken[1] : taken[0], slot = 4 * from + (n & 3u), turn_parity = (n >> 2) & 1u;
-                if (staged >= 2 && !f8_wait(older_bar, older_parity, abort_flag)) return false;
-                if (!f8_wait<CG == 2>(sff0 + 8 * slot, turn_parity, abort_flag)) return false;
+                if (staged >= 2 && !f8_wait(older_bar, older_parity, abort_flag, p.patience)) return false;
+                if (!f8_wait<CG == 2>(sff0 + 8 * slot, turn_parity, abort_flag, p.patience)) return false;
                 older_bar = last_bar; older_parity = last_parity;
                 last_bar = sfe0 + 8 * slot; last_parity = turn_parity;
                 if (from) ++taken[1]; else ++taken[0];
@@ -454,8 +498,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 const uint32_t buf = tile & 1u, d = tmem + buf * d_step;
                 const int now = min(left, item_quads), kb_left = min(4 * now, kb_n - 4 * (quads - left));   // of this accumulator
                 left = left == now ? quads : left - now;
-                if (!(ok = f8_wait(acce0 + 8 * buf, ((tile >> 1) & 1u) ^ 1u, abort_flag))) break;
-                if (overlap && tile > 0 && !(ok = f8_wait(accp, (tile - 1) & 1u, abort_flag))) break;
+                if (!(ok = f8_wait(acce0 + 8 * buf, ((tile >> 1) & 1u) ^ 1u, abort_flag, p.patience))) break;
+                if (overlap && tile > 0 && !(ok = f8_wait(accp, (tile - 1) & 1u, abort_flag, p.patience))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 for (int q = 0; q < now && ok; ++q, ++quad) {
                     const uint32_t sfa = tmem + kF8SfCol + (quad & 1u) * kF8SfCols, slot = last_bar;
@@ -463,7 +507,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (i >= slices) break;
-                        if (!ready && !(ok = f8_wait(full, parity, abort_flag))) break;
+                        if (!ready && !(ok = f8_wait(full, parity, abort_flag, p.patience))) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint32_t at = a_lo, empty = full + (empty0 - full0);
                         a_lo += a_step;
@@ -484,6 +528,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (ok && f8_elect()) f8_commit<CG>(accf0 + 8 * buf);
                 __syncwarp();
             }
+            if (f8_elect()) f8_commit_here<CG>(done0);
+            __syncwarp();
+            f8_settle(done0, 0);
         }
     } else if (warp < kF8EpiWarp) {
         // Warps 2 and 3 take every other run.  A warp asks for its next run after the hand-over of the one before (the fence of
@@ -499,7 +546,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             for (int q = 0; q < 4; ++q) {
                 if (4 * sf_run + q >= quads) break;
                 const uint32_t n = handed + q, slot = 4 * (warp - 2) + (n & 3u), dst = sf0 + slot * kF8SfSlotBytes + lane * 16;
-                if (!(ok = f8_wait(sfe0 + 8 * slot, ((n >> 2) & 1u) ^ 1u, abort_flag))) break;
+                if (!(ok = f8_wait(sfe0 + 8 * slot, ((n >> 2) & 1u) ^ 1u, abort_flag, p.patience))) break;
 #pragma unroll
                 for (int j = 0; j < 3; ++j)
                     asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst + 512 * j), "r"(f8_word(w[4 * j], q)), "r"(f8_word(w[4 * j + 1], q)),
@@ -580,10 +627,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (lane == 0) { if (CG == 2) f8_arrive_leader(acce0 + 8 * buf); else f8_arrive(acce0 + 8 * buf); }
         };
         // an accumulator may take long where the reduction is: a second for every 65536 slices, which take 26 ms
-        const int patience = kF8Patience * (1 + (kb_n >> 16));
+        const int patience = p.patience * (1 + (kb_n >> 16));
         uint32_t item = 0;                                   // accumulators read so far
         bool ok = true;
-        for (int t = first; t < ntiles && ok; t += step) {
+        int t = first;
+        for (; t < ntiles; t += step) {
             int tm, tn;
             f8_tile(t, p.mt, p.nt, tm, tn);
             const int m0 = (tm * CG + rank) * kF8TileM + row0, n0 = tn * p.tile_n, rows = p.M - m0;
@@ -643,11 +691,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 ++item;
             }
         }
+        if (!ok) f8_blank<T, SUMS>(p, t, step, CG, rank);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     if (CG == 2) f8_cluster_sync(); else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    if (tid == 0 && s_abort) g_fp8_status = 1;
+    if (tid == 0 && s_abort) f8_report(p.error);
     if (warp == 3) {
         if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -663,21 +712,25 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 // it.  No workspace, no counters, one launch.  Measured back to back, bf16 results, against the best tile of
 // fp8_gemm_kernel: 1 x 4096 x 4096 5.4 us (12.3; the weights' 17 MB pass at 3.1 TB/s), 64 x 4096 x 4096 7.8 us (11.5),
 // 256 x 1000 x 2048 6.1 us (7.3).
+// (128 bytes, with the two maps 384 of a launch: at 400 the same kernel takes 0.2 to 0.6 us longer)
 struct Fp8SplitParams {
     const uint8_t* sa;
     const uint8_t* sb;
     long long ldsa, ldsb;
-    int a_shift, b_shift;
     const float* bias;
-    float alpha;
     void* y;
     long long ldy;
+    DropState drop;
+    int* error;
+    float alpha;
+    int patience;
     int M, N, kblocks;
-    int tile_c, ct, splits, stages;          // ct: column tiles
+    int tile_c, ct;                          // rows of A to a tile, column tiles
     uint32_t tmem_cols;
     uint32_t idesc;
-    DropState drop;
+    uint8_t a_shift, b_shift, splits, stages;
 };
+static_assert(sizeof(Fp8SplitParams) <= 128, "see above");
 
 __device__ __forceinline__ float f8_remote(uint32_t addr, uint32_t block)
 {
@@ -693,27 +746,29 @@ __device__ __forceinline__ uint32_t f8_cluster_rank()
     return r;
 }
 
-template <class T>
+// CUT: more than one block to a tile.  A form for each (and the rare path marked as such): what follows the product is short
+// enough for fetching its instructions to show, 256 x 1000 x 2048 5.6 instead of 6.1 us, 128 x 2048 x 1000 4.4 instead of 4.7.
+template <class T, bool CUT>
 __global__ void __launch_bounds__(kF8SplitThreads)
 fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_a, const Fp8SplitParams p)
 {
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    __shared__ __align__(8) uint64_t s_full[kF8MaxStages], s_empty[kF8MaxStages], s_sf[kF8MaxQuads], s_acc;
+    __shared__ __align__(8) uint64_t s_full[kF8MaxStages], s_empty[kF8MaxStages], s_sf[kF8MaxQuads], s_acc, s_mma_done;
     __shared__ unsigned s_keep[kF8TileM][4];                 // [row of A]: a bit for each row of B
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
-    const uint32_t rank = f8_cluster_rank();
-    const int tile = blockIdx.x / p.splits, n0 = (tile / p.ct) * kF8TileM, m0 = (tile % p.ct) * p.tile_c;
-    const int kb0 = static_cast<int>(static_cast<long long>(p.kblocks) * rank / p.splits);
-    const int kb1 = static_cast<int>(static_cast<long long>(p.kblocks) * (rank + 1) / p.splits);
+    const uint32_t rank = CUT ? f8_cluster_rank() : 0u;
+    const int tile = blockIdx.x / (CUT ? p.splits : 1), n0 = (tile / p.ct) * kF8TileM, m0 = (tile % p.ct) * p.tile_c;
+    const int kb0 = CUT ? static_cast<int>(static_cast<long long>(p.kblocks) * rank / p.splits) : 0;
+    const int kb1 = CUT ? static_cast<int>(static_cast<long long>(p.kblocks) * (rank + 1) / p.splits) : p.kblocks;
     const uint32_t smem0 = (f8_smem(smem_raw) + 1023u) & ~1023u;
     const uint32_t stage_bytes = (kF8TileM + p.tile_c) * 128, sf0 = smem0 + p.stages * stage_bytes;
-    const uint32_t full0 = f8_smem(s_full), empty0 = f8_smem(s_empty), sff0 = f8_smem(s_sf), acc0 = f8_smem(&s_acc);
+    const uint32_t full0 = f8_smem(s_full), empty0 = f8_smem(s_empty), sff0 = f8_smem(s_sf), acc0 = f8_smem(&s_acc), done0 = f8_smem(&s_mma_done);
     volatile int* abort_flag = &s_abort;
     if (warp == 0) {
-        if (lane == 0) { s_abort = 0; f8_bar_init(acc0, 1); }
+        if (lane == 0) { s_abort = 0; f8_bar_init(acc0, 1); f8_bar_init(done0, 1); }
         if (lane < kF8MaxStages) { f8_bar_init(full0 + 8 * lane, 1); f8_bar_init(empty0 + 8 * lane, 1); }
         for (int i = lane; i < kF8MaxQuads; i += 32) f8_bar_init(sff0 + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -732,12 +787,13 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
     after_previous();
     const uint32_t tmem = s_tmem;
     const int q0 = kb0 >> 2, quads = ((kb1 + 3) >> 2) - q0;      // of this block, by place in a scale row
+    uint32_t issued = 0;                                     // slices asked for (warp 0)
+    bool ok = true;
 
     if (warp == 0) {
         uint32_t s = 0, parity = 1;
-        bool ok = true;
-        for (int kb = kb0; kb < kb1; ++kb) {
-            if (!(ok = f8_wait(empty0 + 8 * s, parity, abort_flag))) break;
+        for (int kb = kb0; kb < kb1; ++kb, ++issued) {
+            if (!f8_wait(empty0 + 8 * s, parity, abort_flag, p.patience)) break;
             if (f8_elect()) {
                 f8_expect(full0 + 8 * s, stage_bytes);
                 f8_tma<1>(smem0 + s * stage_bytes, &map_b, kb * 128, n0, full0 + 8 * s);
@@ -746,17 +802,15 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
             __syncwarp();
             if (++s == static_cast<uint32_t>(p.stages)) { s = 0; parity ^= 1u; }
         }
-        if (!ok)                                             // nothing may be in flight when the block ends
-            for (int j = 0; j < p.stages; ++j) { int never = 0; f8_wait(full0 + 8 * j, parity ^ (j < static_cast<int>(s) ? 1u : 0u), &never); }
     } else if (warp == 1) {
         const uint32_t a_first = static_cast<uint32_t>(f8_desc(smem0)), a_step = stage_bytes >> 4, a_end = a_first + p.stages * a_step;
         uint32_t a_lo = a_first, full = full0, parity = 0, sfa = tmem + p.tile_c - 8;
-        bool ok = true, ready = false;
+        bool ready = false;
         for (int kb = kb0; kb < kb1; ++kb) {
             if (kb == kb0 || (kb & 3) == 0) {
                 const int q = (kb >> 2) - q0;
                 sfa += 8;
-                if (!(ok = f8_wait(sff0 + 8 * q, 0, abort_flag))) break;
+                if (!(ok = f8_wait(sff0 + 8 * q, 0, abort_flag, p.patience))) break;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (f8_elect()) {
                     f8_copy_scales<1>(sfa, f8_sf_desc(sf0 + q * 1024));
@@ -764,7 +818,7 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
                 }
                 __syncwarp();
             }
-            if (!ready && !(ok = f8_wait(full, parity, abort_flag))) break;
+            if (!ready && !(ok = f8_wait(full, parity, abort_flag, p.patience))) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t at = a_lo, empty = full + (empty0 - full0);
             a_lo += a_step;
@@ -779,7 +833,7 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
             }
             __syncwarp();
         }
-        if (ok && f8_elect()) f8_commit<1>(acc0);
+        if (f8_elect()) f8_commit<1>(ok ? acc0 : done0);
         __syncwarp();
     } else if (warp < kF8EpiWarp) {
         // scale words of a quad: lane i takes rows i, i + 32, ... of both operands
@@ -817,14 +871,14 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
             }
             asm volatile("bar.sync 1, 128;" ::: "memory");
         }
-        if (f8_wait(acc0, 0, abort_flag)) {
+        if (f8_wait(acc0, 0, abort_flag, p.patience)) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int row = (warp & 3) * 32 + lane, n = n0 + row;
-            const float bias = p.splits == 1 && p.bias != nullptr && n < p.N ? __uint_as_float(read4(p.bias + n)) : 0.0f;
+            const float bias = !CUT && p.bias != nullptr && n < p.N ? __uint_as_float(read4(p.bias + n)) : 0.0f;
             for (int c = 0; c < cols; c += 16) {
                 uint32_t v[16];
                 f8_tmem_ld16(v, tmem + c + (static_cast<uint32_t>((warp & 3) * 32) << 16));
-                if (p.splits == 1) {                         // nothing to meet: straight to y, a warp's lanes side by side
+                if constexpr (!CUT) {                        // nothing to meet: straight to y, a warp's lanes side by side
                     if (n < p.N) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j) if (c + j < cols) store(n, c + j, __uint_as_float(v[j]), bias);
@@ -838,15 +892,28 @@ fp8_split_kernel(const __grid_constant__ CUtensorMap map_b, const __grid_constan
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         }
     }
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (__builtin_expect(s_abort, 0)) {                      // once nothing is in flight, NaN for this block's part or its results
+        if (warp == 0)
+            for (uint32_t j = issued > static_cast<uint32_t>(p.stages) ? issued - p.stages : 0; j < issued; ++j)
+                if (!f8_settle(full0 + 8 * (j % p.stages), (j / p.stages) & 1u)) break;
+        if (warp == 1) f8_settle(ok ? acc0 : done0, 0);
+        __syncthreads();
+        const float nan = __uint_as_float(0x7FC00000u);
+        if (tid == 0) f8_report(p.error);
+        for (int i = tid; i < cols * kF8TileM; i += kF8SplitThreads) {
+            const int c = i / kF8TileM, n = n0 + i % kF8TileM;
+            if (CUT) asm volatile("st.shared.f32 [%0], %1;" ::"r"(smem0 + 4 * i), "f"(nan) : "memory");
+            else if (n < p.N) y[c * p.ldy + n] = f8_out<T>(nan);
+        }
+        __syncwarp();
+    }
     // Tensor memory goes back before this block waits for the others of its cluster: tcgen05.alloc waits without a limit, so a
     // block that kept its columns while it waited for one that still waits for columns could close a circle through a tensor-core
     // kernel of another stream that shares their SMs.
-    __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 3) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
-    if (tid == 0 && s_abort) g_fp8_status = 1;
-    if (p.splits == 1) return;
-    __syncwarp();
+    if (!CUT) return;
     f8_cluster_sync();                                       // the parts are in place
     // ---- every block finishes its share of the columns, four at a time so that the reads overlap
     const int row = tid & (kF8TileM - 1), n = n0 + row;
@@ -943,8 +1010,8 @@ static int fp8_cluster_blocks(int size)
         cfg.attrs = &attr;
         cfg.numAttrs = 1;
         int n = 0;
-        if (allow_smem(fp8_split_kernel<float>, kF8SplitSmem, done) != cudaSuccess ||
-            cudaOccupancyMaxActiveClusters(&n, fp8_split_kernel<float>, &cfg) != cudaSuccess || n <= 0) {
+        if (allow_smem(fp8_split_kernel<float, true>, kF8SplitSmem, done) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, fp8_split_kernel<float, true>, &cfg) != cudaSuccess || n <= 0) {
             cudaGetLastError();                              // an estimate does; the launch reports what is wrong
             n = sm_count() / size;
         }
@@ -1020,14 +1087,20 @@ static int launch_fp8_cg(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8
     return cg == 2 ? launch_fp8<T, 2, SUMS>(ma, mb, p, s) : launch_fp8<T, 1, SUMS>(ma, mb, p, s);
 }
 
-template <class T>
+template <class T, bool CUT>
 static int launch_split(const CUtensorMap& mb, const CUtensorMap& ma, const Fp8SplitParams& p, int tiles, size_t smem, cudaStream_t s)
 {
     static bool done[64];
-    cudaError_t e = allow_smem(fp8_split_kernel<T>, kF8SplitSmem, done);
-    if (e == cudaSuccess) e = launch_after(fp8_split_kernel<T>, dim3(tiles * p.splits), dim3(kF8SplitThreads), smem, s, p.splits, mb, ma, p);
+    cudaError_t e = allow_smem(fp8_split_kernel<T, CUT>, kF8SplitSmem, done);
+    if (e == cudaSuccess) e = launch_after(fp8_split_kernel<T, CUT>, dim3(tiles * p.splits), dim3(kF8SplitThreads), smem, s, p.splits, mb, ma, p);
     if (e != cudaSuccess) { set_error("fp8_split_kernel: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
     return check_launch("fp8_split_kernel");
+}
+
+template <class T>
+static int launch_split_cut(const CUtensorMap& mb, const CUtensorMap& ma, const Fp8SplitParams& p, int tiles, size_t smem, cudaStream_t s)
+{
+    return p.splits > 1 ? launch_split<T, true>(mb, ma, p, tiles, smem, s) : launch_split<T, false>(mb, ma, p, tiles, smem, s);
 }
 
 template <class T>
@@ -1035,6 +1108,29 @@ static int launch_bias(void* y, long long ldy, const float* bias, int M, int N, 
 {
     launch_after(fp8_bias_kernel<T>, dim3(grid_for(static_cast<long long>(M) * N, 256, 16 * sm_count())), dim3(256), 0, s, 0, static_cast<T*>(y), ldy, bias, M, N);
     return check_launch("fp8_bias_kernel");
+}
+
+// A word that the kernels of every device set when a block gave up, in pinned host memory so that the host sees it without
+// waiting for a device: 4 bytes, allocated by the first product and kept.
+static std::atomic<int*> g_error_word{nullptr};
+static std::atomic<int> g_patience{kF8Patience};
+
+static int* error_word()
+{
+    int* word = g_error_word.load(std::memory_order_acquire);
+    if (word != nullptr) return word;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;      // the first product may come inside a capture
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    int* fresh = nullptr;
+    if (cudaHostAlloc(reinterpret_cast<void**>(&fresh), sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
+        *fresh = 0;
+        if (g_error_word.compare_exchange_strong(word, fresh)) word = fresh;
+        else cudaFreeHost(fresh);                            // another thread was first: `word` is its
+    } else {
+        cudaGetLastError();
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return word;
 }
 
 }  // namespace atb
@@ -1071,7 +1167,16 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     ATB_REQUIRE(aligned_to(sa, 4) && aligned_to(sb, 4) && ldsa >= kblocks && ldsb >= kblocks && ldsa % 4 == 0 && ldsb % 4 == 0,
                 "scale rows must start on 4-byte boundaries");
 
+    int* const error = error_word();
+    if (error == nullptr) { set_error("no pinned memory for the product's error word"); return ATB_ERR_CUDA; }
+    if (__atomic_load_n(error, __ATOMIC_RELAXED) != 0 && __atomic_exchange_n(error, 0, __ATOMIC_ACQ_REL) != 0) {
+        set_error("an earlier product gave up waiting for its operands: the results that it left out are NaN (this call has done nothing)");
+        return ATB_ERR_CUDA;
+    }
+    const int patience = g_patience.load(std::memory_order_relaxed);
+
     Fp8Params p{};
+    p.patience = patience; p.error = error;
     p.sa = sa; p.sb = sb; p.ldsa = ldsa; p.ldsb = ldsb;
     p.a_shift = a_block_rows == 128 ? 7 : 0; p.b_shift = b_block_rows == 128 ? 7 : 0;
     p.sf_vec = aligned_to(sa, 16) && ldsa % 16 == 0 && aligned_to(sb, 16) && ldsb % 16 == 0;
@@ -1082,33 +1187,35 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     const uint32_t formats = (1u << 23);                     // scales are powers of two (ue8m0)
     CUtensorMap ma, mb;
     if (plan.splits) {
-        Fp8SplitParams q{sa, sb, ldsa, ldsb, p.a_shift, p.b_shift, bias, alpha, y, ldy, M, N, kblocks};
+        Fp8SplitParams q{sa, sb, ldsa, ldsb, bias, y, ldy, drop, error, alpha, patience, M, N, kblocks};
+        q.a_shift = static_cast<uint8_t>(p.a_shift);
+        q.b_shift = static_cast<uint8_t>(p.b_shift);
         q.tile_c = plan.tile;
         q.ct = (M + plan.tile - 1) / plan.tile;
-        q.splits = plan.splits;
+        q.splits = static_cast<uint8_t>(plan.splits);
         const int kbs = (kblocks + plan.splits - 1) / plan.splits, quads = kbs / 4 + 2, stage = (kF8TileM + plan.tile) * 128;
         const int sums = plan.tile * kF8TileM * 4;           // the partial tile takes the stages' place
-        q.stages = (kF8SplitSmem - 1024 - quads * 1024) / stage;
-        q.stages = q.stages < kbs ? q.stages : kbs;
-        q.stages = q.stages < kF8MaxStages ? q.stages : kF8MaxStages;
-        q.stages = q.stages * stage >= sums ? q.stages : (sums + stage - 1) / stage;
+        int stages = (kF8SplitSmem - 1024 - quads * 1024) / stage;
+        stages = stages < kbs ? stages : kbs;
+        stages = stages < kF8MaxStages ? stages : kF8MaxStages;
+        stages = stages * stage >= sums ? stages : (sums + stage - 1) / stage;
+        q.stages = static_cast<uint8_t>(stages);
         q.tmem_cols = 32;
         while (q.tmem_cols < static_cast<uint32_t>(plan.tile + 8 * quads)) q.tmem_cols *= 2;
         q.idesc = formats | (b_f8 == ATB_E5M2 ? 1u << 7 : 0u) | (a_f8 == ATB_E5M2 ? 1u << 10 : 0u) | (static_cast<uint32_t>(plan.tile >> 3) << 17) | (1u << 27);
-        q.drop = drop;
         // At least the tensor memory's share of an SM's 228 KB: blocks that fit an SM together then find their columns at once
         // instead of waiting for a neighbour's.
         const size_t share = 456 * static_cast<size_t>(q.tmem_cols) - 1024;
-        size_t smem = 1024 + static_cast<size_t>(q.stages) * stage + static_cast<size_t>(quads) * 1024;
+        size_t smem = 1024 + static_cast<size_t>(stages) * stage + static_cast<size_t>(quads) * 1024;
         smem = smem < share ? share : smem;
         smem = smem < kF8SplitSmem ? smem : kF8SplitSmem;    // (which leaves no room for a second block either)
         const int tiles = ((N + kF8TileM - 1) / kF8TileM) * q.ct;
         int rc = operand_map(&mb, b, N, K, ldb, kF8TileM);
         if (rc == ATB_OK) rc = operand_map(&ma, a, M, K, lda, plan.tile);
         if (rc != ATB_OK) return rc;
-        if (y_dtype == ATB_F32) return launch_split<float>(mb, ma, q, tiles, smem, s);
-        if (y_dtype == ATB_BF16) return launch_split<__nv_bfloat16>(mb, ma, q, tiles, smem, s);
-        return launch_split<__half>(mb, ma, q, tiles, smem, s);
+        if (y_dtype == ATB_F32) return launch_split_cut<float>(mb, ma, q, tiles, smem, s);
+        if (y_dtype == ATB_BF16) return launch_split_cut<__nv_bfloat16>(mb, ma, q, tiles, smem, s);
+        return launch_split_cut<__half>(mb, ma, q, tiles, smem, s);
     }
     const int cg = plan.cg;
     p.tile_n = plan.tile;
@@ -1134,7 +1241,14 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
 extern "C" int atb_fp8_status(int* status)
 {
     ATB_REQUIRE(status != nullptr, "null pointer");
-    const cudaError_t e = cudaMemcpyFromSymbol(status, g_fp8_status, sizeof(int));
-    if (e != cudaSuccess) { set_error("cudaMemcpyFromSymbol: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
+    const cudaError_t e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) { set_error("cudaDeviceSynchronize: %s", cudaGetErrorString(e)); return ATB_ERR_CUDA; }
+    int* const error = g_error_word.load(std::memory_order_acquire);
+    *status = error != nullptr ? __atomic_exchange_n(error, 0, __ATOMIC_ACQ_REL) : 0;
     return ATB_OK;
+}
+
+extern "C" int atb_fp8_patience(int looks)
+{
+    return g_patience.exchange(looks < 0 ? kF8Patience : looks < kF8Patience ? looks : kF8Patience);
 }

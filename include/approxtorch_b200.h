@@ -321,9 +321,14 @@ int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_t* sa, long
                  const void* b, int b_f8, long long ldb, const uint8_t* sb, long long ldsb, int b_block_rows,
                  const float* bias, float alpha, void* y, int y_dtype, long long ldy, int M, int N, int K,
                  int drop_threshold, const void* rng, void* stream);
-/* Device-side error word of the product (host pointer out; synchronises): 1 = a block gave up waiting for its operands
- * and left tiles unwritten. */
+/* Waits inside the product are bounded.  A block that gave up (about a second without progress) leaves NaN where its results
+ * would be and sets an error word, 4 bytes of pinned host memory that the first product allocates and every device shares.  The
+ * next atb_fp8_gemm clears it and returns ATB_ERR_CUDA without launching anything.  atb_fp8_status synchronises the current
+ * device, hands the word out (1 = a block gave up since it was last cleared) and clears it. */
 int atb_fp8_status(int* status /*host*/);
+/* Test aid: how many looks at a barrier the products launched from now on take before they give up (0: none at all; negative, or
+ * more than the default: the default).  Returns what held before. */
+int atb_fp8_patience(int looks);
 
 /* ---- counter-based dropout (no counterpart in the reference) ----------------------------------------------
  * y[i] = kept(i) ? x[i] * 65536 / (65536 - threshold) : 0.  kept(i): the 16 bits of element i drawn by Philox4x32-10

@@ -21,3 +21,18 @@ def test_split_kernel_returns_tensor_memory_before_it_waits_for_its_cluster():
     body = _kernel("fp8_gemm.cu", "fp8_split_kernel", "fp8_bias_kernel")
     alloc, free, wait = body.index("tcgen05.alloc"), body.index("tcgen05.dealloc"), body.index("f8_cluster_sync()")
     assert alloc < free < wait and "barrier.cluster" not in body[:free]
+
+
+def test_patience_of_the_products_waits():
+    from approxtorch_b200.backend import _C
+    assert _C.lib.atb_fp8_patience(5) == 1 << 18
+    assert _C.lib.atb_fp8_patience(-1) == 5 and _C.lib.atb_fp8_patience(1 << 30) == 1 << 18 and _C.lib.atb_fp8_patience(-1) == 1 << 18
+
+
+def test_products_fill_what_they_leave_out():
+    """Every wait of the two kernels is bounded by the launch's patience or is the wait for what is in flight at the end."""
+    import re
+    text = _kernel("fp8_gemm.cu", "fp8_gemm_kernel", "// ---- host side")
+    calls = re.findall(r"f8_wait(?:<[^(]*>)?\(.*", text)
+    assert len(calls) >= 12 and all("patience)" in c for c in calls)
+    assert text.count("f8_report(p.error)") == 2

@@ -62,3 +62,42 @@ def test_c_quantiser_leaves_a_wider_buffer_around_its_rows(dev, R, C, block_rows
         before, inside, after = buf[:, :32], buf[:, 32:32 + cols], buf[:, 32 + up(cols, to):]
         assert torch.equal(inside, ref.view(torch.uint8))
         assert before.numel() and after.shape[1] >= 160 and (before == 0xEE).all() and (after == 0xEE).all()
+
+
+# forms of the product: cut over a cluster and not, whole tiles of one block and of pairs, partial sums; with and without a mask
+GIVE_UP = [(1, 256, 128, 0.0), (5, 300, 700, 0.0), (5, 300, 700, 0.3), (64, 4096, 4096, 0.0), (2600, 2700, 700, 0.0), (2600, 2700, 700, 0.3),
+           (129, 9000, 4200, 0.0), (1300, 1301, 3000, 0.0), (3000, 40, 40, 0.0)]
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K,p", GIVE_UP)
+def test_a_product_that_gives_up_says_so(dev, M, N, K, p, out):
+    """Blocks that take no look at their barriers leave NaN and an error that the next product raises; the one after it is whole."""
+    import ctypes
+    from approxtorch_b200.backend import _C, ops
+    g = torch.Generator(dev).manual_seed(M + N)
+    a, b = ops.fp8_quantize_rows(_x(g, M, K)), ops.fp8_quantize_blocks(_x(g, N, K) / 64, transposed=False)
+    bias, state = torch.randn(N, device=dev), torch.tensor([1, 2], dtype=torch.int64, device=dev)
+    call = lambda: ops.fp8_gemm(*a, *b, bias=bias, out_dtype=out, drop_p=p, rng=state if p else None)   # noqa: E731
+    want = call()
+    kept = torch.ones_like(want, dtype=torch.bool) if not p else ops.dropout(torch.ones(M, N, device=dev), p, state) != 0
+    status = ctypes.c_int(-1)
+    assert torch.isfinite(want).all() and _C.lib.atb_fp8_status(ctypes.byref(status)) == 0 and status.value == 0
+    _C.lib.atb_fp8_patience(0)
+    try:
+        y = call()
+        torch.cuda.synchronize()
+    finally:
+        _C.lib.atb_fp8_patience(-1)
+    assert torch.isnan(y[kept]).all()
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        call()
+    assert torch.equal(call(), want)
+    _C.lib.atb_fp8_patience(0)
+    try:
+        call()
+    finally:
+        _C.lib.atb_fp8_patience(-1)
+    for value in (1, 0):
+        assert _C.lib.atb_fp8_status(ctypes.byref(status)) == 0 and status.value == value
+    assert torch.equal(call(), want)

@@ -451,7 +451,8 @@ def dropout(x: Tensor, p: float, rng: Tensor | None) -> Tensor:
 
 def dropout_advance(rng: Tensor) -> Tensor:
     """A copy of ``rng`` = {seed, offset} to draw from, after which the offset in ``rng`` moves on by one.  One launch and
-    no host work, so every replay of a captured graph draws anew."""
+    no host work, so every replay of a captured graph draws anew.  To autograd it is a change of ``rng`` in place: the backward
+    pass of what drew from ``rng`` itself raises."""
     return _native.dropout_advance(rng)
 
 

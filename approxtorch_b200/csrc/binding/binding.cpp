@@ -116,6 +116,8 @@ Tensor dropout_advance(const Tensor& rng)
     Tensor taken = fresh({2}, at::kLong, rng);
     const On on(rng);
     check_status(atb_dropout_advance(rng.mutable_data_ptr(), taken.mutable_data_ptr(), on.stream), "atb_dropout_advance");
+    // a change in place: a graph that saved `rng` itself refuses its backward pass instead of drawing another mask
+    if (!rng.is_inference()) rng.unsafeGetTensorImpl()->bump_version();
     return taken;
 }
 

@@ -101,3 +101,25 @@ def test_a_product_that_gives_up_says_so(dev, M, N, K, p, out):
     for value in (1, 0):
         assert _C.lib.atb_fp8_status(ctypes.byref(status)) == 0 and status.value == value
     assert torch.equal(call(), want)
+
+
+def test_a_state_that_moved_on_is_refused_in_the_backward_pass(dev):
+    """The mask of the backward pass is drawn from the state that the forward pass was given: one that changed since raises, as
+    every saved tensor that was changed in place does; a state handed out by dropout_advance stays as it is."""
+    import approxtorch_b200 as at
+    from approxtorch_b200.backend import ops
+    x, w = torch.randn(40, 96, device=dev, requires_grad=True), torch.randn(50, 96, device=dev, requires_grad=True)
+    for run in (lambda r: at.nn.dropout.counter_dropout(x, 0.5, r), lambda r: at.nn.gemm_fp8.linear_fp8(x, w, None, 0.5, r)):
+        state = torch.tensor([3, 0], dtype=torch.int64, device=dev)
+        want, = torch.autograd.grad(run(state).sum(), x)
+        y = run(state)
+        taken = ops.dropout_advance(state)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y.sum(), x)
+        y = run(taken)
+        ops.dropout_advance(state)
+        assert torch.equal(torch.autograd.grad(y.sum(), x)[0], want)
+    with torch.inference_mode():
+        state = torch.tensor([3, 0], dtype=torch.int64, device=dev)
+        assert ops.dropout_advance(state).tolist() == [3, 0]
+    assert ops.dropout_advance(state).tolist() == [3, 1] and state.tolist() == [3, 2]     # an inference tensor has no version

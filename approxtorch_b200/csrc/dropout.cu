@@ -93,15 +93,13 @@ __global__ void __launch_bounds__(256, 4) dropout_kernel(const T* x, T* y, long 
     }
 }
 
-// state = {seed, offset}: `taken` gets the state that this call draws from, the offset moves on by one.  On the device,
-// so that every replay of a captured graph draws anew.
+// state = {seed, offset}: `taken` gets the state that this call draws from, the offset moves on by one.  On the device, so that
+// every replay of a captured graph draws anew; in one step, so that calls of several streams get offsets of their own.
 __global__ void drop_advance_kernel(unsigned long long* state, unsigned long long* taken)
 {
     after_previous();
-    const unsigned long long seed = state[0], off = state[1];
-    taken[0] = seed;
-    taken[1] = off;
-    state[1] = off + 1;
+    taken[0] = state[0];
+    taken[1] = atomicAdd(state + 1, 1ull);
 }
 
 template <class T>

@@ -335,7 +335,8 @@ int atb_fp8_patience(int looks);
  * (key = seed, counter = (i / 8, offset), low halves first) are >= threshold.  rng: device {seed, offset}, 2 x 64 bits.
  * The gradient is the same call on the incoming gradient.  x == y is allowed. */
 int atb_dropout(const void* x, void* y, int dtype, long long numel, int threshold, const void* rng, void* stream);
-/* taken = state; state.offset += 1 (on the device, so that replays of a captured graph draw anew). */
+/* taken = state; state.offset += 1 (on the device, so that replays of a captured graph draw anew; atomically, so that calls on
+ * several streams take different offsets). */
 int atb_dropout_advance(void* state, void* taken, void* stream);
 
 /* ---- measurement aid (no counterpart in the reference) ---------------------------------------------

@@ -123,3 +123,19 @@ def test_a_state_that_moved_on_is_refused_in_the_backward_pass(dev):
         state = torch.tensor([3, 0], dtype=torch.int64, device=dev)
         assert ops.dropout_advance(state).tolist() == [3, 0]
     assert ops.dropout_advance(state).tolist() == [3, 1] and state.tolist() == [3, 2]     # an inference tensor has no version
+
+
+def test_streams_that_share_a_state_take_offsets_of_their_own(dev):
+    from approxtorch_b200.backend import ops
+    state = torch.tensor([3, 100], dtype=torch.int64, device=dev)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(8)]
+    taken = []
+    for _ in range(100):
+        for s in streams:
+            with torch.cuda.stream(s):
+                taken.append(ops.dropout_advance(state))
+    torch.cuda.synchronize()
+    assert state.tolist() == [3, 900]
+    got = torch.stack(taken)
+    assert (got[:, 0] == 3).all() and sorted(got[:, 1].tolist()) == list(range(100, 900))

@@ -10,17 +10,21 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG, "lib", "libapproxtorch_b200.so")
 
 
+def _have_nvcc() -> bool:
+    import shutil
+    return os.path.exists("/usr/local/cuda/bin/nvcc") or shutil.which("nvcc") is not None
+
+
 def _refresh_if_stale() -> None:
     """Rebuild the library when a source is newer than it and a compiler is at hand (a no-op otherwise)."""
     from ..build import build_library, sources
-    import shutil
-    have_nvcc = os.path.exists("/usr/local/cuda/bin/nvcc") or shutil.which("nvcc") is not None
-    if have_nvcc and sources():
+    if _have_nvcc() and sources():
         build_library()
 
 
@@ -98,22 +102,44 @@ for _name, (_res, _args) in _SIGNATURES.items():
 EXPORTED = tuple(_SIGNATURES)
 
 
+_binding_lock = threading.Lock()
+
+
 def _load_binding():
     """The native binding (``csrc/binding/binding.cpp``) of the 8-bit floating point operators and dropout; it finds the
     library above beside itself."""
     import importlib.machinery
     import importlib.util
     import torch  # noqa: F401  (its libraries have to be in the process)
-    path = os.path.join(_PKG, "lib", "_binding.so")
-    if not os.path.exists(path):
-        raise ImportError(f"{path} is missing: build it first with `python -m approxtorch_b200.build`")
-    loader = importlib.machinery.ExtensionFileLoader("_binding", path)
+    from ..build import BINDING_PATH, build_binding
+    if _have_nvcc():
+        try:
+            build_binding()
+        except RuntimeError as e:
+            raise ImportError("the native binding of the 8-bit floating point operators and of counter-based dropout cannot be built "
+                              f"against this torch ({torch.__version__}): {e}") from e
+    if not os.path.exists(BINDING_PATH):
+        raise ImportError(f"{BINDING_PATH} is missing (the native binding of the 8-bit floating point operators and of counter-based "
+                          "dropout): build it first with `python -m approxtorch_b200.build`")
+    loader = importlib.machinery.ExtensionFileLoader("_binding", BINDING_PATH)
     module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
-    loader.exec_module(module)
+    try:
+        loader.exec_module(module)
+    except ImportError as e:
+        raise ImportError(f"{BINDING_PATH} does not load beside this torch ({torch.__version__}): {e}.  Build it anew with "
+                          "`python -m approxtorch_b200.build --force`") from e
     return module
 
 
-binding = _load_binding()
+def __getattr__(name: str):
+    """``binding`` is loaded (and refreshed like the library) when one of its operators is first asked for: what goes through
+    the C ABI alone needs neither torch's headers nor a host compiler that takes them."""
+    if name != "binding":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    with _binding_lock:
+        if "binding" not in globals():
+            globals()["binding"] = _load_binding()
+    return globals()["binding"]
 
 
 def last_error() -> str:

@@ -425,20 +425,19 @@ def decode_table(device, offset: int) -> Tensor:
 
 
 # --------------------------------------------------------------------------- 8-bit floating point, counter-based dropout
-# Checks, outputs and launches of these are native (csrc/binding/binding.cpp).  Conventions as above: fresh outputs on the
+# Checks, outputs and launches of these are native (csrc/binding/binding.cpp, loaded by the first call).  Conventions as above: fresh outputs on the
 # input's device, the current stream, no synchronisation, RuntimeError before any launch; inputs that the kernels can
 # read as they lie (a row pitch, an offset) are not copied.
-_native = _C.binding
 
 
 def drop_threshold(p: float) -> int:
     """The drop rate as the generator holds it: round(p 65536) of 65536."""
-    return _native.drop_threshold(p)
+    return _C.binding.drop_threshold(p)
 
 
 def drop_factor(p: float) -> float:
     """1 / (1 - rate) for the rounded rate (0 where everything is dropped)."""
-    return _native.drop_factor(p)
+    return _C.binding.drop_factor(p)
 
 
 def dropout(x: Tensor, p: float, rng: Tensor | None) -> Tensor:
@@ -446,14 +445,14 @@ def dropout(x: Tensor, p: float, rng: Tensor | None) -> Tensor:
 
     ``rng``: int64 {seed, offset} on x's device.  The same call on the incoming gradient is the backward pass.  ``p`` is
     rounded to a multiple of 2^-16.  fp32, bf16 or fp16; elements are numbered in row-major order whatever the strides."""
-    return _native.dropout(x, p, rng)
+    return _C.binding.dropout(x, p, rng)
 
 
 def dropout_advance(rng: Tensor) -> Tensor:
     """A copy of ``rng`` = {seed, offset} to draw from, after which the offset in ``rng`` moves on by one.  One launch and
     no host work, so every replay of a captured graph draws anew.  To autograd it is a change of ``rng`` in place: the backward
     pass of what drew from ``rng`` itself raises."""
-    return _native.dropout_advance(rng)
+    return _C.binding.dropout_advance(rng)
 
 
 def fp8_quantize_rows(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn, drop_p: float = 0.0, rng: Tensor | None = None):
@@ -466,19 +465,19 @@ def fp8_quantize_rows(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn, drop_
 
     ``drop_p`` / ``rng``: x is dropped out first, with the mask of ``dropout`` but without its factor 1 / (1 - p), which is
     left to the product's ``alpha`` so that what is quantised stays exact."""
-    return tuple(_native.fp8_quantize(x, dtype, 1, False, drop_p, rng))
+    return tuple(_C.binding.fp8_quantize(x, dtype, 1, False, drop_p, rng))
 
 
 def fp8_quantize_both(x: Tensor, dtype: torch.dtype = torch.float8_e4m3fn, drop_p: float = 0.0, rng: Tensor | None = None):
     """(q, scale, qt, scale_t) in one pass over x [R, C]: ``fp8_quantize_rows(x)`` and ``fp8_quantize_rows(x.t())``, the
     operands of a product along C and of its gradient product along R.  The mask of ``drop_p`` is numbered in x."""
-    return tuple(_native.fp8_quantize(x, dtype, 1, True, drop_p, rng))
+    return tuple(_C.binding.fp8_quantize(x, dtype, 1, True, drop_p, rng))
 
 
 def fp8_quantize_blocks(w: Tensor, dtype: torch.dtype = torch.float8_e4m3fn, transposed: bool = True):
     """Weights w [R, C] with one scale for each 128 x 128 block: (q [R, C], scale [ceil(R / 128), ceil(C / 128)]) and, with
     ``transposed``, the same numbers as (qt [C, R], scale_t) for the product with the transposed weights."""
-    return tuple(_native.fp8_quantize(w, dtype, 128, transposed, 0.0, None))
+    return tuple(_C.binding.fp8_quantize(w, dtype, 128, transposed, 0.0, None))
 
 
 def fp8_gemm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Tensor | None = None, alpha: float = 1.0,
@@ -492,7 +491,7 @@ def fp8_gemm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Tenso
 
     A product whose blocks waited for their operands in vain (a second without progress) leaves NaN; the next product raises
     RuntimeError."""
-    return _native.fp8_gemm(a, a_scale, b, b_scale, bias, alpha, out_dtype, drop_p, rng)
+    return _C.binding.fp8_gemm(a, a_scale, b, b_scale, bias, alpha, out_dtype, drop_p, rng)
 
 
 # --------------------------------------------------------------------------- operator implementations

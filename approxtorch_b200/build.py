@@ -12,6 +12,7 @@ library and torch's.  nvcc cross-compiles, so no GPU is needed to build.
 from __future__ import annotations
 
 import concurrent.futures
+import contextlib
 import glob
 import os
 import shutil
@@ -61,14 +62,24 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     Safe to call from several processes at once (every rank of a torchrun job imports the package): the
     build runs under an exclusive file lock, and the library is linked under a temporary name and moved into
     place atomically, so no process ever opens a half-written file."""
+    with _build_lock():
+        return _build_locked(force, verbose)
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> str:
+    """Compile (if stale) and return the path of the native binding; needs the library, torch and a host compiler."""
+    with _build_lock():
+        return _build_binding(force, verbose)
+
+
+@contextlib.contextmanager
+def _build_lock():
     import fcntl
     os.makedirs(LIB_DIR, exist_ok=True)
     with open(os.path.join(LIB_DIR, ".build.lock"), "w") as lock:
         fcntl.flock(lock, fcntl.LOCK_EX)
         try:
-            lib = _build_locked(force, verbose)
-            _build_binding(force, verbose)
-            return lib
+            yield
         finally:
             fcntl.flock(lock, fcntl.LOCK_UN)
 
@@ -115,18 +126,27 @@ def _build_locked(force: bool, verbose: bool) -> str:
 def _build_binding(force: bool, verbose: bool) -> str:
     import importlib.util
     import sysconfig
-    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("torch is not installed")
+    torch_dir = os.path.dirname(spec.origin)
     if not force and not _stale(BINDING_PATH, [BINDING_SRC, HEADER, os.path.join(torch_dir, "version.py")]):
         return BINDING_PATH
+    import torch
+    abi = int(torch.compiled_with_cxx11_abi())
     include = os.path.join(torch_dir, "include")
     cuda_include = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include")
     cxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else shutil.which("g++") or "g++"
     tmp = f"{BINDING_PATH}.{os.getpid()}.tmp"
-    cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_binding", "-isystem", include,
+    cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_binding",
+           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-isystem", include,
            "-isystem", os.path.join(include, "torch", "csrc", "api", "include"), "-isystem", sysconfig.get_paths()["include"],
            "-isystem", cuda_include, BINDING_SRC, "-o", tmp, "-L" + LIB_DIR, "-lapproxtorch_b200", "-Wl,-rpath,$ORIGIN",
            "-L" + os.path.join(torch_dir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
+    try:
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+    except OSError as error:
+        raise RuntimeError(f"{cxx}: {error}") from error
     if verbose or proc.returncode != 0:
         sys.stderr.write(f"--- binding.cpp\n{proc.stdout}{proc.stderr}\n")
     if proc.returncode != 0:
@@ -138,4 +158,9 @@ def _build_binding(force: bool, verbose: bool) -> str:
 
 
 if __name__ == "__main__":
-    print(build_library(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
+    options = {"force": "--force" in sys.argv, "verbose": "--verbose" in sys.argv}
+    print(build_library(**options))
+    try:
+        print(build_binding(**options))
+    except RuntimeError as error:                            # the library serves everything else
+        sys.stderr.write(f"{error}: no 8-bit floating point operators and no counter-based dropout from Python\n")

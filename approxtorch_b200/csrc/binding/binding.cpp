@@ -53,6 +53,10 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like)
     return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt));
 }
 
+// A tensor whose memory holds its values: a view that only notes that it is negative (the imaginary part of a conjugate) is what
+// the dispatcher resolves on the way to a kernel, and these operators are called beside it.
+Tensor in_memory(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // The gradient node of a leaf belongs to the stream on which an operator first asked for it, for as long as a result of that
@@ -88,7 +92,7 @@ double drop_factor(double p)
 const void* drop_state(int threshold, const std::optional<Tensor>& rng, const c10::Device& device)
 {
     if (threshold == 0) return nullptr;
-    TORCH_CHECK(rng.has_value() && rng->scalar_type() == at::kLong && rng->numel() == 2 && rng->is_contiguous() && rng->device() == device,
+    TORCH_CHECK(rng.has_value() && rng->scalar_type() == at::kLong && rng->numel() == 2 && rng->is_contiguous() && !rng->is_neg() && rng->device() == device,
                 "rng must be a contiguous int64 tensor {seed, offset} on the input's device");
     return rng->const_data_ptr();
 }
@@ -99,7 +103,7 @@ Tensor dropout(const Tensor& x, double p, const std::optional<Tensor>& rng)
     const int code = float_code(x.scalar_type()), threshold = drop_threshold(p);
     TORCH_CHECK(code >= 0, "x must be float32, bfloat16 or float16");
     const void* state = drop_state(threshold, rng, x.device());
-    const Tensor xc = x.contiguous();
+    const Tensor xc = in_memory(x).contiguous();
     if (threshold == 0) return xc.clone();
     Tensor y = fresh(xc.sizes(), xc.scalar_type(), xc);
     if (y.numel()) {
@@ -112,7 +116,7 @@ Tensor dropout(const Tensor& x, double p, const std::optional<Tensor>& rng)
 Tensor dropout_advance(const Tensor& rng)
 {
     TORCH_CHECK(rng.is_cuda(), "rng must be a CUDA tensor");
-    TORCH_CHECK(rng.scalar_type() == at::kLong && rng.numel() == 2 && rng.is_contiguous(), "rng must be a contiguous int64 tensor {seed, offset}");
+    TORCH_CHECK(rng.scalar_type() == at::kLong && rng.numel() == 2 && rng.is_contiguous() && !rng.is_neg(), "rng must be a contiguous int64 tensor {seed, offset}");
     Tensor taken = fresh({2}, at::kLong, rng);
     const On on(rng);
     check_status(atb_dropout_advance(rng.mutable_data_ptr(), taken.mutable_data_ptr(), on.stream), "atb_dropout_advance");
@@ -160,8 +164,9 @@ struct Held {
 };
 
 // rows that the kernel can read as they lie, or a copy
-Tensor quantiser_input(const Tensor& x, const char* name = "x")
+Tensor quantiser_input(const Tensor& given, const char* name = "x")
 {
+    const Tensor x = in_memory(given);
     TORCH_CHECK(x.is_cuda(), name, " must be a CUDA tensor");
     TORCH_CHECK(float_code(x.scalar_type()) >= 0, name, " must be float32, bfloat16 or float16");
     TORCH_CHECK(x.dim() == 2, name, " must have shape [R, C]");
@@ -242,6 +247,7 @@ Operand operand(const Tensor& t, const Tensor& scale, const char* name)
     TORCH_CHECK(scale.scalar_type() == kScale || scale.scalar_type() == at::kByte, name, "_scale must be torch.float8_e8m0fnu (or its bytes)");
     TORCH_CHECK(t.dim() == 2 && scale.dim() == 2, name, " and ", name, "_scale must have two dimensions");
     TORCH_CHECK(scale.device() == t.device(), name, " and ", name, "_scale must be on one device");
+    TORCH_CHECK(!t.is_neg() && !scale.is_neg(), name, " and ", name, "_scale must not be negative views");
     Held& h = o.at;
     h.R = t.size(0);
     h.C = t.size(1);
@@ -285,7 +291,9 @@ Tensor bias_vector(const std::optional<Tensor>& bias, int64_t N, const c10::Devi
     if (!bias.has_value() || !bias->defined()) return Tensor();
     TORCH_CHECK(bias->device() == device && bias->dim() == 1 && bias->size(0) == N && float_code(bias->scalar_type()) >= 0,
                 "bias must be a float tensor of ", N, " elements on the operands' device");
-    return bias->detach().to(at::kFloat).contiguous();
+    Tensor b = in_memory(bias->detach().to(at::kFloat)).contiguous();
+    TORCH_CHECK(N == 0 || b.const_data_ptr() != nullptr, "bias holds no data");          // (a null pointer means none)
+    return b;
 }
 const float* bias_pointer(const Tensor& bias) { return bias.defined() ? bias.const_data_ptr<float>() : nullptr; }
 

@@ -139,3 +139,39 @@ def test_streams_that_share_a_state_take_offsets_of_their_own(dev):
     assert state.tolist() == [3, 900]
     got = torch.stack(taken)
     assert (got[:, 0] == 3).all() and sorted(got[:, 1].tolist()) == list(range(100, 900))
+
+
+def test_negative_views_are_resolved(dev):
+    """Views that only note that they are negative (the imaginary part of a conjugate) count as the values they stand for, as
+    inputs, weights, biases and incoming gradients; as operands and states they are refused."""
+    import approxtorch_b200 as at
+    from approxtorch_b200.backend import ops
+    g = torch.Generator(dev).manual_seed(6)
+    state = torch.tensor([3, 0], dtype=torch.int64, device=dev)
+    base = torch.randn(40, 96, generator=g, device=dev)
+    imag = torch.randn(40, 96, dtype=torch.complex64, generator=g, device=dev).conj().imag
+    for x in (torch._neg_view(base), torch._neg_view(base.t()), imag, torch._neg_view(base.bfloat16())):
+        assert x.is_neg()
+        ref = torch.empty(x.shape, dtype=x.dtype, device=dev).copy_(x)
+        assert not ref.is_neg() and (ref != 0).any()
+        for f in (ops.fp8_quantize_rows, ops.fp8_quantize_both, ops.fp8_quantize_blocks, lambda t: (ops.dropout(t, 0.5, state),),
+                  lambda t: (ops.dropout(t, 0.0, None),)):
+            for got, want in zip(f(x), f(ref)):
+                assert torch.equal(got.contiguous().view(torch.uint8), want.contiguous().view(torch.uint8))
+    w, b, go = (torch.randn(s, generator=g, device=dev) for s in ((50, 96), (50,), (40, 50)))
+    neg = torch._neg_view
+    leaves = [t.clone().requires_grad_(True) for t in (-base, -w, -b)]
+    want = at.nn.gemm_fp8.linear_fp8(*leaves, 0.25, state)
+    views = [t.clone().requires_grad_(True) for t in (base, w, b)]
+    got = at.nn.gemm_fp8.linear_fp8(*(neg(t) for t in views), 0.25, state)
+    assert torch.equal(got, want)
+    for p, q in zip(torch.autograd.grad(got, views, neg(go)), torch.autograd.grad(want, leaves, go)):
+        assert torch.equal(p, q)                             # two signs: of the view and of the incoming gradient
+    a = ops.fp8_quantize_rows(base)
+    assert torch.equal(ops.fp8_gemm(*a, *a, bias=neg(b[:40])), ops.fp8_gemm(*a, *a, bias=-b[:40]))
+    assert torch.equal(ops.fp8_gemm(*a, *a, bias=neg(b[:40].half())), ops.fp8_gemm(*a, *a, bias=-b[:40].half()))
+    for bad in (lambda: ops.dropout(base, 0.5, neg(state)), lambda: ops.dropout_advance(neg(state)), lambda: ops.fp8_gemm(neg(a[0]), a[1], *a),
+                lambda: ops.fp8_gemm(a[0], neg(a[1].view(torch.uint8)), *a)):
+        with pytest.raises(RuntimeError):
+            bad()
+    assert state.tolist() == [3, 0]

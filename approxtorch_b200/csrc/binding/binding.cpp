@@ -380,7 +380,12 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
         // the bias gradient comes out of the quantiser's pass over the gradient where that makes both layouts
         const int64_t sum_rows = (M + 127) / 128, sum_bytes = need_b && need_w && M ? up(sum_rows * N * 4, 256) : 0;
         Tensor scratch, dx, dw, db;
+        // hooks for saved tensors may hand back anything, and the kernels would read it as device memory
+        TORCH_CHECK(!threshold || (rng.defined() && drop_state(threshold, rng, go.device())), "the saved state of the dropout is missing");
         if (need_x || need_w) {
+            TORCH_CHECK(kept.defined() && kept.device() == go.device() && kept.scalar_type() == at::kByte && kept.is_contiguous() &&
+                            kept.numel() == (laid_w ? xt.bytes() : 0) + (laid_x ? wt.bytes() : 0),
+                        "the saved operands of linear_fp8 came back on another device or in another form");
             uint8_t* at = kept.mutable_data_ptr<uint8_t>();
             if (laid_w) at = xt.place(at);
             if (laid_x) wt.place(at);
@@ -398,7 +403,7 @@ struct LinearFp8 : torch::autograd::Function<LinearFp8> {
         }
         if (need_x) {
             dx = fresh(x_shape, go.scalar_type(), go);
-            product(gq, ATB_E4M3, wt, ATB_E4M3, nullptr, alpha, dx, threshold, rng.defined() ? rng.const_data_ptr() : nullptr, on.stream);
+            product(gq, ATB_E4M3, wt, ATB_E4M3, nullptr, alpha, dx, threshold, threshold ? rng.const_data_ptr() : nullptr, on.stream);
         }
         if (need_w) {
             dw = fresh({N, K}, static_cast<at::ScalarType>(ctx->saved_data["w_type"].toInt()), go);

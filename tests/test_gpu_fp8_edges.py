@@ -175,3 +175,26 @@ def test_negative_views_are_resolved(dev):
         with pytest.raises(RuntimeError):
             bad()
     assert state.tolist() == [3, 0]
+
+
+def test_saved_operands_that_come_back_changed_are_refused(dev):
+    """Hooks for saved tensors may hand back anything: what is not the memory that was saved is refused before a launch."""
+    import approxtorch_b200 as at
+    state = torch.tensor([3, 0], dtype=torch.int64, device=dev)
+    x, w, go = torch.randn(40, 96, device=dev, requires_grad=True), torch.randn(50, 96, device=dev, requires_grad=True), torch.randn(40, 50, device=dev)
+    lin = lambda p: at.nn.gemm_fp8.linear_fp8(x, w, None, p, state)          # noqa: E731
+    want = torch.autograd.grad(lin(0.3), (x, w), go)
+    only = lambda size, f: lambda t: f(t) if (t.numel() == 2) == size else t                                   # noqa: E731
+    for change in (only(False, lambda t: t.cpu()), only(False, lambda t: t[:-1]), only(False, lambda t: t[::2]), only(False, lambda t: t.short()),
+                   only(True, lambda t: t.cpu()), only(True, lambda t: t.float()), only(True, lambda t: t[:1])):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            y = lin(0.3)
+            z = at.nn.dropout.counter_dropout(x, 0.3, state)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, (x, w), go)
+        if change(state) is not state:
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(z.sum(), x)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(dev)):
+        y = lin(0.3)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (x, w), go), want))

@@ -485,8 +485,10 @@ def fp8_gemm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Tenso
     """y [M, N] = alpha * A B^T + bias for 8-bit floating point A [M, K], B [N, K] with a power-of-two scale for each block
     of 128 along K: scale shapes [rows, ceil(K / 128)] or, for 128 x 128 blocks, [ceil(rows / 128), ceil(K / 128)].
 
-    The sum is held in fp32 (the tensor core applies the scales) and rounded once to ``out_dtype`` (fp32, bf16, fp16).
-    e4m3 and e5m2 operands may be mixed.  ``drop_p`` / ``rng``: elements of y that ``dropout`` would drop become zero
+    The sum is held in the tensor core's 24-bit accumulator (which applies the scales, and cuts what does not fit) and rounded
+    once to ``out_dtype`` (fp32, bf16, fp16).  Where nothing cancels, an fp32 result comes out low by up to about 5e-7 of itself;
+    long reductions (beyond 2048 steps to fp32, 2^15 to fp16, 2^18 to bf16) are added up from partial sums in rounded fp32, so
+    that it stays there and a 16-bit result is as good as its rounding.  e4m3 and e5m2 operands may be mixed.  ``drop_p`` / ``rng``: elements of y that ``dropout`` would drop become zero
     (without its factor): the gradient of a product whose input was dropped out.
 
     A product whose blocks waited for their operands in vain (a second without progress) leaves NaN; the next product raises

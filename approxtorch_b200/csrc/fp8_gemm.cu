@@ -2,8 +2,8 @@
 //
 //   y[m, n] = alpha * sum_k  A[m, k] 2^(sa[m', k/128] - 127)  B[n, k] 2^(sb[n', k/128] - 127)  + bias[n]
 //
-// with m' = m or m / 128 (one scale for a row's block, or for a 128 x 128 block), n' likewise; the sum in fp32 in the
-// tensor core, one rounding at the end.  The scales are applied by the tensor core itself: tcgen05.mma
+// with m' = m or m / 128 (one scale for a row's block, or for a 128 x 128 block), n' likewise; the sum in the tensor core's 24-bit
+// accumulator, which cuts instead of rounding (what that costs, and what is done about it: SUMS below), one rounding at the end.  The scales are applied by the tensor core itself: tcgen05.mma
 // kind::mxf8f6f4.block_scale takes one exponent byte per row and 32 steps of the reduction from tensor memory, and four
 // consecutive instructions read the same byte.  So the product runs at the rate of an unscaled 8-bit product; promoting
 // every 128-step partial sum through registers instead would cost a read of the accumulator per 128 steps.
@@ -51,7 +51,8 @@ constexpr int kF8SfSlots = 8, kF8SfSlotBytes = 3 * 512;   // a run of quads for 
 constexpr int kF8SfCol = 488, kF8SfCols = 12;             // tensor-memory columns of the two scale buffers
 constexpr int kF8Smem = 226 * 1024, kF8MaxStages = 8;
 constexpr int kF8SplitSmem = kF8Smem - kF8TileM * 16;    // fp8_split_kernel: its mask besides
-constexpr int kF8SumsFrom = 16;                          // slices beyond which an fp32 result is added up from partial sums
+constexpr int kF8SumsFrom = 16;                          // slices beyond which an fp32 result is added up from partial sums,
+constexpr int kF8SumsFromFp16 = 256, kF8SumsFromBf16 = 2048;     // a 16-bit one
 constexpr int kF8MaxQuads = 40;                           // of one block of fp8_split_kernel
 constexpr int kF8Group = 8;                               // row tiles that are walked together (their operands meet in L2)
 
@@ -324,10 +325,14 @@ __device__ __noinline__ void f8_blank(const Fp8Params& p, int t, int step, int c
     }
 }
 
-// SUMS: the tensor core's accumulator cuts what does not fit its 24 bits instead of rounding it, which leaves a bias towards
-// zero that grows with the number of additions (2e-6 of a result over 8192 steps).  A bf16 or fp16 result hides it; for a
-// long reduction to fp32 the accumulators are read every 1024 steps (kF8SumQuads quads) and added up, rounded, in the
-// registers of the epilogue warps, the two accumulators taking turns.
+// SUMS: the tensor core's accumulator has the 24 bits of fp32, but cuts what does not fit instead of rounding it, at several
+// places of an MMA, which leaves a bias towards zero that grows with the number of additions.  Measured with magnitudes of normal
+// numbers, which is a sum without cancellation: 1.8e-7 of the result over 1024 steps, 5e-7 over 2048, 4e-4 over 2^18, 3e-3 over
+// 2^20, 8e-2 over 2^24 (of numbers of both signs the magnitudes' 1e-8 and less).  So a long reduction reads the accumulators
+// every 1024 steps (kF8SumQuads quads) and adds them up, rounded, in the registers of the epilogue warps, the two accumulators
+// taking turns: beyond 2048 steps to fp32 (8192 steps 117 us, every 2048 steps 114, never 111; 2e-7 to 5e-7), and where the bias
+// would near a quarter of a step of a 16-bit result, n 2^-23 for n = steps / 32 additions as an estimate: 2^15 steps to fp16, 2^18
+// to bf16.
 template <class T, int CG, bool SUMS>
 __global__ void __launch_bounds__(kF8Threads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ Fp8Params p)
@@ -1033,11 +1038,11 @@ struct Fp8Plan {
     int splits;              // fp8_split_kernel where not 0: blocks to a tile; tile = rows of A
 };
 
-// fp32: the result is fp32, so a reduction over more than 2048 steps is added up from partial sums (SUMS): tiles of 64, 128 or
-// 192 columns, and no block of the split kernel gets more than that.
-static Fp8Plan fp8_plan(int M, int N, int kblocks, bool fp32)
+// A reduction over more than sums_from slices is added up from partial sums (SUMS): tiles of 64, 128 or 192 columns, and no block
+// of the split kernel gets more slices than that.
+static Fp8Plan fp8_plan(int M, int N, int kblocks, int sums_from)
 {
-    const bool sums = fp32 && kblocks > kF8SumsFrom;
+    const bool sums = kblocks > sums_from;
     Fp8Plan best{1, sums ? 64 : 32, 0};
     double least = 1e300;
     const int sms = sm_count();
@@ -1059,7 +1064,7 @@ static Fp8Plan fp8_plan(int M, int N, int kblocks, bool fp32)
         if (mt * nt > 16.0 * sms) continue;                  // many tiles: never the better kernel
         for (int splits = 1; splits <= 8 && splits <= kblocks; ++splits) {
             const int slices = (kblocks + splits - 1) / splits;
-            if (slices / 4 + 2 > kF8MaxQuads || (fp32 && slices > kF8SumsFrom)) continue;
+            if (slices / 4 + 2 > kF8MaxQuads || slices > sums_from) continue;
             const double waves = ceil(mt * nt * splits / fp8_cluster_blocks(splits));
             const double t = waves * (slices * (0.14 + 0.0016 * tile) + 0.8 + 0.025 * tile + 0.06 * splits) + (splits > 1 ? 2.8 : 2.0);
             if (t < least) { least = t; best = Fp8Plan{1, tile, splits}; }
@@ -1081,10 +1086,11 @@ static int launch_fp8(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Par
     return check_launch("fp8_gemm_kernel");
 }
 
-template <class T, bool SUMS>
-static int launch_fp8_cg(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Params& p, int cg, cudaStream_t s)
+template <class T>
+static int launch_fp8_cg(const CUtensorMap& ma, const CUtensorMap& mb, const Fp8Params& p, int cg, bool sums, cudaStream_t s)
 {
-    return cg == 2 ? launch_fp8<T, 2, SUMS>(ma, mb, p, s) : launch_fp8<T, 1, SUMS>(ma, mb, p, s);
+    if (sums) return cg == 2 ? launch_fp8<T, 2, true>(ma, mb, p, s) : launch_fp8<T, 1, true>(ma, mb, p, s);
+    return cg == 2 ? launch_fp8<T, 2, false>(ma, mb, p, s) : launch_fp8<T, 1, false>(ma, mb, p, s);
 }
 
 template <class T, bool CUT>
@@ -1181,8 +1187,9 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     p.a_shift = a_block_rows == 128 ? 7 : 0; p.b_shift = b_block_rows == 128 ? 7 : 0;
     p.sf_vec = aligned_to(sa, 16) && ldsa % 16 == 0 && aligned_to(sb, 16) && ldsb % 16 == 0;
     p.bias = bias; p.alpha = alpha; p.y = y; p.ldy = ldy; p.M = M; p.N = N; p.kblocks = kblocks;
-    const Fp8Plan plan = fp8_plan(M, N, kblocks, y_dtype == ATB_F32);
-    const bool sums = y_dtype == ATB_F32 && kblocks > kF8SumsFrom && !plan.splits;
+    const int sums_from = y_dtype == ATB_F32 ? kF8SumsFrom : y_dtype == ATB_F16 ? kF8SumsFromFp16 : kF8SumsFromBf16;
+    const Fp8Plan plan = fp8_plan(M, N, kblocks, sums_from);
+    const bool sums = kblocks > sums_from && !plan.splits;
     const DropState drop{drop_threshold ? static_cast<const unsigned long long*>(rng) : nullptr, static_cast<unsigned>(drop_threshold)};
     const uint32_t formats = (1u << 23);                     // scales are powers of two (ue8m0)
     CUtensorMap ma, mb;
@@ -1232,10 +1239,9 @@ extern "C" int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_
     int rc = operand_map(&ma, a, M, K, lda, kF8TileM);
     if (rc == ATB_OK) rc = operand_map(&mb, b, N, K, ldb, p.tile_n / cg);
     if (rc != ATB_OK) return rc;
-    if (sums) return launch_fp8_cg<float, true>(ma, mb, p, cg, s);
-    if (y_dtype == ATB_F32) return launch_fp8_cg<float, false>(ma, mb, p, cg, s);
-    if (y_dtype == ATB_BF16) return launch_fp8_cg<__nv_bfloat16, false>(ma, mb, p, cg, s);
-    return launch_fp8_cg<__half, false>(ma, mb, p, cg, s);
+    if (y_dtype == ATB_F32) return launch_fp8_cg<float>(ma, mb, p, cg, sums, s);
+    if (y_dtype == ATB_BF16) return launch_fp8_cg<__nv_bfloat16>(ma, mb, p, cg, sums, s);
+    return launch_fp8_cg<__half>(ma, mb, p, cg, sums, s);
 }
 
 extern "C" int atb_fp8_status(int* status)

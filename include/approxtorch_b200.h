@@ -312,8 +312,10 @@ int atb_fp8_quantize(const void* x, int x_dtype, long long R, long long C, long 
                      long long ldst, float* column_sums, int drop_threshold, const void* rng, void* stream);
 /* out[c] = sum over r of p[r, c], p [rows, C] fp32, in the order of the rows. */
 int atb_sum_rows(const float* p, int rows, long long C, float* out, void* stream);
-/* y[m, n] = alpha * sum_k A[m, k] B[n, k] (scales applied) + bias[n], summed in fp32, rounded once to y_dtype
- * (fp32 / bf16 / fp16); A [M, K], B [N, K].  Row pitches lda, ldb: multiples of 16, bases 16-byte aligned; ldsa, ldsb:
+/* y[m, n] = alpha * sum_k A[m, k] B[n, k] (scales applied) + bias[n], rounded once to y_dtype (fp32 / bf16 / fp16);
+ * A [M, K], B [N, K].  The sum is the tensor core's: 24 bits, what does not fit is cut.  Where nothing cancels, an fp32 result is
+ * low by up to about 5e-7 of itself (2e-7 at 1024 steps); beyond 2048 steps (fp16 results: 2^15, bf16: 2^18) partial sums are
+ * added in rounded fp32, which keeps it there, and a 16-bit result's error that of its rounding.  Row pitches lda, ldb: multiples of 16, bases 16-byte aligned; ldsa, ldsb:
  * multiples of 4, bases 4-byte aligned, and every scale row readable up to a multiple of 4 bytes (of 16, where base and
  * pitch are multiples of 16).  bias fp32 or NULL.
  * drop_threshold > 0: elements of y that atb_dropout would drop from the contiguous [M, N] tensor become 0 (no factor). */

@@ -198,3 +198,40 @@ def test_saved_operands_that_come_back_changed_are_refused(dev):
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(dev)):
         y = lin(0.3)
     assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, (x, w), go), want))
+
+
+def _exact(a, b):
+    """A B^T and |A| |B|^T in 64 bits, from the bytes of values and scales, a stretch of the reduction at a time."""
+    (qa, sa), (qb, sb) = a, b
+    out = [torch.zeros(qa.shape[0], qb.shape[0], dtype=torch.float64, device=qa.device) for _ in range(2)]
+    part = lambda q, s, i: q[:, 128 * i:128 * (i + 512)].float().double() * torch.exp2(                        # noqa: E731
+        s[:, i:i + 512].contiguous().view(torch.uint8).double() - 127).repeat_interleave(128, 1)[:, :q.shape[1] - 128 * i]
+    for i in range(0, sa.shape[1], 512):
+        da, db = part(qa, sa, i), part(qb, sb, i)
+        out[0] += da @ db.t()
+        out[1] += da.abs() @ db.abs().t()
+    return out
+
+
+@pytest.mark.parametrize("out,M,N,K", [(torch.float16, 8, 300, 2 ** 18), (torch.float16, 8, 300, 2 ** 20 - 77), (torch.bfloat16, 8, 300, 2 ** 20),
+                                       (torch.float16, 2, 3, 2 ** 22 + 130), (torch.bfloat16, 2, 3, 2 ** 22), (torch.float16, 700, 500, 2 ** 18),
+                                       (torch.bfloat16, 300, 290, 2 ** 19 + 5), (torch.float32, 8, 300, 2 ** 20)])
+def test_long_sums_of_one_sign_keep_their_size(dev, out, M, N, K):
+    """The accumulator cuts: an MMA adds 32 products to it, and each of the 33 may lose a unit, 2^-23 of the running sum at most.  Over
+    the 32 MMAs of a partial sum that grows evenly this is 33 (1 + ... + 32) / 32 2^-23 = 545 2^-23 of it; the K / 1024 partial sums
+    are added in fp32, half a unit of the running sum each; the epilogue rounds twice in fp32 and once to the result's type."""
+    from approxtorch_b200.backend import ops
+    g = torch.Generator(dev).manual_seed(K)
+    a, b = (ops.fp8_quantize_rows(torch.randn(n, K, generator=g, device=dev).abs()) for n in (M, N))
+    ref, _ = _exact(a, b)
+    alpha = 2.0 ** -18
+    bias = torch.rand(N, generator=g, device=dev)
+    for p in (0.0, 0.5):
+        state = torch.tensor([4, 2], dtype=torch.int64, device=dev)
+        want = alpha * ref + bias.double()
+        if p:
+            want = torch.where(ops.dropout(torch.ones(M, N, device=dev), p, state) != 0, want, 0.0)
+        y = ops.fp8_gemm(*a, *b, bias=bias, alpha=alpha, out_dtype=out, drop_p=p, rng=state).double()
+        # evenly: quantised magnitudes of normal numbers, whose sums over 1024 steps are within a tenth of one another
+        tol = 1.1 * 545 * 2.0 ** -23 + (-(-K // 1024) + 2) * 2.0 ** -24 + torch.finfo(out).eps / 2
+        assert ((y - want).abs() <= tol * want.abs()).all(), ((y - want).abs() / want.abs().clamp(min=1e-30)).max().item()

@@ -235,3 +235,69 @@ def test_long_sums_of_one_sign_keep_their_size(dev, out, M, N, K):
         # evenly: quantised magnitudes of normal numbers, whose sums over 1024 steps are within a tenth of one another
         tol = 1.1 * 545 * 2.0 ** -23 + (-(-K // 1024) + 2) * 2.0 ** -24 + torch.finfo(out).eps / 2
         assert ((y - want).abs() <= tol * want.abs()).all(), ((y - want).abs() / want.abs().clamp(min=1e-30)).max().item()
+
+
+def _whole_numbers(g, R, K):
+    """An operand of the numbers -2 .. 2 with a scale of 1, 2, 4 or 8 for each row and slice."""
+    q = torch.randint(-2, 3, (R, K), generator=g, device=g.device, dtype=torch.int8).half().to(E4)
+    return q, torch.randint(127, 131, (R, -(-K // 128)), generator=g, device=g.device, dtype=torch.uint8)
+
+
+# one and several blocks to a tile, pairs, partial sums of every result's type
+WHOLE = [(1, 1000, 2048), (17, 700, 33000), (1, 300, 100000), (3, 200, 200000), (700, 64, 65536), (300, 500, 2049), (300, 500, 20000),
+         (2600, 1500, 5000), (256, 1000, 2048), (40, 60, 300001), (520, 300, 270000)]
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("M,N,K", WHOLE)
+def test_every_slice_counts_once(dev, M, N, K, out):
+    """Whole numbers whose magnitudes add up to less than 2^24: every order of additions is exact, so a result equals the exact one
+    rounded once.  A slice left out, taken twice or scaled by the next power of two would change most of them."""
+    from approxtorch_b200.backend import ops
+    g = torch.Generator(dev).manual_seed(M + N + K)
+    a, b = _whole_numbers(g, M, K), _whole_numbers(g, N, K)
+    b[1].clamp_(max=128)
+    ref, mag = _exact(a, b)
+    assert mag.max() < 2 ** 24
+    alpha = 2.0 ** -6 if out == torch.float16 else 1.0
+    round_ = lambda v: (v * alpha).float().to(out)           # noqa: E731  (v fits fp32)
+    assert torch.equal(ops.fp8_gemm(*a, *b, alpha=alpha, out_dtype=out), round_(ref))
+    # what a fault of one slice would do, on the reference
+    for i in (0, a[1].shape[1] // 3, a[1].shape[1] - 1):
+        part = [(q[:, 128 * i:128 * (i + 1)].contiguous(), s[:, i:i + 1].contiguous()) for q, s in (a, b)]
+        one = _exact(*part)[0]
+        for fault in (ref - one, ref + one):                 # left out; taken twice, or twice the scale
+            assert (round_(fault) != round_(ref)).float().mean() > 0.3
+
+
+@pytest.mark.parametrize("M,N", [(8, 300), (512, 512)])
+@pytest.mark.parametrize("K", [128, 256, 512, 1000, 1024, 1500, 2048, 4096, 8192])
+def test_sums_to_fp32_lose_little(dev, M, N, K):
+    """Sums of one sign.  An MMA's result is cut to 24 bits: half a unit on average, a unit being 2^-23 of the running sum at most;
+    over the n = K / 32 MMAs of a sum that grows evenly n / 4 units, n 2^-25 of the result (n = 64 at most, then partial sums
+    are added in fp32), and the last rounding.  The root mean square of the errors stays within that."""
+    from approxtorch_b200.backend import ops
+    g = torch.Generator(dev).manual_seed(K)
+    a, b = (ops.fp8_quantize_rows(torch.randn(n, K, generator=g, device=dev).abs()) for n in (M, N))
+    ref, _ = _exact(a, b)
+    err = (ops.fp8_gemm(*a, *b, out_dtype=torch.float32).double() - ref) / ref
+    n = min(-(-K // 32), 64)
+    assert err.square().mean().sqrt() <= n * 2.0 ** -25 + (1 + -(-K // 1024)) * 2.0 ** -24
+
+
+def test_transforms_are_refused(dev):
+    """No batching rule and no forward derivative: torch refuses both instead of computing something else."""
+    import approxtorch_b200 as at
+    from approxtorch_b200.backend import ops
+    state = torch.tensor([3, 0], dtype=torch.int64, device=dev)
+    x, w = torch.randn(4, 40, 96, device=dev), torch.randn(50, 96, device=dev)
+    lin, drop = at.nn.gemm_fp8.linear_fp8, at.nn.dropout.counter_dropout
+    for f in (lambda t: lin(t, w), lambda t: drop(t, 0.5, state), lambda t: ops.fp8_quantize_rows(t), lambda t: ops.dropout(t, 0.5, state)):
+        with pytest.raises(RuntimeError):
+            torch.vmap(f)(x)
+    for f in (lambda t: lin(t, w), lambda t: drop(t, 0.5, state)):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x[0],), (x[1],))
+        with pytest.raises(RuntimeError):
+            with torch.autograd.forward_ad.dual_level():
+                f(torch.autograd.forward_ad.make_dual(x[0], x[1]))

@@ -256,6 +256,7 @@ Operand operand(const Tensor& t, const Tensor& scale, const char* name)
                 (h.R + 127) / 128, ", ", nb, "], got ", scale.sizes());
     h.block_rows = rows == h.R ? 1 : 128;
     if (h.R == 0 || h.C == 0) return o;
+    TORCH_CHECK(t.const_data_ptr() != nullptr && scale.const_data_ptr() != nullptr, name, " and ", name, "_scale must hold data");
     h.ldq = h.R > 1 ? t.stride(0) : up(h.C, 16);
     if ((h.C > 1 && t.stride(1) != 1) || h.ldq % 16 || h.ldq < h.C || reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16) {
         o.values = repacked(t);

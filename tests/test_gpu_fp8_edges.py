@@ -301,3 +301,22 @@ def test_transforms_are_refused(dev):
         with pytest.raises(RuntimeError):
             with torch.autograd.forward_ad.dual_level():
                 f(torch.autograd.forward_ad.make_dual(x[0], x[1]))
+
+
+def test_tensors_without_data_are_refused(dev):
+    """What a tracer hands in (shapes without memory) reaches no kernel."""
+    import approxtorch_b200 as at
+    from approxtorch_b200.backend import ops
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    x, w, b = torch.randn(40, 96, device=dev), torch.randn(50, 96, device=dev), torch.randn(50, device=dev)
+    state = torch.tensor([3, 0], dtype=torch.int64, device=dev)
+    a, aw = ops.fp8_quantize_rows(x), ops.fp8_quantize_rows(w)
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        fake = mode.from_tensor
+        for call in (lambda: ops.dropout(fake(x), 0.5, state), lambda: ops.dropout(x, 0.5, fake(state)), lambda: ops.dropout_advance(fake(state)),
+                     lambda: ops.fp8_quantize_rows(fake(x)), lambda: ops.fp8_quantize_both(fake(x.t())), lambda: ops.fp8_quantize_rows(x, drop_p=0.5, rng=fake(state)),
+                     lambda: at.nn.gemm_fp8.linear_fp8(fake(x), w, b), lambda: at.nn.gemm_fp8.linear_fp8(x, fake(w), b),
+                     lambda: at.nn.gemm_fp8.linear_fp8(x, w, fake(b)), lambda: ops.fp8_gemm(fake(a[0]), a[1], *aw), lambda: ops.fp8_gemm(a[0], fake(a[1]), *aw),
+                     lambda: ops.fp8_gemm(*a, fake(aw[0]), aw[1]), lambda: ops.fp8_gemm(*a, *aw, bias=fake(b))):
+            with pytest.raises(RuntimeError):
+                call()

@@ -320,3 +320,49 @@ def test_tensors_without_data_are_refused(dev):
                      lambda: ops.fp8_gemm(*a, fake(aw[0]), aw[1]), lambda: ops.fp8_gemm(*a, *aw, bias=fake(b))):
             with pytest.raises(RuntimeError):
                 call()
+
+
+FIRST = """
+import threading, torch
+from approxtorch_b200.backend import ops
+dev = torch.device("cuda:0")
+x, w = torch.randn(130, 700, device=dev), torch.randn(300, 700, device=dev)
+a, b = ops.fp8_quantize_rows(x), ops.fp8_quantize_blocks(w, transposed=False)
+torch.cuda.synchronize()
+{first}
+torch.cuda.synchronize()
+want = ops.fp8_gemm(*a, *b)
+assert torch.isfinite(want).all() and len(got) > 0 and all(torch.equal(y, want) for y in got)
+print("whole")
+"""
+CAPTURED = """
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = [ops.fp8_gemm(*a, *b)]
+graph.replay()
+"""
+THREADS = """
+got, start = [], threading.Barrier(8)
+def work():
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        for _ in range(20):
+            got.append(ops.fp8_gemm(*a, *b))
+        torch.cuda.current_stream().synchronize()
+threads = [threading.Thread(target=work) for _ in range(8)]
+for t in threads: t.start()
+for t in threads: t.join()
+assert len(got) == 160
+"""
+
+
+@pytest.mark.parametrize("first", [CAPTURED, THREADS], ids=["captured", "threads"])
+def test_first_product_of_a_process(dev, first):
+    """The first product sets up what later ones find (allowed shared memory, the error word): inside a capture, or by several host
+    threads at once."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST.format(first=first)], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "whole" in done.stdout, done.stderr[-2000:]

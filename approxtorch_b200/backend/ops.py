@@ -427,7 +427,8 @@ def decode_table(device, offset: int) -> Tensor:
 # --------------------------------------------------------------------------- 8-bit floating point, counter-based dropout
 # Checks, outputs and launches of these are native (csrc/binding/binding.cpp, loaded by the first call).  Conventions as above: fresh outputs on the
 # input's device, the current stream, no synchronisation, RuntimeError before any launch; inputs that the kernels can
-# read as they lie (a row pitch, an offset) are not copied.
+# read as they lie (a row pitch, an offset) are not copied.  They are not operators of torch's dispatcher: torch.compile runs them
+# as they are, between the graphs that it makes, torch.export refuses them, and so do vmap and forward derivatives.
 
 
 def drop_threshold(p: float) -> int:
@@ -488,7 +489,9 @@ def fp8_gemm(a: Tensor, a_scale: Tensor, b: Tensor, b_scale: Tensor, bias: Tenso
     The sum is held in the tensor core's 24-bit accumulator (which applies the scales, and cuts what does not fit) and rounded
     once to ``out_dtype`` (fp32, bf16, fp16).  Where nothing cancels, an fp32 result comes out low by up to about 5e-7 of itself;
     long reductions (beyond 2048 steps to fp32, 2^15 to fp16, 2^18 to bf16) are added up from partial sums in rounded fp32, so
-    that it stays there and a 16-bit result is as good as its rounding.  e4m3 and e5m2 operands may be mixed.  ``drop_p`` / ``rng``: elements of y that ``dropout`` would drop become zero
+    that it stays there and a 16-bit result is as good as its rounding.
+
+    e4m3 and e5m2 operands may be mixed.  ``drop_p`` / ``rng``: elements of y that ``dropout`` would drop become zero
     (without its factor): the gradient of a product whose input was dropped out.
 
     A product whose blocks waited for their operands in vain (a second without progress) leaves NaN; the next product raises

@@ -22,10 +22,11 @@
 // Two accumulators let the epilogue of a tile run under the MMAs of the next; where two of 256 columns and the scales do
 // not fit the 512 columns of tensor memory, they share 24 columns, which the epilogue reads first.  Why pairs: each block of
 // a pair holds its own 128 rows of A and half the rows of B and the tensor core reads both halves, so a slice of a 256 x 256
-// tile costs each SM 32 KB from L2 instead of the 48 KB of a 128 x 256 tile.  What bounds it: 8192^3 in 376 us (2.92 PFLOP/s, a
-// library product of the same operands with a scale for each 32: 404 us), 510 clocks for a slice of a 256 x 256 tile that
-// the tensor core needs 512 for at its nominal rate; kept up for long, the power limit (445 us).  What it took to get there, and
-// what a change should not lose: the issuing warp runs converged and walks uniform values (a branch on the lane number cost
+// tile costs each SM 32 KB from L2 instead of the 48 KB of a 128 x 256 tile.  What bounds it: the
+// tensor core, at the clock that the power limit leaves.  8192^3: 541 clocks for a slice of a 256 x 256 tile, first loads and last
+// results included, where the tensor core's nominal rate is 512.  One call by itself 353 us (3.1 PFLOP/s) at 1.39 GHz, the fifth in a
+// row 400 at 1.30, four seconds of them 450 at 1.13 GHz (990 W, the power limit the only reason; a library product of the same
+// operands with a scale for each 32: 404).  What it took to get there, and what a change should not lose: the issuing warp runs converged and walks uniform values (a branch on the lane number cost
 // 40 %), the scales arrive a quad ahead, and only hand-overs of memory between the blocks pay for cluster scope.
 //
 // fp8_split_kernel, for products of few tiles (serving, small heads): see there.
@@ -715,8 +716,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 // block requests its whole share of B at once (up to kF8MaxStages slices).  The S partial tiles meet in shared memory: every
 // block adds up its share of the columns over the cluster in the order of the blocks (bit for bit repeatable) and stores
 // it.  No workspace, no counters, one launch.  Measured back to back, bf16 results, against the best tile of
-// fp8_gemm_kernel: 1 x 4096 x 4096 5.4 us (12.3; the weights' 17 MB pass at 3.1 TB/s), 64 x 4096 x 4096 7.8 us (11.5),
-// 256 x 1000 x 2048 6.1 us (7.3).
+// fp8_gemm_kernel: 1 x 4096 x 4096 5.6 us (12.3; the weights' 17 MB pass at 3.0 TB/s), 64 x 4096 x 4096 7.2 us (11.5),
+// 256 x 1000 x 2048 5.6 us (7.3).
 // (128 bytes, with the two maps 384 of a launch: at 400 the same kernel takes 0.2 to 0.6 us longer)
 struct Fp8SplitParams {
     const uint8_t* sa;

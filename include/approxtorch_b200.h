@@ -315,9 +315,9 @@ int atb_sum_rows(const float* p, int rows, long long C, float* out, void* stream
 /* y[m, n] = alpha * sum_k A[m, k] B[n, k] (scales applied) + bias[n], rounded once to y_dtype (fp32 / bf16 / fp16);
  * A [M, K], B [N, K].  The sum is the tensor core's: 24 bits, what does not fit is cut.  Where nothing cancels, an fp32 result is
  * low by up to about 5e-7 of itself (2e-7 at 1024 steps); beyond 2048 steps (fp16 results: 2^15, bf16: 2^18) partial sums are
- * added in rounded fp32, which keeps it there, and a 16-bit result's error that of its rounding.  Row pitches lda, ldb: multiples of 16, bases 16-byte aligned; ldsa, ldsb:
- * multiples of 4, bases 4-byte aligned, and every scale row readable up to a multiple of 4 bytes (of 16, where base and
- * pitch are multiples of 16).  bias fp32 or NULL.
+ * added in rounded fp32, which keeps it there, and a 16-bit result's error that of its rounding.
+ * Row pitches lda, ldb: multiples of 16, bases 16-byte aligned; ldsa, ldsb: multiples of 4, bases 4-byte aligned, and every scale
+ * row readable up to a multiple of 4 bytes (of 16, where base and pitch are multiples of 16).  bias fp32 or NULL.
  * drop_threshold > 0: elements of y that atb_dropout would drop from the contiguous [M, N] tensor become 0 (no factor). */
 int atb_fp8_gemm(const void* a, int a_f8, long long lda, const uint8_t* sa, long long ldsa, int a_block_rows,
                  const void* b, int b_f8, long long ldb, const uint8_t* sb, long long ldsb, int b_block_rows,

@@ -24,10 +24,11 @@
 // a pair holds its own 128 rows of A and half the rows of B and the tensor core reads both halves, so a slice of a 256 x 256
 // tile costs each SM 32 KB from L2 instead of the 48 KB of a 128 x 256 tile.  What bounds it: the
 // tensor core, at the clock that the power limit leaves.  8192^3: 541 clocks for a slice of a 256 x 256 tile, first loads and last
-// results included, where the tensor core's nominal rate is 512.  One call by itself 353 us (3.1 PFLOP/s) at 1.39 GHz, the fifth in a
-// row 400 at 1.30, four seconds of them 450 at 1.13 GHz (990 W, the power limit the only reason; a library product of the same
-// operands with a scale for each 32: 404).  What it took to get there, and what a change should not lose: the issuing warp runs converged and walks uniform values (a branch on the lane number cost
-// 40 %), the scales arrive a quad ahead, and only hand-overs of memory between the blocks pay for cluster scope.
+// results included, where the tensor core's nominal rate is 512.  One call by itself 353 us (3.1 PFLOP/s) at 1.39 GHz, the fifth
+// in a row 400 at 1.30, four seconds of them 450 at 1.13 GHz (990 W, the power limit the only reason; a library product of the
+// same operands with a scale for each 32: 404).  What it took to get there, and what a change should not lose: the issuing warp
+// runs converged and walks uniform values (a branch on the lane number cost 40 %), the scales arrive a quad ahead, and only
+// hand-overs of memory between the blocks pay for cluster scope.
 //
 // fp8_split_kernel, for products of few tiles (serving, small heads): see there.
 //

@@ -3,10 +3,11 @@
 //   y[m, n] = alpha * sum_k  A[m, k] 2^(sa[m', k/128] - 127)  B[n, k] 2^(sb[n', k/128] - 127)  + bias[n]
 //
 // with m' = m or m / 128 (one scale for a row's block, or for a 128 x 128 block), n' likewise; the sum in the tensor core's 24-bit
-// accumulator, which cuts instead of rounding (what that costs, and what is done about it: SUMS below), one rounding at the end.  The scales are applied by the tensor core itself: tcgen05.mma
-// kind::mxf8f6f4.block_scale takes one exponent byte per row and 32 steps of the reduction from tensor memory, and four
-// consecutive instructions read the same byte.  So the product runs at the rate of an unscaled 8-bit product; promoting
-// every 128-step partial sum through registers instead would cost a read of the accumulator per 128 steps.
+// accumulator, which cuts instead of rounding (what that costs, and what is done about it: SUMS below), one rounding at the end.
+// The scales are applied by the tensor core itself: tcgen05.mma kind::mxf8f6f4.block_scale takes one exponent byte per row and
+// 32 steps of the reduction from tensor memory, and four consecutive instructions read the same byte.  So the product runs at the
+// rate of an unscaled 8-bit product; promoting every 128-step partial sum through registers instead would cost a read of the
+// accumulator per 128 steps.
 //
 // fp8_gemm_kernel, for products of many tiles: one block of threads per SM (CG = 1), or two blocks on two SMs that work on
 // one tile of 256 rows (CG = 2), walk over the output tiles:
@@ -22,11 +23,12 @@
 // Two accumulators let the epilogue of a tile run under the MMAs of the next; where two of 256 columns and the scales do
 // not fit the 512 columns of tensor memory, they share 24 columns, which the epilogue reads first.  Why pairs: each block of
 // a pair holds its own 128 rows of A and half the rows of B and the tensor core reads both halves, so a slice of a 256 x 256
-// tile costs each SM 32 KB from L2 instead of the 48 KB of a 128 x 256 tile.  What bounds it: the
-// tensor core, at the clock that the power limit leaves.  8192^3: 541 clocks for a slice of a 256 x 256 tile, first loads and last
-// results included, where the tensor core's nominal rate is 512.  One call by itself 353 us (3.1 PFLOP/s) at 1.39 GHz, the fifth
-// in a row 400 at 1.30, four seconds of them 450 at 1.13 GHz (990 W, the power limit the only reason; a library product of the
-// same operands with a scale for each 32: 404).  What it took to get there, and what a change should not lose: the issuing warp
+// tile costs each SM 32 KB from L2 instead of the 48 KB of a 128 x 256 tile.
+//
+// What bounds it: the tensor core, at the clock that the power limit leaves.  8192^3: 541 clocks for a slice of a 256 x 256 tile,
+// first loads and last results included, where the tensor core's nominal rate is 512.  One call by itself 353 us (3.1 PFLOP/s) at
+// 1.39 GHz, the fifth in a row 400 at 1.30, four seconds of them 450 at 1.13 GHz (990 W, the power limit the only reason; a library
+// product of the same operands with a scale for each 32: 404).  What it took to get there, and what a change should not lose: the issuing warp
 // runs converged and walks uniform values (a branch on the lane number cost 40 %), the scales arrive a quad ahead, and only
 // hand-overs of memory between the blocks pay for cluster scope.
 //
@@ -308,8 +310,8 @@ __device__ __forceinline__ void f8_tile(int t, int mt, int nt, int& tm, int& tn)
     tm = g * kF8Group + (in - tn * rows);
 }
 
-// NaN for what an epilogue warp still had to write when it gave up: its part of the tiles t, t + step, ...  Out of line, for the
-// loop's sake (inside it: 0.3 to 0.6 us of 5 to 14 us of a small product).
+// NaN for what an epilogue warp still had to write when it gave up: its part of the tiles t, t + step, ...  Out of line: the
+// loop need not carry it.
 template <class T, bool SUMS>
 __device__ __noinline__ void f8_blank(const Fp8Params& p, int t, int step, int cg, int rank)
 {
